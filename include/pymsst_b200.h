@@ -637,6 +637,93 @@ PMB_API int pmb_stft_frames_forward(const float* x, const float* window, float* 
 PMB_API int pmb_stft_frames_backward(const float* grad_frames, const float* window, float* grad_x, int64_t batch,
                                      int64_t length, int64_t n_fft, int64_t hop, int64_t frames, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Dropout from counter-based random bits: no mask is stored, the backward
+ * draws it again.  `key` is a device pointer to two int64 (seed, step); `site`
+ * tells apart the places that share a key; `threshold` = round(65536 p) in
+ * [0, 65536] (0: nothing is dropped and key may be NULL; 65536: everything).
+ * The 16 random bits of element e (row-major index) come from Philox4x32
+ * with seven rounds (Salmon et al., SC 2011), key words (seed low, seed high
+ * ^ site), counter words (low, high of e / 8, 2^32 - 1, step low): word
+ * (e % 8) / 2, low half when e is even.  Elements whose bits are below
+ * threshold are dropped, the others multiplied by c = 65536 / (65536 -
+ * threshold).  Computed in fp32, rounded once; dropped elements are exact
+ * zeros whatever x holds.
+ *   pmb_dropout_next_key       key = state, then state's step + 1 (both
+ *                              int64[2]): one key per forward, also in a
+ *                              captured graph, where each replay moves on
+ *   pmb_dropout                y = drop(x), or residual + drop(x); with x the
+ *                              gradient of y and no residual it is the
+ *                              backward
+ *   pmb_gelu_dropout_forward   y = drop(gelu(x)) (exact erf form)
+ *   pmb_gelu_dropout_backward  grad_x = drop(grad_out) gelu'(x)
+ * Replaces nn.Dropout and nn.GELU + nn.Dropout of pymss-core's Attention and
+ * FeedForward (the reference trains them unchanged,
+ * src/pymsst/training/module.py:221-224). */
+PMB_API int pmb_dropout_next_key(int64_t* state, int64_t* key, void* stream);
+PMB_API int pmb_dropout(const void* x, const void* residual, void* y, int64_t n, int threshold, const int64_t* key,
+                        uint32_t site, int dtype, void* stream);
+PMB_API int pmb_gelu_dropout_forward(const void* x, void* y, int64_t n, int threshold, const int64_t* key,
+                                     uint32_t site, int dtype, void* stream);
+PMB_API int pmb_gelu_dropout_backward(const void* grad_out, const void* x, void* grad_x, int64_t n, int threshold,
+                                      const int64_t* key, uint32_t site, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Attention of nq queries over nk keys of another length: O = (keep c
+ * softmax(scale Q K^T over keys < key_lengths[b])) V per (batch, head), head
+ * dims 1 to 256, heads a multiple of kv_heads (query head h reads key / value
+ * head h / (heads / kv_heads)).  q, o, grad_out, grad_q are [batch, nq,
+ * heads, dim] planes, k, v, grad_k, grad_v [batch, nk, kv_heads, dim], each
+ * given by a base pointer and three element strides (batch, position, head)
+ * with the head elements contiguous; `strides` holds them plane by plane
+ * (forward: q, k, v, o = 12 values; backward: q, k, v, o, grad_out, grad_q,
+ * grad_k, grad_v = 24 values).  key_lengths: device int32 [batch], clamped to
+ * [0, nk], or NULL (every key).  Keys at or behind the length never reach a
+ * result, whatever they hold, and get zero gradients.  A row without keys has
+ * O = 0 and no gradient.  lse: fp32 [batch * heads * nq], natural-log row
+ * sums (-inf without keys), written by the forward, read by the backward.
+ * Dropout on the probabilities as above (threshold, key, site), the bits of
+ * (batch * heads + head, query, key) taken from the group of keys key / 8:
+ * counter words (key / 8, query, batch * heads + head, step low), element
+ * key % 8.  Both passes are deterministic.  `workspace` holds the byte counts
+ * the *_workspace_size functions give (16-byte aligned).
+ * Covers scaled_dot_product_attention with dropout in pymss-core's Attention
+ * (src/pymsst/training/module.py:96-107) and key lengths beyond it. */
+PMB_API int64_t pmb_cross_attention_forward_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads, int64_t nq,
+                                                           int64_t nk, int64_t dim, int dtype);
+PMB_API int pmb_cross_attention_forward(const void* q, const void* k, const void* v, void* o, float* lse,
+                                        const int32_t* key_lengths, int64_t batch, int64_t heads, int64_t kv_heads,
+                                        int64_t nq, int64_t nk, int64_t dim, const int64_t* strides, float scale,
+                                        int threshold, const int64_t* key, uint32_t site, int dtype, void* workspace,
+                                        int64_t workspace_bytes, void* stream);
+PMB_API int64_t pmb_cross_attention_backward_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads,
+                                                            int64_t nq, int64_t nk, int64_t dim, int dtype);
+PMB_API int pmb_cross_attention_backward(const void* q, const void* k, const void* v, const void* o,
+                                         const void* grad_out, const float* lse, void* grad_q, void* grad_k,
+                                         void* grad_v, const int32_t* key_lengths, int64_t batch, int64_t heads,
+                                         int64_t kv_heads, int64_t nq, int64_t nk, int64_t dim,
+                                         const int64_t* strides, float scale, int threshold, const int64_t* key,
+                                         uint32_t site, int dtype, void* workspace, int64_t workspace_bytes,
+                                         void* stream);
+
+/* ------------------------------------------------------------------------
+ * Rotary embedding of tokens with several positions (frame, band, channel):
+ * interleaved pair p of a head belongs to the axis whose section holds p
+ * (sections: host array of `axes` pair counts, 1 to 4 axes), angle =
+ * positions[b, token, axis] * freqs[p], (e, o) -> (e cos - o sin, o cos + e
+ * sin), or the opposite angle with `inverse` (the backward); pairs behind the
+ * sections are copied.  x, y: [batch, tokens, heads, dim] views, three
+ * element strides (batch, token, head) each in `strides` (6 values, even),
+ * head elements contiguous, dim even.  positions [batch, tokens, axes] with
+ * position_batch_stride elements between batch items (0: shared), of type 0 =
+ * int32, 1 = int64, 2 = float32; freqs fp32.  The angle is formed and reduced
+ * in fp64.  The one-axis form is pmb_rotary_forward
+ * (src/pymsst/training/cuda/fused_band_split.cu:1077-1128). */
+PMB_API int pmb_rotary_axes(const void* x, const void* positions, const float* freqs, void* y, int64_t batch,
+                            int64_t tokens, int64_t heads, int64_t dim, const int64_t* strides,
+                            int64_t position_batch_stride, int position_type, int axes, const int64_t* sections,
+                            int inverse, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

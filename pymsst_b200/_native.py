@@ -21,6 +21,7 @@ _DTYPE_CODES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i = ctypes.c_int
+_u32 = ctypes.c_uint32
 _f32 = ctypes.c_float
 _pp = ctypes.POINTER(ctypes.c_void_p)
 _pi64 = ctypes.POINTER(ctypes.c_int64)
@@ -107,6 +108,19 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "pmb_spectral_l1_backward": (_i, [_p, _p, _i64, _i64, _i64, _p, _p, _p]),
     "pmb_stft_frames_forward": (_i, [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "pmb_stft_frames_backward": (_i, [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
+    "pmb_dropout_next_key": (_i, [_p, _p, _p]),
+    "pmb_dropout": (_i, [_p, _p, _p, _i64, _i, _p, _u32, _i, _p]),
+    "pmb_gelu_dropout_forward": (_i, [_p, _p, _i64, _i, _p, _u32, _i, _p]),
+    "pmb_gelu_dropout_backward": (_i, [_p, _p, _p, _i64, _i, _p, _u32, _i, _p]),
+    "pmb_cross_attention_forward_workspace_size": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i]),
+    "pmb_cross_attention_forward": (
+        _i, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _pi64, _f32, _i, _p, _u32, _i, _p, _i64,
+             _p]),
+    "pmb_cross_attention_backward_workspace_size": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i]),
+    "pmb_cross_attention_backward": (
+        _i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _pi64, _f32, _i, _p, _u32,
+             _i, _p, _i64, _p]),
+    "pmb_rotary_axes": (_i, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _pi64, _i64, _i, _i, _pi64, _i, _i, _p]),
 }
 
 

@@ -1,0 +1,153 @@
+// Dropout from counter-based random bits (philox.cuh), elementwise:
+//   y  = keep ? c x : 0                    (also its own backward on gy)
+//   y  = residual + (keep ? c x : 0)       the sum behind a projection
+//   y  = keep ? c gelu(x) : 0              the feed-forward's activation
+//   gx = keep ? c gy gelu'(x) : 0
+// c = 1 / (keep probability).  A dropped element is a select, so an infinity
+// or NaN under the mask does not reach y.  Computed in fp32 and rounded once.
+//
+// One thread takes groups of eight consecutive elements: one Philox call, and
+// for 16-bit types one 16-byte vector per tensor.  Bound by HBM: nothing but
+// the tensors themselves moves (a stored mask would add a byte per element to
+// both passes).  The loads of kUnroll groups are issued before the first
+// call's rounds, so the integer work runs while they are in flight.
+#include "common.cuh"
+#include "gelu.cuh"
+#include "philox.cuh"
+
+namespace pmb {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kUnroll = 4;
+
+enum Mode { kPlain = 0, kResidual = 1, kGelu = 2, kGeluGrad = 3 };
+
+template <typename T>
+struct alignas(16) Pack8 {
+  T v[8];
+};
+
+template <typename T, int MODE>
+__device__ __forceinline__ float value(float a, float b, bool keep, float c) {
+  if (MODE == kPlain) return keep ? a * c : 0.f;
+  if (MODE == kResidual) return keep ? fmaf(a, c, b) : b;
+  if (MODE == kGelu) return keep ? gelu_of<T>(a) * c : 0.f;
+  return keep ? b * gelu_grad_of<T>(a) * c : 0.f;  // a = x, b = gy
+}
+
+template <typename T, int MODE, bool DROP, bool VEC>
+__global__ void __launch_bounds__(kThreads)
+    dropout_kernel(const T* __restrict__ a, const T* __restrict__ b, T* __restrict__ y, int64_t n, DropArgs drop) {
+  constexpr bool kTwo = MODE == kResidual || MODE == kGeluGrad;
+  const int64_t stride = (int64_t)gridDim.x * kThreads;
+  const int64_t groups = (n + 7) / 8, full = VEC ? n / 8 : 0;
+  const Philox rng = DROP ? Philox(drop) : Philox(DropArgs{nullptr, 0, 0, 0.f});
+  for (int64_t g0 = (int64_t)blockIdx.x * kThreads + threadIdx.x; g0 < groups; g0 += stride * kUnroll) {
+    Pack8<T> pa[kUnroll], pb[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t g = g0 + u * stride;
+      if (g < full) {
+        pa[u] = reinterpret_cast<const Pack8<T>*>(a)[g];
+        if (kTwo) pb[u] = reinterpret_cast<const Pack8<T>*>(b)[g];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int64_t i = g * 8 + e;
+          pa[u].v[e] = i < n ? a[i] : Elem<T>::from_f(0.f);
+          if (kTwo) pb[u].v[e] = i < n ? b[i] : Elem<T>::from_f(0.f);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t g = g0 + u * stride;
+      if (g >= groups) break;
+      uint32_t keep = 0xffu;
+      if (DROP) keep = keep_bits(rng((uint32_t)g, (uint32_t)((uint64_t)g >> 32), 0xffffffffu), drop.limit);
+      Pack8<T> out;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        out.v[e] = Elem<T>::from_f(value<T, MODE>(Elem<T>::to_f(pa[u].v[e]), kTwo ? Elem<T>::to_f(pb[u].v[e]) : 0.f,
+                                                  (keep >> e) & 1u, DROP ? drop.scale : 1.f));
+      if (g < full) {
+        reinterpret_cast<Pack8<T>*>(y)[g] = out;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (g * 8 + e < n) y[g * 8 + e] = out.v[e];
+      }
+    }
+  }
+}
+
+template <typename T, int MODE>
+int launch(const void* a, const void* b, void* y, int64_t n, int threshold, const DropArgs& drop, cudaStream_t s,
+           const char* name) {
+  const bool vec = ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) |
+                     reinterpret_cast<uintptr_t>(y)) & 15) == 0;
+  int64_t grid = ((n + 7) / 8 + kThreads - 1) / kThreads;
+  const int64_t cap = (int64_t)num_sms() * 8;
+  if (grid > cap) grid = cap;
+  auto kernel = threshold > 0 ? (vec ? dropout_kernel<T, MODE, true, true> : dropout_kernel<T, MODE, true, false>)
+                              : (vec ? dropout_kernel<T, MODE, false, true> : dropout_kernel<T, MODE, false, false>);
+  kernel<<<(unsigned)grid, kThreads, 0, s>>>(static_cast<const T*>(a), static_cast<const T*>(b), static_cast<T*>(y), n,
+                                             drop);
+  PMB_CHECK_LAUNCH(name);
+  return PMB_OK;
+}
+
+template <int MODE>
+int entry(const void* a, const void* b, void* y, int64_t n, int threshold, const int64_t* key, uint32_t site,
+          int dtype, void* stream, const char* name) {
+  PMB_REQUIRE(n >= 0, "%s: bad size", name);
+  PMB_REQUIRE(threshold >= 0 && threshold <= 65536, "%s: drop threshold %d outside [0, 65536]", name, threshold);
+  if (n == 0) return PMB_OK;
+  PMB_REQUIRE(a && y && (b || MODE == kPlain || MODE == kGelu), "%s: NULL tensor argument", name);
+  PMB_REQUIRE(key || threshold == 0, "%s: NULL key", name);
+  const DropArgs drop = drop_args(key, site, threshold);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return PMB_DISPATCH(dtype, T, name, [&] { return launch<T, MODE>(a, b, y, n, threshold, drop, s, name); });
+}
+
+// out = state, then the state's step moves on: what one forward's dropout sites share.
+__global__ void next_key_kernel(int64_t* state, int64_t* out) {
+  out[0] = state[0];
+  out[1] = state[1];
+  state[1] = state[1] + 1;
+}
+
+}  // namespace
+}  // namespace pmb
+
+using namespace pmb;
+
+extern "C" int pmb_dropout_next_key(int64_t* state, int64_t* key, void* stream) {
+  clear_error();
+  const char* name = "pmb_dropout_next_key";
+  PMB_REQUIRE(state && key, "%s: NULL argument", name);
+  next_key_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(state, key);
+  PMB_CHECK_LAUNCH(name);
+  return PMB_OK;
+}
+
+extern "C" int pmb_dropout(const void* x, const void* residual, void* y, int64_t n, int threshold, const int64_t* key,
+                           uint32_t site, int dtype, void* stream) {
+  clear_error();
+  const char* name = "pmb_dropout";
+  return residual ? entry<kResidual>(x, residual, y, n, threshold, key, site, dtype, stream, name)
+                  : entry<kPlain>(x, nullptr, y, n, threshold, key, site, dtype, stream, name);
+}
+
+extern "C" int pmb_gelu_dropout_forward(const void* x, void* y, int64_t n, int threshold, const int64_t* key,
+                                        uint32_t site, int dtype, void* stream) {
+  clear_error();
+  return entry<kGelu>(x, nullptr, y, n, threshold, key, site, dtype, stream, "pmb_gelu_dropout_forward");
+}
+
+extern "C" int pmb_gelu_dropout_backward(const void* grad_out, const void* x, void* grad_x, int64_t n, int threshold,
+                                         const int64_t* key, uint32_t site, int dtype, void* stream) {
+  clear_error();
+  return entry<kGeluGrad>(x, grad_out, grad_x, n, threshold, key, site, dtype, stream, "pmb_gelu_dropout_backward");
+}
