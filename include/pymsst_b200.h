@@ -680,8 +680,13 @@ PMB_API int pmb_gelu_dropout_backward(const void* grad_out, const void* x, void*
  * grad_k, grad_v = 24 values).  key_lengths: device int32 [batch], clamped to
  * [0, nk], or NULL (every key).  Keys at or behind the length never reach a
  * result, whatever they hold, and get zero gradients.  A row without keys has
- * O = 0 and no gradient.  lse: fp32 [batch * heads * nq], natural-log row
- * sums (-inf without keys), written by the forward, read by the backward.
+ * O = 0 and no gradient.  lse: fp32, pmb_cross_attention_lse_size(batch,
+ * heads, nq) values, 16-byte aligned: row statistics that the forward writes
+ * for the backward of the same call (their order and base are its own).
+ * 16-bit types with head dims that are multiples of 8 up to 128 and scale >=
+ * 0 run on the tensor cores; their planes must be 16-byte aligned with
+ * positive strides that are multiples of 8 (strides of extents of 1 are not
+ * looked at).
  * Dropout on the probabilities as above (threshold, key, site), the bits of
  * (batch * heads + head, query, key) taken from the group of keys key / 8:
  * counter words (key / 8, query, batch * heads + head, step low), element
@@ -689,6 +694,7 @@ PMB_API int pmb_gelu_dropout_backward(const void* grad_out, const void* x, void*
  * the *_workspace_size functions give (16-byte aligned).
  * Covers scaled_dot_product_attention with dropout in pymss-core's Attention
  * (src/pymsst/training/module.py:96-107) and key lengths beyond it. */
+PMB_API int64_t pmb_cross_attention_lse_size(int64_t batch, int64_t heads, int64_t nq);
 PMB_API int64_t pmb_cross_attention_forward_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads, int64_t nq,
                                                            int64_t nk, int64_t dim, int dtype);
 PMB_API int pmb_cross_attention_forward(const void* q, const void* k, const void* v, void* o, float* lse,

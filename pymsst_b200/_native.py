@@ -112,6 +112,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "pmb_dropout": (_i, [_p, _p, _p, _i64, _i, _p, _u32, _i, _p]),
     "pmb_gelu_dropout_forward": (_i, [_p, _p, _i64, _i, _p, _u32, _i, _p]),
     "pmb_gelu_dropout_backward": (_i, [_p, _p, _p, _i64, _i, _p, _u32, _i, _p]),
+    "pmb_cross_attention_lse_size": (_i64, [_i64, _i64, _i64]),
     "pmb_cross_attention_forward_workspace_size": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i]),
     "pmb_cross_attention_forward": (
         _i, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _pi64, _f32, _i, _p, _u32, _i, _p, _i64,

@@ -25,11 +25,22 @@ def _plane_empty(b, h, n, d, dtype, device) -> torch.Tensor:
     return torch.empty(b, n, h, d, dtype=dtype, device=device).transpose(1, 2)
 
 
+def _copy_plane(t: torch.Tensor) -> torch.Tensor:
+    """A copy of t [b, h, n, d], always a new one, as a view of a [b, n, h, d] plane."""
+    return t.transpose(1, 2).clone(memory_format=torch.contiguous_format).transpose(1, 2)
+
+
 def _plane(t: torch.Tensor) -> torch.Tensor:
-    """t itself when its head elements are contiguous, else a copy in a [b, n, h, d] plane."""
-    if t.stride(-1) != 1 and t.shape[-1] != 1:
-        t = t.transpose(1, 2).contiguous().transpose(1, 2)
-    return t
+    """t itself when the kernels read it in place, else a copy in a [b, n, h, d] plane.  They need contiguous head
+    elements and, for the tensor cores (16-bit types, head dims in multiples of 8), 16-byte aligned rows at positive
+    strides; the stride of a dimension of one does not count."""
+    b, h, n, d = t.shape
+    sb, sh, sn, sd = t.stride()
+    ok = sd == 1 or d == 1
+    if ok and t.element_size() == 2 and d % 8 == 0:
+        ok = (t.data_ptr() % 16 == 0 and (b < 2 or (sb > 0 and sb % 8 == 0)) and (h < 2 or (sh > 0 and sh % 8 == 0))
+              and (n < 2 or (sn > 0 and sn % 8 == 0)))
+    return t if ok else _copy_plane(t)
 
 
 def _strides(*planes: torch.Tensor):
@@ -46,9 +57,10 @@ def _attention_forward(q, k, v, lengths, scale, threshold, key, site):
     hk, nk = k.shape[1], k.shape[2]
     device = q.device
     o = _plane_empty(b, hq, nq, d, q.dtype, device)
-    lse = torch.empty(b * hq * nq, dtype=torch.float32, device=device)
     code = nat.dtype_code(q.dtype)
-    ws_bytes = int(nat.library().pmb_cross_attention_forward_workspace_size(b, hq, hk, nq, nk, d, code))
+    lib = nat.library()
+    lse = torch.empty(lib.pmb_cross_attention_lse_size(b, hq, nq), dtype=torch.float32, device=device)
+    ws_bytes = lib.pmb_cross_attention_forward_workspace_size(b, hq, hk, nq, nk, d, code)
     ws = nat.workspace(ws_bytes, device) if ws_bytes else None
     with on_device(device):
         nat.call(
@@ -146,7 +158,7 @@ def _pair_view(t: torch.Tensor) -> torch.Tensor:
     """t itself when pairs of head elements can be read whole, else a copy in a [b, n, h, d] plane."""
     strides = [s for s, size in zip(t.stride()[:3], t.shape[:3]) if size > 1]
     if t.stride(-1) != 1 or any(s % 2 for s in strides) or t.data_ptr() % (2 * t.element_size()):
-        t = t.transpose(1, 2).contiguous().transpose(1, 2)
+        t = _copy_plane(t)
     return t
 
 

@@ -42,6 +42,7 @@
 // the default scale 1/sqrt(64), as called by the BS-/Mel-RoFormer Attention
 // module of pymss-core (the attention backend the reference selects with
 // cuda_attention_backend, src/pymsst/training/module.py:96-107).
+#include "attention_tiles.cuh"
 #include "tma.cuh"
 #include "umma.cuh"
 
@@ -57,39 +58,10 @@ constexpr int kThreads = 192;   // TMA warp, MMA warp, 4 row warps
 constexpr int TILE128 = BM * kD * 2;  // 16 KB: 128 rows x 64 16-bit
 constexpr int TILE64 = BN * kD * 2;   // 8 KB
 constexpr uint32_t kTmemCols = 256;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 struct Plane {
   int64_t s_b, s_n, s_h;  // element strides of a [sequences, N, H, 64] plane
 };
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&v);
-  } else {
-    __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&v);
-  }
-}
-
-// Byte offset of 16-byte chunk ch (elements 8ch..8ch+7) of row r in a
-// 128-byte-swizzled K-major tile of 64-element rows.
-__device__ __forceinline__ uint32_t sw128(int r, int ch) {
-  return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((ch ^ (r & 7)) << 4));
-}
-
-// 32 fp32 values -> chunks [c0, c0 + 4) of row r of a 16-bit SW128 tile
-template <typename T>
-__device__ __forceinline__ void put_row32(uint8_t* tile, int r, int c0, const float (&v)[32]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    *reinterpret_cast<uint4*>(tile + sw128(r, c0 + i)) =
-        make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
-                   pack2<T>(v[8 * i + 4], v[8 * i + 5]), pack2<T>(v[8 * i + 6], v[8 * i + 7]));
-}
 
 // 64 fp32 values (times mul) -> one 128-byte row of a global plane
 template <typename T>
@@ -126,19 +98,6 @@ struct Idesc {
   static constexpr uint32_t K = umma::idesc_f16(kBf16, false, false, BM, BN);  // B K-major, N = 64 rows
   static constexpr uint32_t MN = umma::idesc_f16(kBf16, false, true, BM, kD);  // B MN-major, N = head dim
 };
-
-__device__ __forceinline__ uint8_t* align1024(uint8_t* p) {
-  return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~uintptr_t(1023));
-}
-
-// Arrive once per row warp on `bar` after this thread's shared / tensor
-// memory accesses (count 4 barriers).
-__device__ __forceinline__ void warp_arrive(uint64_t* bar, bool wrote_smem) {
-  if (wrote_smem) umma::fence_proxy_async_smem();
-  umma::tc_fence_before();
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0) umma::mbar_arrive(bar);
-}
 
 struct Item {
   int bh, blk, b, h;
@@ -393,37 +352,6 @@ __global__ void __launch_bounds__(kThreads, 2)
 constexpr int kRowWarpsBwd = 8;
 constexpr int kBwdThreads = 64 + 32 * kRowWarpsBwd;
 
-// 32 columns of this warp's TMEM lane quarter, without waiting: the values
-// are valid after tmem_wait(), which also orders their uses after the wait.
-__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-
-// Register dependency on all 32 values (an empty statement the compiler
-// cannot move the values' uses ahead of).
-__device__ __forceinline__ void tie32(uint32_t (&r)[32]) {
-  asm volatile(""
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                 "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
-                 "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
-                 "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
-}
-
-// Wait for this thread's outstanding tcgen05.ld and tie both arrays after it.
-__device__ __forceinline__ void tmem_wait2(uint32_t (&a)[32], uint32_t (&b)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-  tie32(a);
-  tie32(b);
-}
-
 // 32 fp32 values (times mul) -> 64 bytes of a global row
 template <typename T>
 __device__ __forceinline__ void store_row32(T* dst, const uint32_t (&a)[32], float mul) {
@@ -463,39 +391,6 @@ __device__ __forceinline__ void unrotate32(uint32_t (&a)[32], const float* __res
       a[e_i + 1] = __float_as_uint(fmaf(o, cc[j], -e * ss[j]));
     }
   }
-}
-
-// 16 columns of this warp's TMEM lane quarter, without waiting (see tmem_wait16).
-__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-
-__device__ __forceinline__ void tie16(uint32_t (&r)[16]) {
-  asm volatile(""
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                 "+r"(r[15]));
-}
-
-__device__ __forceinline__ void tmem_wait16(uint32_t (&a)[16], uint32_t (&b)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-  tie16(a);
-  tie16(b);
-}
-
-// 16 fp32 values -> chunks c0, c0 + 1 of row r of a 16-bit SW128 tile
-template <typename T>
-__device__ __forceinline__ void put_row16(uint8_t* tile, int r, int c0, const float* v) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    *reinterpret_cast<uint4*>(tile + sw128(r, c0 + i)) =
-        make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
-                   pack2<T>(v[8 * i + 4], v[8 * i + 5]), pack2<T>(v[8 * i + 6], v[8 * i + 7]));
 }
 
 // D[tmem] (+)= A * B^T over K = 16 * ksteps: A a 128-row K-major SW128 tile

@@ -10,35 +10,22 @@
 // O = 0, lse = -inf and no gradient; keys at or behind `len` are never read,
 // and their gradients are zeros.
 //
-// One warp per query row (forward, dQ) or key row (dK / dV), all arithmetic
-// fp32; every output row is written by one warp, so results do not depend on
-// the order of execution.
-#include "common.cuh"
-#include "philox.cuh"
+// The C entries, and the row form: one warp per query row (forward, dQ) or
+// key row (dK / dV), all arithmetic fp32; every output row is written by one
+// warp, so results do not depend on the order of execution.  It serves fp32
+// and head dims the tensor-core form (cross_attention_tc.cu) does not take.
+#include "cross_attention.cuh"
 
 namespace pmb {
 namespace {
+
+using xattn::Plane;
+using xattn::Shape;
 
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxDim = 256;
 constexpr int kAcc = kMaxDim / 32;
-
-struct Plane {
-  int64_t s_b, s_n, s_h;  // element strides, the head elements contiguous
-};
-
-struct Shape {
-  int batch, heads, kv_heads, nq, nk, dim;
-  const int32_t* lengths;  // keys of each batch item, or NULL: nk
-  float scale;
-
-  __device__ __forceinline__ int keys(int b) const {
-    if (lengths == nullptr) return nk;
-    const int n = __ldg(lengths + b);
-    return n < 0 ? 0 : (n < nk ? n : nk);
-  }
-};
 
 // sum_c a[c] * row[c] with a in shared memory
 template <typename T>
@@ -246,10 +233,26 @@ int64_t delta_bytes(int64_t rows) { return (rows * 4 + 255) / 256 * 256; }
 
 using namespace pmb;
 
+extern "C" int64_t pmb_cross_attention_lse_size(int64_t batch, int64_t heads, int64_t nq) {
+  return batch > 0 && heads > 0 && nq > 0 ? xattn::tc_lse_floats(batch * heads, nq) : 0;
+}
+
+namespace pmb {
+namespace {
+// Shape of a workspace query; false where the sizes make no call.
+bool query_shape(Shape& sh, int64_t batch, int64_t heads, int64_t kv_heads, int64_t nq, int64_t nk, int64_t dim) {
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || nq <= 0 || nk < 0 || dim <= 0) return false;
+  sh = Shape{(int)batch, (int)heads, (int)kv_heads, (int)nq, (int)nk, (int)dim, nullptr, 1.f};
+  return true;
+}
+}  // namespace
+}  // namespace pmb
+
 extern "C" int64_t pmb_cross_attention_forward_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads,
                                                               int64_t nq, int64_t nk, int64_t dim, int dtype) {
-  (void)batch, (void)heads, (void)kv_heads, (void)nq, (void)nk, (void)dim, (void)dtype;
-  return 0;
+  Shape sh;
+  if (!query_shape(sh, batch, heads, kv_heads, nq, nk, dim) || !xattn::tc_takes(sh, dtype)) return 0;
+  return xattn::tc_forward_workspace(sh);
 }
 
 extern "C" int pmb_cross_attention_forward(const void* q, const void* k, const void* v, void* o, float* lse,
@@ -266,14 +269,19 @@ extern "C" int pmb_cross_attention_forward(const void* q, const void* k, const v
   PMB_REQUIRE(q && o && lse && strides && ((k && v) || nk == 0), "%s: NULL argument", name);
   const DropArgs drop = drop_args(key, site, threshold);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const Plane pq = plane_at(strides, 0), pk = plane_at(strides, 1), pv = plane_at(strides, 2),
+              po = plane_at(strides, 3);
+  if (xattn::tc_takes(sh, dtype))
+    return xattn::tc_forward(sh,
+                             xattn::Forward{q, k, v, o, lse, pq, pk, pv, po, dtype, threshold, drop, workspace,
+                                            workspace_bytes, s},
+                             name);
   unsigned grid;
   if (int st = row_grid(rows, grid, name)) return st;
-  (void)workspace, (void)workspace_bytes;
   return PMB_DISPATCH(dtype, T, name, [&] {
     auto kernel = threshold > 0 ? attn_rows_fwd<T, true> : attn_rows_fwd<T, false>;
     kernel<<<grid, kThreads, 0, s>>>(static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
-                                     static_cast<T*>(o), lse, plane_at(strides, 0), plane_at(strides, 1),
-                                     plane_at(strides, 2), plane_at(strides, 3), sh, drop);
+                                     static_cast<T*>(o), lse, pq, pk, pv, po, sh, drop);
     PMB_CHECK_LAUNCH(name);
     return PMB_OK;
   });
@@ -281,8 +289,9 @@ extern "C" int pmb_cross_attention_forward(const void* q, const void* k, const v
 
 extern "C" int64_t pmb_cross_attention_backward_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads,
                                                                int64_t nq, int64_t nk, int64_t dim, int dtype) {
-  (void)kv_heads, (void)nk, (void)dim, (void)dtype;
-  return batch > 0 && heads > 0 && nq > 0 ? delta_bytes(batch * heads * nq) : 0;
+  Shape sh;
+  if (!query_shape(sh, batch, heads, kv_heads, nq, nk, dim)) return 0;
+  return xattn::tc_takes(sh, dtype) ? xattn::tc_backward_workspace(sh) : delta_bytes(batch * heads * nq);
 }
 
 extern "C" int pmb_cross_attention_backward(const void* q, const void* k, const void* v, const void* o,
@@ -312,6 +321,11 @@ extern "C" int pmb_cross_attention_backward(const void* q, const void* k, const 
               pgk = plane_at(strides, 6), pgv = plane_at(strides, 7);
   const DropArgs drop = drop_args(key, site, threshold);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (xattn::tc_takes(sh, dtype))
+    return xattn::tc_backward(sh,
+                              xattn::Backward{q, k, v, o, grad_out, lse, grad_q, grad_k, grad_v, pq, pk, pv, po, pgo,
+                                              pgq, pgk, pgv, dtype, threshold, drop, workspace, workspace_bytes, s},
+                              name);
   float* delta = static_cast<float*>(workspace);
   unsigned qgrid, kgrid;
   if (int st = row_grid(rows, qgrid, name)) return st;

@@ -1,0 +1,1392 @@
+// Cross attention on the tcgen05 tensor cores (16-bit types, head dims up to
+// 128 in multiples of 8); the formulas are at the top of cross_attention.cu.
+//
+// Rows.  Query heads that share a key / value head are packed: with gp the
+// largest power of two (up to 64) that divides the group, gp heads form a
+// unit and row R = position * gp + head of the unit, so a few queries of many
+// heads fill a tile and each key / value head is read once for all of them.
+// A 5-D TMA map (dim, gp, positions, units, batch) loads packed tiles as they
+// lie; rows behind the last are zeros.  Head dims below 64 (or between 64 and
+// 128) use the 64-wide tiles, the TMA filling the rest with zeros.
+//
+// All three kernels are persistent and warp-specialised: warp 0 feeds tiles
+// by TMA, one lane of warp 1 issues tcgen05.mma, the row warps own one tensor
+// memory lane per thread.  Waits are bounded (umma.cuh).  Nothing is summed
+// with atomics, so results do not depend on the order of execution.
+//
+// Keys at or behind a batch item's length are masked in the scores by a
+// select, and their value (forward) or key (dQ) rows are zeroed in shared
+// memory before the product that multiplies them by a zero weight, so NaN
+// there stays there.
+//
+// Row statistics are kept as base-2 logarithms (lse2 = max + log2(sum), of
+// scores times scale * log2 e); +inf for a row without keys, whose
+// probabilities then come out as 0.
+#include "attention_tiles.cuh"
+#include "cross_attention.cuh"
+#include "tma.cuh"
+#include "umma.cuh"
+
+namespace pmb {
+unsigned int timeout_flag_cross(int reset) { return umma::flag_reader(reset); }
+
+namespace xattn {
+namespace {
+
+constexpr int BM = 128;                // rows of a tile
+constexpr int TILE = BM * 128;         // bytes of 128 rows x 64 16-bit elements
+constexpr int kMaxSplits = 64;
+
+// What a kernel needs to find its tiles.
+struct Geometry {
+  int units, gp_shift, kv_units;       // units per batch item, log2 gp, units per key / value head
+  int rows, ldr, nblk;                 // packed rows per unit, their pitch in lse, row tiles per unit
+  int width, splits;                   // forward: keys per chunk, key ranges per row tile
+  int total;                           // work items
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// 16-bit instruction descriptors, fp32 accumulate, M = 128.
+template <typename T>
+struct Desc {
+  static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  // A, B K-major, N columns
+  __device__ __forceinline__ static uint32_t kk(int n) {
+    return umma::idesc_f16(kBf16, false, false, BM, 16) + ((uint32_t)((n - 16) >> 3) << 17);
+  }
+  static constexpr uint32_t MN = umma::idesc_f16(kBf16, false, true, BM, 64);  // B MN-major, 64 head elements
+};
+
+// D (+)= A B^T, A and B K-major: DC sub-tiles of 64 elements, strides a_sub / b_sub bytes apart.
+template <int DC>
+__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t a_sub, uint32_t b, uint32_t b_sub,
+                                           uint32_t idesc) {
+#pragma unroll
+  for (int dc = 0; dc < DC; ++dc)
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+      umma::mma_f16(d, umma::smem_desc_sw128(a + dc * a_sub + kk * 32, 16, 1024),
+                    umma::smem_desc_sw128(b + dc * b_sub + kk * 32, 16, 1024), idesc, (dc || kk) ? 1u : 0u);
+}
+
+// D (+)= A B with A K-major (64-element sub-tiles TILE bytes apart) and B MN-major: its rows are the K index, its 64
+// head elements the N index, DC sub-tiles b_sub bytes apart into accumulators 64 columns apart.
+template <int DC>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t b_sub, uint32_t idesc, int ksteps,
+                                         bool accumulate) {
+  for (int ks = 0; ks < ksteps; ++ks)
+#pragma unroll
+    for (int dc = 0; dc < DC; ++dc)
+      umma::mma_f16(d + dc * 64, umma::smem_desc_sw128(a + (ks >> 2) * TILE + (ks & 3) * 32, 16, 1024),
+                    umma::smem_desc_sw128(b + dc * b_sub + ks * 2048, 16, 1024), idesc, (accumulate || ks) ? 1u : 0u);
+}
+
+// Zero the 128-byte rows [first, rows) of DC sub-tiles, one row per thread.
+template <int DC>
+__device__ __forceinline__ void zero_rows(uint8_t* tile, uint32_t sub, int first, int rows, int thread) {
+  const int r = thread;
+  if (r < first || r >= rows) return;
+#pragma unroll
+  for (int dc = 0; dc < DC; ++dc)
+#pragma unroll
+    for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile + dc * sub + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+}
+
+// Keep bits of the 32 keys from `key` (a multiple of 8) on, of one query.
+__device__ __forceinline__ uint32_t keep_word(const Philox& rng, uint32_t limit, int key, int query, uint32_t bh) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w |= keep_bits(rng(((uint32_t)key >> 3) + i, (uint32_t)query, bh), limit) << (8 * i);
+  return w;
+}
+
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// ---------------------------------------------------------------- forward
+// Item = 128 packed rows of a unit, over one of `splits` key ranges.  Keys
+// come in chunks of `width` <= 96 (a multiple of 16 that divides the keys
+// evenly): S (two buffers of 96 columns) and O (64 columns per 64 head
+// elements) then fill 256 tensor memory columns, two CTAs fit an SM, and a
+// row thread holds its whole chunk of scores in registers.
+//
+// The MMA lane issues S of chunk c + 1 before O += P V of chunk c, so scores
+// are ready while the row warps work.  O stays in tensor memory; the running
+// maximum moves only when a row's grows by more than 8 (a factor 256 in P,
+// harmless in fp32 sums and 16-bit P), which after the first chunks is rare,
+// and then the row threads rescale O themselves.  P is rounded to the input
+// type (as in attention.cu); the row sums add the unrounded values before
+// dropout, whose scale is applied once at the end.
+//
+// K and V have separate rings: a K stage is free as soon as its scores are
+// formed.
+namespace fw {
+constexpr int kThreads = 192;
+constexpr int kMaxW = 96;
+constexpr int kStages = 2;
+constexpr int SUB = kMaxW * 128;  // one 64-element sub-tile of a K or V stage
+template <int DC>
+struct L {
+  static constexpr int OFF_K = DC * TILE;
+  static constexpr int OFF_V = OFF_K + kStages * DC * SUB;
+  static constexpr int OFF_P = OFF_V + kStages * DC * SUB;  // 128 rows x 96 keys: two sub-tiles
+  static constexpr int OFF_BAR = OFF_P + 2 * TILE;
+  static constexpr int SMEM = OFF_BAR + 256 + 1024;
+  static constexpr uint32_t kTmemO = 2 * kMaxW;
+  static constexpr uint32_t kCols = DC == 1 ? 256 : 512;
+};
+constexpr int kBars = 2 + 4 * kStages + 2 + 3;
+constexpr float kRescale = 8.f;
+}  // namespace fw
+
+struct Item {
+  int b, u, blk, split;
+};
+
+__device__ __forceinline__ Item forward_item(int item, const Geometry& g) {
+  Item it;
+  it.blk = item % g.nblk;
+  int r = item / g.nblk;
+  it.split = r % g.splits;
+  r /= g.splits;
+  it.u = r % g.units;
+  it.b = r / g.units;
+  return it;
+}
+
+// Chunks [c0, c1) of an item.
+__device__ __forceinline__ void chunk_range(int len, const Item& it, const Geometry& g, int& c0, int& c1) {
+  const int n = (len + g.width - 1) / g.width;
+  c0 = (int)((int64_t)n * it.split / g.splits);
+  c1 = (int)((int64_t)n * (it.split + 1) / g.splits);
+}
+
+template <typename T, int DC, bool DROP>
+__global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
+    xattn_fwd(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+              const __grid_constant__ CUtensorMap tmV, T* __restrict__ o, float* __restrict__ lse,
+              float* __restrict__ part_o, float* __restrict__ part_lse, Plane po, Shape sh, Geometry g,
+              DropArgs drop) {
+  using namespace fw;
+  using Y = L<DC>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Y::OFF_BAR);
+  uint64_t* q_full = bars;
+  uint64_t* q_empty = bars + 1;
+  uint64_t* k_full = bars + 2;
+  uint64_t* k_empty = k_full + kStages;
+  uint64_t* v_full = k_empty + kStages;
+  uint64_t* v_empty = v_full + kStages;
+  uint64_t* s_full = v_empty + kStages;  // [2]
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_done = p_full + 1;
+  uint64_t* o_empty = o_done + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
+  __shared__ int abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int gp_mask = (1 << g.gp_shift) - 1;
+  if (threadIdx.x == 0) {
+    umma::mbar_init(q_full, 1);
+    umma::mbar_init(q_empty, 1);
+    for (int s = 0; s < kStages; ++s) {
+      umma::mbar_init(&k_full[s], 1);
+      umma::mbar_init(&k_empty[s], 1);
+      umma::mbar_init(&v_full[s], 1);
+      umma::mbar_init(&v_empty[s], 1);
+    }
+    umma::mbar_init(&s_full[0], 1);
+    umma::mbar_init(&s_full[1], 1);
+    umma::mbar_init(p_full, 4);
+    umma::mbar_init(o_done, 1);
+    umma::mbar_init(o_empty, 4);
+    abort_flag = 0;
+    umma::fence_barrier_init();
+  }
+  if (warp == 0) umma::tmem_alloc(tmem_slot, Y::kCols);
+  umma::tc_fence_before();
+  __syncthreads();
+  umma::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {  // Q tiles
+      umma::tma_prefetch(&tmQ);
+      uint32_t t = 0;
+      for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
+        const Item it = forward_item(item, g);
+        int c0, c1;
+        chunk_range(sh.keys(it.b), it, g, c0, c1);
+        if (c0 >= c1) continue;
+        if (!umma::mbar_wait(q_empty, (t & 1) ^ 1, 0x91)) {
+          abort_flag = 1;
+          break;
+        }
+        umma::mbar_arrive_expect_tx(q_full, DC * TILE);
+#pragma unroll
+        for (int dc = 0; dc < DC; ++dc)
+          umma::tma_load_5d(smem + dc * TILE, &tmQ, q_full, dc * 64, 0, (it.blk * BM) >> g.gp_shift, it.u, it.b);
+        ++t;
+      }
+    } else if (lane <= 2) {  // K chunks (lane 1), V chunks (lane 2)
+      const CUtensorMap* map = lane == 1 ? &tmK : &tmV;
+      uint64_t* full = lane == 1 ? k_full : v_full;
+      uint64_t* empty = lane == 1 ? k_empty : v_empty;
+      uint8_t* ring = smem + (lane == 1 ? Y::OFF_K : Y::OFF_V);
+      umma::tma_prefetch(map);
+      uint32_t cc = 0;
+      for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
+        const Item it = forward_item(item, g);
+        int c0, c1;
+        chunk_range(sh.keys(it.b), it, g, c0, c1);
+        for (int c = c0; c < c1; ++c, ++cc) {
+          const int s = cc % kStages;
+          if (!umma::mbar_wait(&empty[s], ((cc / kStages) & 1) ^ 1, 0x92)) {
+            abort_flag = 1;
+            break;
+          }
+          umma::mbar_arrive_expect_tx(&full[s], DC * g.width * 128);
+#pragma unroll
+          for (int dc = 0; dc < DC; ++dc)
+            umma::tma_load_4d(ring + (s * DC + dc) * SUB, map, &full[s], dc * 64, c * g.width, it.u / g.kv_units,
+                              it.b);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // O += P V of the chunk issued last; first / number of an item decide the accumulator
+      struct Pending {
+        bool live, first;
+        int keys;
+        uint32_t t;
+      } prev{false, false, 0, 0};
+      uint32_t cc = 0, t = 0;
+      auto issue_o = [&](uint32_t c) -> bool {
+        const int s = c % kStages;
+        if (!umma::mbar_wait(p_full, c & 1, 0x94) || !umma::mbar_wait(&v_full[s], (c / kStages) & 1, 0x95)) return false;
+        if (prev.first && !umma::mbar_wait(o_empty, (prev.t & 1) ^ 1, 0x96)) return false;
+        umma::tc_fence_after();
+        mma_rows<DC>(tmem + Y::kTmemO, umma::smem_u32(smem + Y::OFF_P),
+                     umma::smem_u32(smem + Y::OFF_V + s * DC * SUB), SUB, Desc<T>::MN, (prev.keys + 15) >> 4,
+                     !prev.first);
+        umma::mma_commit(o_done);
+        umma::mma_commit(&v_empty[s]);
+        return true;
+      };
+      bool ok = true;
+      for (int item = blockIdx.x; item < g.total && ok && !abort_flag; item += gridDim.x) {
+        const Item it = forward_item(item, g);
+        const int len = sh.keys(it.b);
+        int c0, c1;
+        chunk_range(len, it, g, c0, c1);
+        if (c0 >= c1) continue;
+        if (!umma::mbar_wait(q_full, t & 1, 0x93)) {
+          ok = false;
+          break;
+        }
+        for (int c = c0; c < c1; ++c, ++cc) {
+          const int s = cc % kStages, keys = min(g.width, len - c * g.width);
+          if (!umma::mbar_wait(&k_full[s], (cc / kStages) & 1, 0x97)) {
+            ok = false;
+            break;
+          }
+          umma::tc_fence_after();
+          mma_scores<DC>(tmem + (cc & 1) * kMaxW, umma::smem_u32(smem), TILE,
+                         umma::smem_u32(smem + Y::OFF_K + s * DC * SUB), SUB, Desc<T>::kk((keys + 15) & ~15));
+          umma::mma_commit(&s_full[cc & 1]);
+          umma::mma_commit(&k_empty[s]);
+          if (c == c1 - 1) umma::mma_commit(q_empty);
+          if (prev.live && !issue_o(cc - 1)) {
+            ok = false;
+            break;
+          }
+          prev = Pending{true, c == c0, keys, t};
+        }
+        ++t;
+      }
+      if (ok && prev.live) ok = issue_o(cc - 1);
+      if (!ok) abort_flag = 1;
+    }
+  } else {
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const float sl2 = sh.scale * kLog2e;
+    const Philox rng = DROP ? Philox(drop) : Philox(DropArgs{nullptr, 0, 0, 0.f});
+    uint32_t cc = 0, t = 0;
+    for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
+      const Item it = forward_item(item, g);
+      const int len = sh.keys(it.b);
+      int c0, c1;
+      chunk_range(len, it, g, c0, c1);
+      const int R = it.blk * BM + row, pos = R >> g.gp_shift, head = (it.u << g.gp_shift) + (R & gp_mask);
+      const bool valid = R < g.rows;
+      const bool idle = it.blk * BM + quarter * 32 >= g.rows;  // no row of this warp exists
+      const int64_t stat = (int64_t)(it.b * g.units + it.u) * g.ldr + R;
+      const int64_t prow = ((int64_t)(it.b * g.units + it.u) * g.splits + it.split) * g.rows + R;
+      T* dst = o + it.b * po.s_b + pos * po.s_n + head * po.s_h;
+      if (c0 >= c1) {
+        if (valid) {
+          if (g.splits > 1) {
+            part_lse[prow] = -INFINITY;
+          } else {
+            for (int d = 0; d < sh.dim; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
+            lse[stat] = INFINITY;
+          }
+        }
+        continue;
+      }
+      const uint32_t bh = (uint32_t)(it.b * sh.heads + head);
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int c = c0; c < c1; ++c, ++cc) {
+        const int kc = c * g.width, keys = min(g.width, len - kc);
+        uint32_t keep[3];  // the chunk's dropout bits, drawn while its scores are formed
+        if (DROP && !idle) {
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            if (k * 32 < keys) keep[k] = keep_word(rng, drop.limit, kc + k * 32, pos, bh);
+          }
+        }
+        if (!umma::mbar_wait(&s_full[cc & 1], (cc >> 1) & 1, 0x98)) {
+          ok = false;
+          break;
+        }
+        umma::tc_fence_after();
+        uint32_t s[3][32];
+        if (!idle) {
+          const uint32_t src = tmem + lane_off + (cc & 1) * kMaxW;
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            if (k * 32 < keys) tmem_ld32_nowait(src + k * 32, s[k]);
+          }
+          wait_ld();
+#pragma unroll
+          for (int k = 0; k < 3; ++k) tie32(s[k]);
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            if (k * 32 + 32 <= keys) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(s[k][e]));
+            } else if (k * 32 < keys) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (k * 32 + e < keys) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(s[k][e]));
+            }
+          }
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
+          if (c == c0) {
+            m = mx;
+          } else {
+            const bool grows = mx > m + kRescale;
+            if (__any_sync(0xffffffffu, grows)) {
+              if (!umma::mbar_wait(o_done, (cc - 1) & 1, 0x99)) {
+                ok = false;
+                break;
+              }
+              umma::tc_fence_after();
+              const float mn = grows ? mx : m, f = grows ? ex2(m - mn) : 1.f;
+              l *= f;
+              m = mn;
+#pragma unroll
+              for (int k = 0; k < 2 * DC; ++k) {
+                uint32_t a[32];
+                tmem_ld32_nowait(tmem + lane_off + Y::kTmemO + k * 32, a);
+                wait_ld();
+                tie32(a);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(__uint_as_float(a[e]) * f);
+                umma::tmem_st32(tmem + lane_off + Y::kTmemO + k * 32, a);
+              }
+            }
+          }
+          float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            if (k * 32 < keys) {
+              const bool tail = k * 32 + 32 > keys;
+#pragma unroll
+              for (int gr = 0; gr < 4; ++gr) {
+                float p[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  p[e] = ex2(fmaf(__uint_as_float(s[k][gr * 8 + e]), sl2, -m));
+                  if (tail && k * 32 + gr * 8 + e >= keys) p[e] = 0.f;
+                  sum4[e & 3] += p[e];
+                }
+                if (DROP) {
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) p[e] = (keep[k] >> (gr * 8 + e)) & 1u ? p[e] : 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[k][gr * 4 + e] = pack2<T>(p[2 * e], p[2 * e + 1]);
+              }
+            }
+          }
+          l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+        }
+        // the product of the previous chunk has read P (and, of the previous item, its O has been read)
+        if (cc > 0 && !umma::mbar_wait(o_done, (cc - 1) & 1, 0x9a)) {
+          ok = false;
+          break;
+        }
+        if (!idle) {
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            if (k * 32 < keys) {
+              uint8_t* tile = smem + Y::OFF_P + (k >> 1) * TILE;
+#pragma unroll
+              for (int gr = 0; gr < 4; ++gr)
+                *reinterpret_cast<uint4*>(tile + sw128(row, (k & 1) * 4 + gr)) =
+                    make_uint4(s[k][gr * 4], s[k][gr * 4 + 1], s[k][gr * 4 + 2], s[k][gr * 4 + 3]);
+            }
+          }
+        }
+        if (keys < g.width && sh.lengths != nullptr) {  // values behind the length: zeros, whatever they were
+          const int st = cc % kStages;
+          if (!umma::mbar_wait(&v_full[st], (cc / kStages) & 1, 0x9b)) {
+            ok = false;
+            break;
+          }
+          zero_rows<DC>(smem + Y::OFF_V + st * DC * SUB, SUB, keys, (keys + 15) & ~15, threadIdx.x - 64);
+        }
+        warp_arrive(p_full, true);
+      }
+      if (!ok || !umma::mbar_wait(o_done, (cc - 1) & 1, 0x9c)) {
+        abort_flag = 1;
+        break;
+      }
+      umma::tc_fence_after();
+      const float inv = (DROP ? drop.scale : 1.f) / l;
+#pragma unroll
+      for (int k = 0; k < 2 * DC; ++k) {
+        if (!idle && k * 32 < sh.dim) {
+          uint32_t a[32];
+          tmem_ld32_nowait(tmem + lane_off + Y::kTmemO + k * 32, a);
+          wait_ld();
+          tie32(a);
+          const float* f = reinterpret_cast<const float*>(a);
+          if (valid) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int d = k * 32 + i * 8;
+              if (d < sh.dim) {
+                if (g.splits > 1) {
+                  float4* out = reinterpret_cast<float4*>(part_o + prow * sh.dim + d);
+                  out[0] = make_float4(f[8 * i] * inv, f[8 * i + 1] * inv, f[8 * i + 2] * inv, f[8 * i + 3] * inv);
+                  out[1] = make_float4(f[8 * i + 4] * inv, f[8 * i + 5] * inv, f[8 * i + 6] * inv, f[8 * i + 7] * inv);
+                } else {
+                  *reinterpret_cast<uint4*>(dst + d) =
+                      make_uint4(pack2<T>(f[8 * i] * inv, f[8 * i + 1] * inv),
+                                 pack2<T>(f[8 * i + 2] * inv, f[8 * i + 3] * inv),
+                                 pack2<T>(f[8 * i + 4] * inv, f[8 * i + 5] * inv),
+                                 pack2<T>(f[8 * i + 6] * inv, f[8 * i + 7] * inv));
+                }
+              }
+            }
+          }
+        }
+      }
+      warp_arrive(o_empty, false);
+      if (valid) {
+        const float stat2 = m + log2f(l);
+        if (g.splits > 1) part_lse[prow] = stat2;
+        else lse[stat] = stat2;
+      }
+      ++t;
+    }
+  }
+  umma::tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    umma::tc_fence_after();
+    umma::tmem_dealloc(tmem, Y::kCols);
+  }
+}
+
+// Joins the key ranges of a row: O = sum_s w_s O_s / sum_s w_s, w_s = 2^(lse_s - max), in the order of s.  One thread
+// per row and 8 head elements.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    xattn_join(const float* __restrict__ part_o, const float* __restrict__ part_lse, T* __restrict__ o,
+               float* __restrict__ lse, Plane po, Shape sh, Geometry g, int64_t threads) {
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= threads) return;
+  const int per_row = sh.dim / 8, d = (int)(id % per_row) * 8;
+  const int64_t row = id / per_row;
+  const int R = (int)(row % g.rows);
+  const int64_t bu = row / g.rows;
+  const int u = (int)(bu % g.units), b = (int)(bu / g.units);
+  const float* ls = part_lse + bu * g.splits * g.rows + R;
+  const float* src = part_o + (bu * g.splits * g.rows + R) * sh.dim + d;
+  float mx = -INFINITY;
+  for (int s = 0; s < g.splits; ++s) mx = fmaxf(mx, ls[(int64_t)s * g.rows]);
+  float acc[8] = {}, w = 0.f;
+  bool any = false;
+  for (int s = 0; s < g.splits; ++s) {
+    const float l2 = ls[(int64_t)s * g.rows];
+    if (l2 == -INFINITY) continue;  // no keys there
+    any = true;
+    const float ws = exp2f(l2 - mx);
+    w += ws;
+    const float4* v = reinterpret_cast<const float4*>(src + (int64_t)s * g.rows * sh.dim);
+    const float4 x = v[0], y = v[1];
+    const float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = fmaf(ws, f[e], acc[e]);
+  }
+  const float inv = any ? 1.f / w : 0.f;
+  const int pos = R >> g.gp_shift, head = (u << g.gp_shift) + (R & ((1 << g.gp_shift) - 1));
+  *reinterpret_cast<uint4*>(o + b * po.s_b + pos * po.s_n + head * po.s_h + d) =
+      make_uint4(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv),
+                 pack2<T>(acc[4] * inv, acc[5] * inv), pack2<T>(acc[6] * inv, acc[7] * inv));
+  if (d == 0) lse[bu * g.ldr + R] = any ? mx + log2f(w) : INFINITY;
+}
+
+// ------------------------------------------------------------ backward: dQ
+// Item = 128 packed rows of a unit; keys in chunks of 64.  The MMA lane forms
+// S = Q K^T and dP = dO V^T of chunk c + 1 as soon as the row warps hold
+// chunk c's in registers, and dQ += dS K once dS is in shared memory.  Eight
+// row warps, two threads per row with 32 columns each, two CTAs per SM.
+// D = rowsum(dO * O) is formed once per item and kept for the dK / dV kernel.
+namespace bw {
+constexpr int kRowWarps = 8;
+constexpr int kThreads = 64 + 32 * kRowWarps;
+constexpr int BC = 64;                 // chunk rows
+constexpr int CT = BC * 128;           // bytes of a chunk's 64-element sub-tile
+}  // namespace bw
+
+namespace bq {
+constexpr int kStages = 3;
+template <int DC>
+struct L {
+  static constexpr int OFF_DO = DC * TILE;
+  static constexpr int OFF_KV = 2 * DC * TILE;             // stages of DC K sub-tiles, DC V sub-tiles
+  static constexpr int STAGE = 2 * DC * bw::CT;
+  static constexpr int OFF_DS = OFF_KV + kStages * STAGE;
+  static constexpr int OFF_X = OFF_DS + TILE;              // [2][128] fp32 halves of D
+  static constexpr int OFF_BAR = OFF_X + 1024;
+  static constexpr int SMEM = OFF_BAR + 256 + 1024;
+  static constexpr uint32_t kTmemDP = 64, kTmemDQ = 128, kCols = 256;
+};
+constexpr int kBars = 2 + 2 * kStages + 7;
+}  // namespace bq
+
+template <typename T, int DC, bool DROP>
+__global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
+    xattn_bwd_dq(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
+                 const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                 const T* __restrict__ o, const float* __restrict__ lse, float* __restrict__ delta, T* __restrict__ dq,
+                 Plane po, Plane pdq, Shape sh, Geometry g, DropArgs drop) {
+  using namespace bw;
+  using namespace bq;
+  using Y = bq::L<DC>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Y::OFF_BAR);
+  uint64_t* qd_full = bars;
+  uint64_t* qd_empty = bars + 1;
+  uint64_t* kv_full = bars + 2;
+  uint64_t* kv_empty = kv_full + kStages;
+  uint64_t* sd_full = kv_empty + kStages;
+  uint64_t* s_free = sd_full + 1;
+  uint64_t* ds_full = s_free + 1;
+  uint64_t* ds_free = ds_full + 1;
+  uint64_t* dq_full = ds_free + 1;
+  uint64_t* dq_empty = dq_full + 1;
+  uint64_t* x_full = dq_empty + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
+  float* xs = reinterpret_cast<float*>(smem + Y::OFF_X);
+  __shared__ int abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int gp_mask = (1 << g.gp_shift) - 1;
+  if (threadIdx.x == 0) {
+    umma::mbar_init(qd_full, 1);
+    umma::mbar_init(qd_empty, 1 + kRowWarps);
+    for (int s = 0; s < kStages; ++s) {
+      umma::mbar_init(&kv_full[s], 1);
+      umma::mbar_init(&kv_empty[s], 1);
+    }
+    umma::mbar_init(sd_full, 1);
+    umma::mbar_init(s_free, kRowWarps);
+    umma::mbar_init(ds_full, kRowWarps);
+    umma::mbar_init(ds_free, 1);
+    umma::mbar_init(dq_full, 1);
+    umma::mbar_init(dq_empty, kRowWarps);
+    umma::mbar_init(x_full, kRowWarps);
+    abort_flag = 0;
+    umma::fence_barrier_init();
+  }
+  if (warp == 0) umma::tmem_alloc(tmem_slot, Y::kCols);
+  umma::tc_fence_before();
+  __syncthreads();
+  umma::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {  // Q and dO tiles
+      umma::tma_prefetch(&tmQ);
+      umma::tma_prefetch(&tmDO);
+      uint32_t t = 0;
+      for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
+        const Item it = forward_item(item, g);
+        if (sh.keys(it.b) == 0) continue;
+        if (!umma::mbar_wait(qd_empty, (t & 1) ^ 1, 0xa1)) {
+          abort_flag = 1;
+          break;
+        }
+        umma::mbar_arrive_expect_tx(qd_full, 2 * DC * TILE);
+#pragma unroll
+        for (int dc = 0; dc < DC; ++dc) {
+          const int pos = (it.blk * BM) >> g.gp_shift;
+          umma::tma_load_5d(smem + dc * TILE, &tmQ, qd_full, dc * 64, 0, pos, it.u, it.b);
+          umma::tma_load_5d(smem + Y::OFF_DO + dc * TILE, &tmDO, qd_full, dc * 64, 0, pos, it.u, it.b);
+        }
+        ++t;
+      }
+    } else if (lane == 1) {  // K / V chunks
+      umma::tma_prefetch(&tmK);
+      umma::tma_prefetch(&tmV);
+      uint32_t cc = 0;
+      for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
+        const Item it = forward_item(item, g);
+        const int nch = (sh.keys(it.b) + BC - 1) / BC;
+        for (int c = 0; c < nch; ++c, ++cc) {
+          const int s = cc % kStages;
+          if (!umma::mbar_wait(&kv_empty[s], ((cc / kStages) & 1) ^ 1, 0xa2)) {
+            abort_flag = 1;
+            break;
+          }
+          uint8_t* dst = smem + Y::OFF_KV + s * Y::STAGE;
+          umma::mbar_arrive_expect_tx(&kv_full[s], Y::STAGE);
+#pragma unroll
+          for (int dc = 0; dc < DC; ++dc) {
+            umma::tma_load_4d(dst + dc * CT, &tmK, &kv_full[s], dc * 64, c * BC, it.u / g.kv_units, it.b);
+            umma::tma_load_4d(dst + (DC + dc) * CT, &tmV, &kv_full[s], dc * 64, c * BC, it.u / g.kv_units, it.b);
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      uint32_t cc = 0, t = 0;
+      auto issue_s = [&](uint32_t c, int keys, bool last) -> bool {
+        const int s = c % kStages;
+        if (!umma::mbar_wait(&kv_full[s], (c / kStages) & 1, 0xa4)) return false;
+        if (!umma::mbar_wait(s_free, (c & 1) ^ 1, 0xa5)) return false;
+        umma::tc_fence_after();
+        const uint32_t k = umma::smem_u32(smem + Y::OFF_KV + s * Y::STAGE), idesc = Desc<T>::kk((keys + 15) & ~15);
+        mma_scores<DC>(tmem, umma::smem_u32(smem), TILE, k, CT, idesc);
+        mma_scores<DC>(tmem + Y::kTmemDP, umma::smem_u32(smem + Y::OFF_DO), TILE, k + DC * CT, CT, idesc);
+        umma::mma_commit(sd_full);
+        if (last) umma::mma_commit(qd_empty);
+        return true;
+      };
+      bool ok = true;
+      for (int item = blockIdx.x; item < g.total && ok && !abort_flag; item += gridDim.x) {
+        const Item it = forward_item(item, g);
+        const int len = sh.keys(it.b), nch = (len + BC - 1) / BC;
+        if (nch == 0) continue;
+        if (!umma::mbar_wait(qd_full, t & 1, 0xa3) || !issue_s(cc, min(BC, len), nch == 1)) {
+          ok = false;
+          break;
+        }
+        for (int c = 0; c < nch; ++c, ++cc) {
+          if (c + 1 < nch && !issue_s(cc + 1, min(BC, len - (c + 1) * BC), c + 2 == nch)) {
+            ok = false;
+            break;
+          }
+          if (!umma::mbar_wait(ds_full, cc & 1, 0xa6) ||
+              (c == 0 && !umma::mbar_wait(dq_empty, (t & 1) ^ 1, 0xa7))) {
+            ok = false;
+            break;
+          }
+          umma::tc_fence_after();
+          mma_rows<DC>(tmem + Y::kTmemDQ, umma::smem_u32(smem + Y::OFF_DS),
+                       umma::smem_u32(smem + Y::OFF_KV + (cc % kStages) * Y::STAGE), CT, Desc<T>::MN,
+                       (min(BC, len - c * BC) + 15) >> 4, c > 0);
+          umma::mma_commit(ds_free);
+          umma::mma_commit(&kv_empty[cc % kStages]);
+          if (c == nch - 1) umma::mma_commit(dq_full);
+        }
+        ++t;
+      }
+      if (!ok) abort_flag = 1;
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const float sl2 = sh.scale * kLog2e, mult = DROP ? drop.scale : 1.f;
+    const Philox rng = DROP ? Philox(drop) : Philox(DropArgs{nullptr, 0, 0, 0.f});
+    uint32_t cc = 0, t = 0;
+    for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
+      const Item it = forward_item(item, g);
+      const int len = sh.keys(it.b), nch = (len + BC - 1) / BC;
+      const int R = it.blk * BM + row, pos = R >> g.gp_shift, head = (it.u << g.gp_shift) + (R & gp_mask);
+      const bool valid = R < g.rows, idle = it.blk * BM + quarter * 32 >= g.rows;
+      const int64_t stat = (int64_t)(it.b * g.units + it.u) * g.ldr + R;
+      T* dst = dq + it.b * pdq.s_b + pos * pdq.s_n + head * pdq.s_h;
+      if (nch == 0) {
+        if (valid) {
+          for (int d = half * 8; d < sh.dim; d += 16) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
+          if (half == 0) delta[stat] = 0.f;
+        }
+        continue;
+      }
+      uint4 orow[4 * DC];
+      float lse2 = 0.f;
+      const T* osrc = o + it.b * po.s_b + pos * po.s_n + head * po.s_h;
+#pragma unroll
+      for (int i = 0; i < 4 * DC; ++i) {
+        const int d = (2 * i + half) * 8;
+        orow[i] = valid && d < sh.dim ? *reinterpret_cast<const uint4*>(osrc + d) : make_uint4(0, 0, 0, 0);
+      }
+      if (valid) lse2 = lse[stat];
+      if (!umma::mbar_wait(qd_full, t & 1, 0xa8)) {
+        abort_flag = 1;
+        break;
+      }
+      float part = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4 * DC; ++i) {
+        const int ch = 2 * i + half;
+        const uint4 d4 =
+            *reinterpret_cast<const uint4*>(smem + Y::OFF_DO + (ch >> 3) * TILE + sw128(row, ch & 7));
+        const T* oe = reinterpret_cast<const T*>(&orow[i]);
+        const T* de = reinterpret_cast<const T*>(&d4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) part = fmaf(Elem<T>::to_f(oe[e]), Elem<T>::to_f(de[e]), part);
+      }
+      xs[half * BM + row] = part;
+      warp_arrive(x_full, false);
+      if (!umma::mbar_wait(x_full, t & 1, 0xa9)) {
+        abort_flag = 1;
+        break;
+      }
+      const float dsum = xs[row] + xs[BM + row];
+      if (valid && half == 0) delta[stat] = dsum;
+      warp_arrive(qd_empty, false);
+      const uint32_t bh = (uint32_t)(it.b * sh.heads + head);
+      bool ok = true;
+      for (int c = 0; c < nch; ++c, ++cc) {
+        const int kc = c * BC, keys = min(BC, len - kc), k0 = half * 32;
+        const bool work = !idle && k0 < keys;
+        uint32_t keep = 0xffffffffu;  // drawn while the products run
+        if (DROP && work) keep = keep_word(rng, drop.limit, kc + k0, pos, bh);
+        if (!umma::mbar_wait(sd_full, cc & 1, 0xaa)) {
+          ok = false;
+          break;
+        }
+        umma::tc_fence_after();
+        uint32_t packed[16];
+        const bool tail = k0 + 32 > keys;
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {  // 16 columns at a time: 32 accumulator registers live
+          uint32_t su[16], du[16];
+          if (work) {
+            tmem_ld16_nowait(tmem + lane_off + k0 + hh * 16, su);
+            tmem_ld16_nowait(tmem + lane_off + Y::kTmemDP + k0 + hh * 16, du);
+            tmem_wait16(su, du);
+          }
+          if (hh == 1) warp_arrive(s_free, false);
+          if (work) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              float ds[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int col = hh * 16 + i + e;
+                const float p = ex2(fmaf(__uint_as_float(su[i + e]), sl2, -lse2));
+                const float dp = (keep >> col) & 1u ? __uint_as_float(du[i + e]) * mult : 0.f;
+                ds[e] = p * (dp - dsum);
+                if (tail && k0 + col >= keys) ds[e] = 0.f;
+              }
+              packed[hh * 8 + i / 2] = pack2<T>(ds[0], ds[1]);
+            }
+          }
+        }
+        if (!umma::mbar_wait(ds_free, (cc & 1) ^ 1, 0xab)) {
+          ok = false;
+          break;
+        }
+        if (work) {
+#pragma unroll
+          for (int gr = 0; gr < 4; ++gr)
+            *reinterpret_cast<uint4*>(smem + Y::OFF_DS + sw128(row, half * 4 + gr)) =
+                make_uint4(packed[gr * 4], packed[gr * 4 + 1], packed[gr * 4 + 2], packed[gr * 4 + 3]);
+        }
+        if (keys < BC && sh.lengths != nullptr)  // S of this chunk is formed: its keys behind the length become zeros
+          zero_rows<DC>(smem + Y::OFF_KV + (cc % kStages) * Y::STAGE, CT, keys, (keys + 15) & ~15, threadIdx.x - 64);
+        warp_arrive(ds_full, true);
+      }
+      if (!ok || !umma::mbar_wait(dq_full, t & 1, 0xac)) {
+        abort_flag = 1;
+        break;
+      }
+      umma::tc_fence_after();
+#pragma unroll
+      for (int dc = 0; dc < DC; ++dc) {
+        const int d0 = dc * 64 + half * 32;
+        if (!idle && d0 < sh.dim) {
+          uint32_t a[32];
+          tmem_ld32_nowait(tmem + lane_off + Y::kTmemDQ + d0, a);
+          wait_ld();
+          tie32(a);
+          const float* f = reinterpret_cast<const float*>(a);
+          if (valid) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (d0 + 8 * i < sh.dim)
+                *reinterpret_cast<uint4*>(dst + d0 + 8 * i) =
+                    make_uint4(pack2<T>(f[8 * i] * sh.scale, f[8 * i + 1] * sh.scale),
+                               pack2<T>(f[8 * i + 2] * sh.scale, f[8 * i + 3] * sh.scale),
+                               pack2<T>(f[8 * i + 4] * sh.scale, f[8 * i + 5] * sh.scale),
+                               pack2<T>(f[8 * i + 6] * sh.scale, f[8 * i + 7] * sh.scale));
+            }
+          }
+        }
+      }
+      warp_arrive(dq_empty, false);
+      ++t;
+    }
+  }
+  umma::tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    umma::tc_fence_after();
+    umma::tmem_dealloc(tmem, Y::kCols);
+  }
+}
+
+// -------------------------------------------------------- backward: dK, dV
+// Item = 128 keys of a key / value head; the packed rows of all its units
+// come in chunks of 64 with their lse2 and D.  S^T = K Q^T and dP^T = V dO^T
+// put a key in each tensor memory lane; dV += P^T dO and dK += dS^T Q take
+// the row threads' 16-bit P^T and dS^T from shared memory.  The dropout bits
+// come in groups of eight keys of one query, that is of eight lanes: each
+// lane draws the groups of four of its 32 columns and the eight exchange the
+// keep bits by shuffles, so a group is still drawn once.
+namespace bk {
+constexpr int kStages = 2;
+template <int DC>
+struct L {
+  static constexpr int OFF_V = DC * TILE;
+  static constexpr int OFF_CH = 2 * DC * TILE;
+  static constexpr int OFF_STAT = 2 * DC * bw::CT;              // within a stage: lse2[64], D[64]
+  static constexpr int STAGE = OFF_STAT + 1024;
+  static constexpr int OFF_PT = OFF_CH + kStages * STAGE;
+  static constexpr int OFF_DST = OFF_PT + TILE;
+  static constexpr int OFF_BAR = OFF_DST + TILE;
+  static constexpr int SMEM = OFF_BAR + 256 + 1024;
+  static constexpr uint32_t kTmemDP = 64, kTmemDV = 128, kTmemDK = 128 + 64 * DC;
+  static constexpr uint32_t kCols = DC == 1 ? 256 : 512;
+};
+constexpr int kBars = 2 + 2 * kStages + 6;
+}  // namespace bk
+
+template <typename T, int DC, bool DROP>
+__global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
+    xattn_bwd_dkdv(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                   const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
+                   const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk,
+                   T* __restrict__ dv, Plane pdk, Plane pdv, Shape sh, Geometry g, int kblk, DropArgs drop) {
+  using namespace bw;
+  using namespace bk;
+  using Y = bk::L<DC>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Y::OFF_BAR);
+  uint64_t* kv_full = bars;
+  uint64_t* kv_empty = bars + 1;
+  uint64_t* ch_full = bars + 2;
+  uint64_t* ch_empty = ch_full + kStages;
+  uint64_t* sd_full = ch_empty + kStages;
+  uint64_t* s_free = sd_full + 1;
+  uint64_t* ps_full = s_free + 1;
+  uint64_t* ps_free = ps_full + 1;
+  uint64_t* acc_full = ps_free + 1;
+  uint64_t* acc_empty = acc_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
+  __shared__ int abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int gp_mask = (1 << g.gp_shift) - 1;
+  const int per_unit = (g.rows + BC - 1) / BC, nch = per_unit * g.kv_units;
+  if (threadIdx.x == 0) {
+    umma::mbar_init(kv_full, 1);
+    umma::mbar_init(kv_empty, 1);
+    for (int s = 0; s < kStages; ++s) {
+      umma::mbar_init(&ch_full[s], 1);
+      umma::mbar_init(&ch_empty[s], 1);
+    }
+    umma::mbar_init(sd_full, 1);
+    umma::mbar_init(s_free, kRowWarps);
+    umma::mbar_init(ps_full, kRowWarps);
+    umma::mbar_init(ps_free, 1);
+    umma::mbar_init(acc_full, 1);
+    umma::mbar_init(acc_empty, kRowWarps);
+    abort_flag = 0;
+    umma::fence_barrier_init();
+  }
+  if (warp == 0) umma::tmem_alloc(tmem_slot, Y::kCols);
+  umma::tc_fence_before();
+  __syncthreads();
+  umma::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // item -> key block, key / value head, batch item
+  auto at = [&](int item, int& blk, int& kh, int& b) {
+    blk = item % kblk;
+    const int r = item / kblk;
+    kh = r % sh.kv_heads;
+    b = r / sh.kv_heads;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {  // K and V tiles
+      umma::tma_prefetch(&tmK);
+      umma::tma_prefetch(&tmV);
+      uint32_t t = 0;
+      for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
+        int blk, kh, b;
+        at(item, blk, kh, b);
+        if (blk * BM >= sh.keys(b)) continue;
+        if (!umma::mbar_wait(kv_empty, (t & 1) ^ 1, 0xb1)) {
+          abort_flag = 1;
+          break;
+        }
+        umma::mbar_arrive_expect_tx(kv_full, 2 * DC * TILE);
+#pragma unroll
+        for (int dc = 0; dc < DC; ++dc) {
+          umma::tma_load_4d(smem + dc * TILE, &tmK, kv_full, dc * 64, blk * BM, kh, b);
+          umma::tma_load_4d(smem + Y::OFF_V + dc * TILE, &tmV, kv_full, dc * 64, blk * BM, kh, b);
+        }
+        ++t;
+      }
+    } else if (lane == 1) {  // query chunks
+      umma::tma_prefetch(&tmQ);
+      umma::tma_prefetch(&tmDO);
+      uint32_t cc = 0;
+      for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
+        int blk, kh, b;
+        at(item, blk, kh, b);
+        if (blk * BM >= sh.keys(b)) continue;
+        for (int c = 0; c < nch; ++c, ++cc) {
+          const int s = cc % kStages, u = kh * g.kv_units + c / per_unit, r0 = (c % per_unit) * BC;
+          if (!umma::mbar_wait(&ch_empty[s], ((cc / kStages) & 1) ^ 1, 0xb2)) {
+            abort_flag = 1;
+            break;
+          }
+          uint8_t* dst = smem + Y::OFF_CH + s * Y::STAGE;
+          umma::mbar_arrive_expect_tx(&ch_full[s], 2 * DC * CT + 2 * BC * 4);
+#pragma unroll
+          for (int dc = 0; dc < DC; ++dc) {
+            umma::tma_load_5d(dst + dc * CT, &tmQ, &ch_full[s], dc * 64, 0, r0 >> g.gp_shift, u, b);
+            umma::tma_load_5d(dst + (DC + dc) * CT, &tmDO, &ch_full[s], dc * 64, 0, r0 >> g.gp_shift, u, b);
+          }
+          const int64_t stat = (int64_t)(b * g.units + u) * g.ldr + r0;  // both buffers end 64 values behind the last row
+          umma::bulk_load(dst + Y::OFF_STAT, lse + stat, BC * 4, &ch_full[s]);
+          umma::bulk_load(dst + Y::OFF_STAT + BC * 4, delta + stat, BC * 4, &ch_full[s]);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      uint32_t cc = 0, t = 0;
+      auto issue_s = [&](uint32_t c, int rows, bool last) -> bool {
+        const int s = c % kStages;
+        if (!umma::mbar_wait(&ch_full[s], (c / kStages) & 1, 0xb4)) return false;
+        if (!umma::mbar_wait(s_free, (c & 1) ^ 1, 0xb5)) return false;
+        umma::tc_fence_after();
+        const uint32_t q = umma::smem_u32(smem + Y::OFF_CH + s * Y::STAGE), idesc = Desc<T>::kk((rows + 15) & ~15);
+        mma_scores<DC>(tmem, umma::smem_u32(smem), TILE, q, CT, idesc);
+        mma_scores<DC>(tmem + Y::kTmemDP, umma::smem_u32(smem + Y::OFF_V), TILE, q + DC * CT, CT, idesc);
+        umma::mma_commit(sd_full);
+        if (last) umma::mma_commit(kv_empty);
+        return true;
+      };
+      auto rows_of = [&](int c) { return min(BC, g.rows - (c % per_unit) * BC); };
+      bool ok = true;
+      for (int item = blockIdx.x; item < g.total && ok && !abort_flag; item += gridDim.x) {
+        int blk, kh, b;
+        at(item, blk, kh, b);
+        if (blk * BM >= sh.keys(b)) continue;
+        if (!umma::mbar_wait(kv_full, t & 1, 0xb3) || !issue_s(cc, rows_of(0), nch == 1)) {
+          ok = false;
+          break;
+        }
+        for (int c = 0; c < nch; ++c, ++cc) {
+          if (c + 1 < nch && !issue_s(cc + 1, rows_of(c + 1), c + 2 == nch)) {
+            ok = false;
+            break;
+          }
+          if (!umma::mbar_wait(ps_full, cc & 1, 0xb6) ||
+              (c == 0 && !umma::mbar_wait(acc_empty, (t & 1) ^ 1, 0xb7))) {
+            ok = false;
+            break;
+          }
+          umma::tc_fence_after();
+          const uint32_t q = umma::smem_u32(smem + Y::OFF_CH + (cc % kStages) * Y::STAGE);
+          const int ksteps = (rows_of(c) + 15) >> 4;
+          mma_rows<DC>(tmem + Y::kTmemDV, umma::smem_u32(smem + Y::OFF_PT), q + DC * CT, CT, Desc<T>::MN, ksteps, c > 0);
+          mma_rows<DC>(tmem + Y::kTmemDK, umma::smem_u32(smem + Y::OFF_DST), q, CT, Desc<T>::MN, ksteps, c > 0);
+          umma::mma_commit(ps_free);
+          umma::mma_commit(&ch_empty[cc % kStages]);
+          if (c == nch - 1) umma::mma_commit(acc_full);
+        }
+        ++t;
+      }
+      if (!ok) abort_flag = 1;
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const float sl2 = sh.scale * kLog2e, mult = DROP ? drop.scale : 1.f;
+    const Philox rng = DROP ? Philox(drop) : Philox(DropArgs{nullptr, 0, 0, 0.f});
+    uint32_t cc = 0, t = 0;
+    for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
+      int blk, kh, b;
+      at(item, blk, kh, b);
+      const int len = sh.keys(b), j = blk * BM + row;
+      const bool exists = j < sh.nk, live = j < len, idle = blk * BM + quarter * 32 >= len;
+      T* out_k = dk + b * pdk.s_b + j * pdk.s_n + kh * pdk.s_h;
+      T* out_v = dv + b * pdv.s_b + j * pdv.s_n + kh * pdv.s_h;
+      if (blk * BM >= len) {
+        if (exists)
+          for (int d = half * 8; d < sh.dim; d += 16) {
+            *reinterpret_cast<uint4*>(out_k + d) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(out_v + d) = make_uint4(0, 0, 0, 0);
+          }
+        continue;
+      }
+      bool ok = true;
+      for (int c = 0; c < nch; ++c, ++cc) {
+        const int s = cc % kStages, u = kh * g.kv_units + c / per_unit, r0 = (c % per_unit) * BC;
+        const int rows = min(BC, g.rows - r0), c0 = half * 32;
+        const bool work = !idle && c0 < ((rows + 15) & ~15);
+        uint32_t word = 0xffffffffu;  // keep bits of four columns x eight keys, drawn by this lane for its eight
+        if (DROP && work) {
+          word = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = r0 + c0 + (lane & 7) * 4 + e;
+            const uint32_t bh = (uint32_t)(b * sh.heads + (u << g.gp_shift) + (r & gp_mask));
+            word |= keep_bits(rng((uint32_t)j >> 3, (uint32_t)(r >> g.gp_shift), bh), drop.limit) << (8 * e);
+          }
+        }
+        if (!umma::mbar_wait(&ch_full[s], (cc / kStages) & 1, 0xb8) || !umma::mbar_wait(sd_full, cc & 1, 0xb9)) {
+          ok = false;
+          break;
+        }
+        umma::tc_fence_after();
+        uint32_t pp[16], pd[16];
+        const bool tail = c0 + 32 > rows;
+        const float* ls = reinterpret_cast<const float*>(smem + Y::OFF_CH + s * Y::STAGE + Y::OFF_STAT) + c0;
+        const float* dl = ls + BC;
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {  // 16 columns at a time: 32 accumulator registers live
+          uint32_t su[16], du[16];
+          if (work) {
+            tmem_ld16_nowait(tmem + lane_off + c0 + hh * 16, su);
+            tmem_ld16_nowait(tmem + lane_off + Y::kTmemDP + c0 + hh * 16, du);
+            tmem_wait16(su, du);
+          }
+          if (hh == 1) warp_arrive(s_free, false);
+          if (work) {
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+              uint32_t bits = 0xffffffffu;
+              if (DROP) bits = __shfl_sync(0xffffffffu, word, (lane & 24) + hh * 4 + q4) >> (lane & 7);
+              const float4 l4 = *reinterpret_cast<const float4*>(ls + hh * 16 + 4 * q4);
+              const float4 d4 = *reinterpret_cast<const float4*>(dl + hh * 16 + 4 * q4);
+              const float lv[4] = {l4.x, l4.y, l4.z, l4.w}, dd[4] = {d4.x, d4.y, d4.z, d4.w};
+              float pt[4], ds[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int i = 4 * q4 + e;
+                // queries behind the last: their statistics are someone else's, so select zeros outright
+                const bool dead = !live || (tail && c0 + hh * 16 + i >= rows);
+                const bool keep = (bits >> (8 * e)) & 1u;
+                const float p = ex2(fmaf(__uint_as_float(su[i]), sl2, -lv[e]));
+                const float dp = keep ? __uint_as_float(du[i]) * mult : 0.f;
+                pt[e] = dead || !keep ? 0.f : p;
+                ds[e] = dead ? 0.f : p * (dp - dd[e]);
+              }
+              pp[hh * 8 + 2 * q4] = pack2<T>(pt[0], pt[1]);
+              pp[hh * 8 + 2 * q4 + 1] = pack2<T>(pt[2], pt[3]);
+              pd[hh * 8 + 2 * q4] = pack2<T>(ds[0], ds[1]);
+              pd[hh * 8 + 2 * q4 + 1] = pack2<T>(ds[2], ds[3]);
+            }
+          }
+        }
+        if (!umma::mbar_wait(ps_free, (cc & 1) ^ 1, 0xba)) {
+          ok = false;
+          break;
+        }
+        if (work) {
+#pragma unroll
+          for (int gr = 0; gr < 4; ++gr) {
+            const uint32_t at16 = sw128(row, half * 4 + gr);
+            *reinterpret_cast<uint4*>(smem + Y::OFF_PT + at16) =
+                make_uint4(pp[gr * 4], pp[gr * 4 + 1], pp[gr * 4 + 2], pp[gr * 4 + 3]);
+            *reinterpret_cast<uint4*>(smem + Y::OFF_DST + at16) =
+                make_uint4(pd[gr * 4], pd[gr * 4 + 1], pd[gr * 4 + 2], pd[gr * 4 + 3]);
+          }
+        }
+        warp_arrive(ps_full, true);
+      }
+      if (!ok || !umma::mbar_wait(acc_full, t & 1, 0xbb)) {
+        abort_flag = 1;
+        break;
+      }
+      umma::tc_fence_after();
+#pragma unroll
+      for (int dc = 0; dc < DC; ++dc) {
+        const int d0 = dc * 64 + half * 32;
+        if (d0 < sh.dim) {
+#pragma unroll
+          for (int which = 0; which < 2; ++which) {
+            uint32_t a[32];
+            if (!idle) {
+              tmem_ld32_nowait(tmem + lane_off + (which ? Y::kTmemDK : Y::kTmemDV) + d0, a);
+              wait_ld();
+              tie32(a);
+            }
+            const float* f = reinterpret_cast<const float*>(a);
+            const float by = which ? sh.scale : mult;
+            T* out = which ? out_k : out_v;
+            if (exists) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if (d0 + 8 * i >= sh.dim) continue;
+                uint4 w = make_uint4(0, 0, 0, 0);
+                if (live)
+                  w = make_uint4(pack2<T>(f[8 * i] * by, f[8 * i + 1] * by),
+                                 pack2<T>(f[8 * i + 2] * by, f[8 * i + 3] * by),
+                                 pack2<T>(f[8 * i + 4] * by, f[8 * i + 5] * by),
+                                 pack2<T>(f[8 * i + 6] * by, f[8 * i + 7] * by));
+                *reinterpret_cast<uint4*>(out + d0 + 8 * i) = w;
+              }
+            }
+          }
+        }
+      }
+      warp_arrive(acc_empty, false);
+      ++t;
+    }
+  }
+  umma::tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    umma::tc_fence_after();
+    umma::tmem_dealloc(tmem, Y::kCols);
+  }
+}
+
+// ------------------------------------------------------------------ host
+int64_t round_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+
+// Rows and tiles of a shape; `splits` from the tile count alone, so that the
+// workspace size, the forward and its join agree.
+Geometry geometry(const Shape& sh) {
+  Geometry g;
+  const int group = sh.heads / sh.kv_heads;
+  g.gp_shift = 0;
+  while (g.gp_shift < 6 && group % (2 << g.gp_shift) == 0) ++g.gp_shift;
+  g.units = sh.heads >> g.gp_shift;
+  g.kv_units = group >> g.gp_shift;
+  g.rows = sh.nq << g.gp_shift;
+  g.ldr = (int)round_up(g.rows, 4);
+  g.nblk = (g.rows + BM - 1) / BM;
+  const int nch = (sh.nk + fw::kMaxW - 1) / fw::kMaxW;
+  g.width = (int)round_up((sh.nk + nch - 1) / nch, 16);
+  // key ranges: enough items for two waves of two CTAs per SM, at least four chunks each
+  const int64_t items = (int64_t)sh.batch * g.units * g.nblk, want = (int64_t)num_sms() * 4;
+  int64_t s = items > 0 ? want / items : 1;
+  if (s > nch / 4) s = nch / 4;
+  if (s > kMaxSplits) s = kMaxSplits;
+  g.splits = s < 1 ? 1 : (int)s;
+  g.total = 0;
+  return g;
+}
+
+int check_planes(const Shape& sh, const Plane* planes, const void* const* ptrs, const bool* query_side, int count,
+                 const char* name) {
+  for (int i = 0; i < count; ++i) {
+    const Plane& p = planes[i];
+    const int n = query_side[i] ? sh.nq : sh.nk, h = query_side[i] ? sh.heads : sh.kv_heads;
+    const bool aligned = (reinterpret_cast<uintptr_t>(ptrs[i]) & 15) == 0 && (sh.batch == 1 || p.s_b % 8 == 0) &&
+                         (n == 1 || p.s_n % 8 == 0) && (h == 1 || p.s_h % 8 == 0);
+    if (!aligned) {
+      set_error("%s: 16-bit planes with head dims in multiples of 8 must be 16-byte aligned, with strides that are "
+                "multiples of 8", name);
+      return PMB_ERR_ALIGNMENT;
+    }
+    PMB_REQUIRE((sh.batch == 1 || p.s_b > 0) && (n == 1 || p.s_n > 0) && (h == 1 || p.s_h > 0),
+                "%s: strides must be positive", name);
+  }
+  return PMB_OK;
+}
+
+uint64_t stride_bytes(int64_t stride, int extent) { return extent > 1 ? (uint64_t)stride * 2 : 16; }
+
+// Packed rows of a query-side plane: box of `rows` packed rows x 64 elements.
+int query_map(CUtensorMap& map, const void* base, const Plane& p, const Shape& sh, const Geometry& g, int dtype,
+              int rows, const char* name) {
+  const int gp = 1 << g.gp_shift;
+  const uint64_t dims[5] = {(uint64_t)sh.dim, (uint64_t)gp, (uint64_t)sh.nq, (uint64_t)g.units, (uint64_t)sh.batch};
+  const uint64_t strides[4] = {stride_bytes(p.s_h, gp), stride_bytes(p.s_n, sh.nq),
+                               stride_bytes(p.s_h * gp, g.units), stride_bytes(p.s_b, sh.batch)};
+  const uint32_t box[5] = {64, (uint32_t)gp, (uint32_t)(rows / gp), 1, 1};
+  return tma::make_map_5d(map, base, dtype, dims, strides, box, name);
+}
+
+int key_map(CUtensorMap& map, const void* base, const Plane& p, const Shape& sh, int dtype, int rows,
+            const char* name) {
+  const uint64_t dims[4] = {(uint64_t)sh.dim, (uint64_t)sh.nk, (uint64_t)sh.kv_heads, (uint64_t)sh.batch};
+  const uint64_t strides[3] = {stride_bytes(p.s_n, sh.nk), stride_bytes(p.s_h, sh.kv_heads),
+                               stride_bytes(p.s_b, sh.batch)};
+  const uint32_t box[4] = {64, (uint32_t)rows, 1, 1};
+  return tma::make_map_4d(map, base, dtype, dims, strides, box, name);
+}
+
+int persistent_grid(int64_t items, int per_sm) {
+  const int64_t g = (int64_t)num_sms() * per_sm;
+  return (int)(g < items ? g : items);
+}
+
+template <typename T, int DC, bool DROP>
+int forward_launch(const Shape& sh, const Forward& a, Geometry g, const char* name) {
+  CUtensorMap mq, mk, mv;
+  if (int st = query_map(mq, a.q, a.pq, sh, g, a.dtype, BM, name)) return st;
+  if (int st = key_map(mk, a.k, a.pk, sh, a.dtype, g.width, name)) return st;
+  if (int st = key_map(mv, a.v, a.pv, sh, a.dtype, g.width, name)) return st;
+  const int64_t rows = (int64_t)sh.batch * g.units * g.rows;
+  float* part_lse = static_cast<float*>(a.workspace);
+  float* part_o = part_lse + round_up(rows * g.splits, 64);
+  auto kernel = xattn_fwd<T, DC, DROP>;
+  constexpr int smem = fw::L<DC>::SMEM;
+  PMB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), name);
+  kernel<<<persistent_grid(g.total, DC == 1 ? 2 : 1), fw::kThreads, smem, a.stream>>>(
+      mq, mk, mv, static_cast<T*>(a.o), a.lse, part_o, part_lse, a.po, sh, g, a.drop);
+  PMB_CHECK_LAUNCH(name);
+  if (g.splits > 1) {
+    const int64_t threads = rows * (sh.dim / 8);
+    xattn_join<T><<<(unsigned)((threads + 255) / 256), 256, 0, a.stream>>>(part_o, part_lse, static_cast<T*>(a.o),
+                                                                          a.lse, a.po, sh, g, threads);
+    PMB_CHECK_LAUNCH(name);
+  }
+  return PMB_OK;
+}
+
+template <typename T, int DC, bool DROP>
+int backward_launch(const Shape& sh, const Backward& a, Geometry g, const char* name) {
+  CUtensorMap q128, do128, q64, do64, k64, v64, k128, v128;
+  if (int st = query_map(q128, a.q, a.pq, sh, g, a.dtype, BM, name)) return st;
+  if (int st = query_map(do128, a.go, a.pgo, sh, g, a.dtype, BM, name)) return st;
+  if (int st = query_map(q64, a.q, a.pq, sh, g, a.dtype, bw::BC, name)) return st;
+  if (int st = query_map(do64, a.go, a.pgo, sh, g, a.dtype, bw::BC, name)) return st;
+  if (int st = key_map(k64, a.k, a.pk, sh, a.dtype, bw::BC, name)) return st;
+  if (int st = key_map(v64, a.v, a.pv, sh, a.dtype, bw::BC, name)) return st;
+  if (int st = key_map(k128, a.k, a.pk, sh, a.dtype, BM, name)) return st;
+  if (int st = key_map(v128, a.v, a.pv, sh, a.dtype, BM, name)) return st;
+  float* delta = static_cast<float*>(a.workspace);
+  constexpr int per_sm = DC == 1 ? 2 : 1;
+  {
+    auto kernel = xattn_bwd_dq<T, DC, DROP>;
+    constexpr int smem = bq::L<DC>::SMEM;
+    PMB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), name);
+    kernel<<<persistent_grid(g.total, per_sm), bw::kThreads, smem, a.stream>>>(
+        q128, do128, k64, v64, static_cast<const T*>(a.o), a.lse, delta, static_cast<T*>(a.gq), a.po, a.pgq, sh, g,
+        a.drop);
+    PMB_CHECK_LAUNCH(name);
+  }
+  const int kblk = (sh.nk + BM - 1) / BM;
+  const int64_t items = (int64_t)sh.batch * sh.kv_heads * kblk;
+  PMB_REQUIRE(items < ((int64_t)1 << 31), "%s: too many keys", name);
+  g.total = (int)items;
+  auto kernel = xattn_bwd_dkdv<T, DC, DROP>;
+  constexpr int smem = bk::L<DC>::SMEM;
+  PMB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), name);
+  kernel<<<persistent_grid(items, per_sm), bw::kThreads, smem, a.stream>>>(
+      k128, v128, q64, do64, a.lse, delta, static_cast<T*>(a.gk), static_cast<T*>(a.gv), a.pgk, a.pgv, sh, g, kblk,
+      a.drop);
+  PMB_CHECK_LAUNCH(name);
+  return PMB_OK;
+}
+
+template <typename T, int DC>
+int forward_drop(const Shape& sh, const Forward& a, const Geometry& g, const char* name) {
+  return a.threshold > 0 ? forward_launch<T, DC, true>(sh, a, g, name) : forward_launch<T, DC, false>(sh, a, g, name);
+}
+template <typename T, int DC>
+int backward_drop(const Shape& sh, const Backward& a, const Geometry& g, const char* name) {
+  return a.threshold > 0 ? backward_launch<T, DC, true>(sh, a, g, name) : backward_launch<T, DC, false>(sh, a, g, name);
+}
+
+int64_t forward_bytes(const Shape& sh, const Geometry& g) {
+  if (g.splits <= 1) return 0;
+  const int64_t rows = (int64_t)sh.batch * g.units * g.rows * g.splits;
+  return round_up(round_up(rows, 64) * 4 + rows * sh.dim * 4, 256);
+}
+
+int count_items(const Shape& sh, Geometry& g, const char* name) {
+  const int64_t items = (int64_t)sh.batch * g.units * g.nblk * g.splits;
+  PMB_REQUIRE(items < ((int64_t)1 << 31) && ((int64_t)sh.nq << g.gp_shift) < (1 << 30), "%s: too many rows", name);
+  g.total = (int)items;
+  return PMB_OK;
+}
+
+}  // namespace
+
+int64_t tc_lse_floats(int64_t heads_total, int64_t nq) { return heads_total * round_up(nq, 4) + 64; }
+
+int64_t tc_forward_workspace(const Shape& sh) { return forward_bytes(sh, geometry(sh)); }
+
+int64_t tc_backward_workspace(const Shape& sh) {
+  return round_up(tc_lse_floats((int64_t)sh.batch * sh.heads, sh.nq) * 4, 256);
+}
+
+int tc_forward(const Shape& sh, const Forward& a, const char* name) {
+  Geometry g = geometry(sh);
+  if (int st = count_items(sh, g, name)) return st;
+  const Plane planes[4] = {a.pq, a.pk, a.pv, a.po};
+  const void* ptrs[4] = {a.q, a.k, a.v, a.o};
+  const bool side[4] = {true, false, false, true};
+  if (int st = check_planes(sh, planes, ptrs, side, 4, name)) return st;
+  const int64_t need = forward_bytes(sh, g);
+  if (need > 0 && (a.workspace == nullptr || a.workspace_bytes < need ||
+                   (reinterpret_cast<uintptr_t>(a.workspace) & 15))) {
+    set_error("%s: needs a 16-byte aligned workspace of %lld bytes (got %lld)", name, (long long)need,
+              (long long)a.workspace_bytes);
+    return PMB_ERR_WORKSPACE;
+  }
+  if (a.dtype == PMB_BFLOAT16)
+    return sh.dim <= 64 ? forward_drop<__nv_bfloat16, 1>(sh, a, g, name) : forward_drop<__nv_bfloat16, 2>(sh, a, g, name);
+  return sh.dim <= 64 ? forward_drop<__half, 1>(sh, a, g, name) : forward_drop<__half, 2>(sh, a, g, name);
+}
+
+int tc_backward(const Shape& sh, const Backward& a, const char* name) {
+  Geometry g = geometry(sh);
+  g.splits = 1;
+  if (int st = count_items(sh, g, name)) return st;
+  const Plane planes[8] = {a.pq, a.pk, a.pv, a.po, a.pgo, a.pgq, a.pgk, a.pgv};
+  const void* ptrs[8] = {a.q, a.k, a.v, a.o, a.go, a.gq, a.gk, a.gv};
+  const bool side[8] = {true, false, false, true, true, true, false, false};
+  if (int st = check_planes(sh, planes, ptrs, side, 8, name)) return st;
+  if ((reinterpret_cast<uintptr_t>(a.lse) | reinterpret_cast<uintptr_t>(a.workspace)) & 15) {
+    set_error("%s: lse and workspace must be 16-byte aligned", name);
+    return PMB_ERR_ALIGNMENT;
+  }
+  if (a.dtype == PMB_BFLOAT16)
+    return sh.dim <= 64 ? backward_drop<__nv_bfloat16, 1>(sh, a, g, name)
+                        : backward_drop<__nv_bfloat16, 2>(sh, a, g, name);
+  return sh.dim <= 64 ? backward_drop<__half, 1>(sh, a, g, name) : backward_drop<__half, 2>(sh, a, g, name);
+}
+
+}  // namespace xattn
+}  // namespace pmb

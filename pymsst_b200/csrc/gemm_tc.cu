@@ -92,6 +92,38 @@ int make_map_4d(CUtensorMap& map, const void* base, int dtype, const uint64_t (&
   return PMB_OK;
 }
 
+int make_map_5d(CUtensorMap& map, const void* base, int dtype, const uint64_t (&dims)[5],
+                const uint64_t (&stride_bytes)[4], const uint32_t (&box)[5], const char* name) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) {
+    set_error("%s: cuTensorMapEncodeTiled is unavailable (driver too old or no GPU)", name);
+    return PMB_ERR_CUDA;
+  }
+  cuuint64_t d[5], st[4];
+  cuuint32_t bx[5], elem[5];
+  uint64_t low = reinterpret_cast<uintptr_t>(base);
+  for (int i = 0; i < 5; ++i) {
+    d[i] = dims[i];
+    bx[i] = box[i];
+    elem[i] = 1;
+    if (i < 4) low |= st[i] = stride_bytes[i];
+  }
+  if (low & 15) {
+    set_error("%s: tensor-core operand needs a 16-byte aligned base and strides", name);
+    return PMB_ERR_ALIGNMENT;
+  }
+  const CUtensorMapDataType t =
+      dtype == PMB_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUresult r = fn(&map, t, 5, const_cast<void*>(base), d, st, bx, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("%s: cuTensorMapEncodeTiled failed (%d) for a 5-D map", name, (int)r);
+    return PMB_ERR_CUDA;
+  }
+  return PMB_OK;
+}
+
 int make_store_map_2d(CUtensorMap& map, const void* base, int dtype, uint64_t cols, uint64_t rows, uint64_t ld_bytes,
                       const char* name) {
   EncodeTiledFn fn = encode_fn();

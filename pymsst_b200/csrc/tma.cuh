@@ -27,6 +27,10 @@ int make_map_3d(CUtensorMap& map, const void* base, int dtype, uint64_t inner, u
 int make_map_4d(CUtensorMap& map, const void* base, int dtype, const uint64_t (&dims)[4],
                 const uint64_t (&stride_bytes)[3], const uint32_t (&box)[4], const char* name);
 
+// 5-D map, otherwise as make_map_4d.
+int make_map_5d(CUtensorMap& map, const void* base, int dtype, const uint64_t (&dims)[5],
+                const uint64_t (&stride_bytes)[4], const uint32_t (&box)[5], const char* name);
+
 // Output map for TMA tile stores: a 16-bit [rows, cols] matrix with a row
 // pitch of ld_bytes (a multiple of 16), box {32 columns, 32 rows}, 64-byte
 // swizzle (the layout ugemm::warp_tma_store writes).

@@ -119,6 +119,16 @@ def test_c_entries_refuse_bad_arguments_without_a_gpu():
     assert fwd(threshold=5) == -1 and b"NULL key" in lib.pmb_last_error()
     assert fwd(threshold=-1) == -1 and fwd(ptr=None) == -1
     assert fwd(dtype=7) == -2
+    assert lib.pmb_cross_attention_lse_size(2, 4, 3) >= 2 * 4 * 3
+    misaligned = nat.i64_array([8, 8, 12] * 8)  # head strides of 12 elements: no 16-byte rows
+    assert lib.pmb_cross_attention_forward(16, 16, 16, 16, 16, None, 2, 4, 2, 3, 5, 8, misaligned, 1.0, 0, None, 0, 2,
+                                           None, 0, None) == -4
+    assert lib.pmb_cross_attention_forward(8, 16, 16, 16, 16, None, 2, 4, 2, 3, 5, 8, strides, 1.0, 0, None, 0, 2,
+                                           None, 0, None) == -4
+    need = lib.pmb_cross_attention_forward_workspace_size(1, 1, 1, 1, 8192, 64, 2)
+    assert need > 0
+    assert lib.pmb_cross_attention_forward(16, 16, 16, 16, 16, None, 1, 1, 1, 1, 8192, 64, strides, 1.0, 0, None, 0, 2,
+                                           16, need - 1, None) == -5
     size = lib.pmb_cross_attention_backward_workspace_size(2, 4, 2, 3, 5, 8, 2)
     assert size >= 2 * 4 * 3 * 4
     bwd = lib.pmb_cross_attention_backward(16, 16, 16, 16, 16, 16, 16, 16, 16, None, 2, 4, 2, 3, 5, 8, strides, 1.0, 0,
