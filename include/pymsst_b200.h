@@ -683,7 +683,7 @@ PMB_API int pmb_gelu_dropout_backward(const void* grad_out, const void* x, void*
  * O = 0 and no gradient.  lse: fp32, pmb_cross_attention_lse_size(batch,
  * heads, nq) values, 16-byte aligned: row statistics that the forward writes
  * for the backward of the same call (their order and base are its own).
- * 16-bit types with head dims that are multiples of 8 up to 128 and scale >=
+ * 16-bit types with head dims that are multiples of 8 up to 128 and scale >
  * 0 run on the tensor cores; their planes must be 16-byte aligned with
  * positive strides that are multiples of 8 (strides of extents of 1 are not
  * looked at).

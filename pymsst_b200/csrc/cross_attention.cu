@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(kThreads)
   if (row >= (int64_t)sh.batch * sh.heads * sh.nq) return;
   const int i = (int)(row % sh.nq), bh = (int)(row / sh.nq), h = bh % sh.heads, b = bh / sh.heads;
   const int kh = h / (sh.heads / sh.kv_heads), len = sh.keys(b);
-  const Philox rng = DROP ? Philox(drop) : Philox(DropArgs{nullptr, 0, 0, 0.f});
+  const Philox rng(DROP ? drop : DropArgs{});
   const T* qr = q + b * pq.s_b + i * pq.s_n + h * pq.s_h;
   for (int c = lane; c < sh.dim; c += 32) qs[warp][c] = Elem<T>::to_f(qr[c]) * sh.scale;
   __syncwarp();
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kThreads)
   if (row >= (int64_t)sh.batch * sh.heads * sh.nq) return;
   const int i = (int)(row % sh.nq), bh = (int)(row / sh.nq), h = bh % sh.heads, b = bh / sh.heads;
   const int kh = h / (sh.heads / sh.kv_heads), len = sh.keys(b);
-  const Philox rng = DROP ? Philox(drop) : Philox(DropArgs{nullptr, 0, 0, 0.f});
+  const Philox rng(DROP ? drop : DropArgs{});
   const T* qr = q + b * pq.s_b + i * pq.s_n + h * pq.s_h;
   const T* gr = go + b * pgo.s_b + i * pgo.s_n + h * pgo.s_h;
   const T* orow = o + b * po.s_b + i * po.s_n + h * po.s_h;
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kThreads)
   if (row >= (int64_t)sh.batch * sh.kv_heads * sh.nk) return;
   const int j = (int)(row % sh.nk), bk = (int)(row / sh.nk), kh = bk % sh.kv_heads, b = bk / sh.kv_heads;
   const int group = sh.heads / sh.kv_heads;
-  const Philox rng = DROP ? Philox(drop) : Philox(DropArgs{nullptr, 0, 0, 0.f});
+  const Philox rng(DROP ? drop : DropArgs{});
   float ak[kAcc] = {}, av[kAcc] = {};
   if (j < sh.keys(b)) {
     const T* kr = k + b * pk.s_b + j * pk.s_n + kh * pk.s_h;

@@ -52,10 +52,10 @@ struct Backward {
 };
 
 // Whether the tensor-core form takes a call: 16-bit types, head dims that are
-// multiples of 8 up to 128, something on both sides, and a scale that keeps
-// the order of the scores (its running maximum is taken before scaling).
+// multiples of 8 up to 128, something on both sides, and a positive scale (the
+// maximum is taken before scaling, and masked scores are -inf before it).
 inline bool tc_takes(const Shape& sh, int dtype) {
-  return dtype_size(dtype) == 2 && sh.dim % 8 == 0 && sh.dim <= 128 && sh.nq > 0 && sh.nk > 0 && sh.scale >= 0.f;
+  return dtype_size(dtype) == 2 && sh.dim % 8 == 0 && sh.dim <= 128 && sh.nq > 0 && sh.nk > 0 && sh.scale > 0.f;
 }
 
 int64_t tc_lse_floats(int64_t heads_total, int64_t nq);

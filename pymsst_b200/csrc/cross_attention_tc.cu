@@ -19,11 +19,13 @@
 // memory before the product that multiplies them by a zero weight, so NaN
 // there stays there.
 //
-// Row statistics are kept as base-2 logarithms (lse2 = max + log2(sum), of
-// scores times scale * log2 e); +inf for a row without keys, whose
-// probabilities then come out as 0.
+// Row statistics are base-2 logarithms (lse2 = max + log2(sum), of scores
+// times scale * log2 e), kept negated, as the backward adds them; -inf for a
+// row without keys, whose probabilities then come out as 0.  D is kept negated
+// too.
 #include "attention_tiles.cuh"
 #include "cross_attention.cuh"
+#include "f32x2.cuh"
 #include "tma.cuh"
 #include "umma.cuh"
 
@@ -97,12 +99,11 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, uint32_t sub, int first
     for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile + dc * sub + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
 }
 
-// Keep bits of the 32 keys from `key` (a multiple of 8) on, of one query.
-__device__ __forceinline__ uint32_t keep_word(const Philox& rng, uint32_t limit, int key, int query, uint32_t bh) {
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w |= keep_bits(rng(((uint32_t)key >> 3) + i, (uint32_t)query, bh), limit) << (8 * i);
-  return w;
+// max of three
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -111,8 +112,12 @@ __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.
 // Item = 128 packed rows of a unit, over one of `splits` key ranges.  Keys
 // come in chunks of `width` <= 96 (a multiple of 16 that divides the keys
 // evenly): S (two buffers of 96 columns) and O (64 columns per 64 head
-// elements) then fill 256 tensor memory columns, two CTAs fit an SM, and a
-// row thread holds its whole chunk of scores in registers.
+// elements) then fill 256 tensor memory columns and two CTAs fit an SM.
+//
+// Eight row warps: two threads per row share its scores by blocks of 16
+// columns (even blocks, odd blocks), so four row warps per scheduler hide one
+// another's latencies.  They agree on the running maximum through shared
+// memory once per chunk; sums stay apart until the end.
 //
 // The MMA lane issues S of chunk c + 1 before O += P V of chunk c, so scores
 // are ready while the row warps work.  O stays in tensor memory; the running
@@ -125,7 +130,8 @@ __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.
 // K and V have separate rings: a K stage is free as soon as its scores are
 // formed.
 namespace fw {
-constexpr int kThreads = 192;
+constexpr int kRowWarps = 8;
+constexpr int kThreads = 64 + 32 * kRowWarps;
 constexpr int kMaxW = 96;
 constexpr int kStages = 2;
 constexpr int SUB = kMaxW * 128;  // one 64-element sub-tile of a K or V stage
@@ -134,12 +140,13 @@ struct L {
   static constexpr int OFF_K = DC * TILE;
   static constexpr int OFF_V = OFF_K + kStages * DC * SUB;
   static constexpr int OFF_P = OFF_V + kStages * DC * SUB;  // 128 rows x 96 keys: two sub-tiles
-  static constexpr int OFF_BAR = OFF_P + 2 * TILE;
+  static constexpr int OFF_X = OFF_P + 2 * TILE;            // [2 turns][2 halves][128] row values exchanged
+  static constexpr int OFF_BAR = OFF_X + 2048;
   static constexpr int SMEM = OFF_BAR + 256 + 1024;
   static constexpr uint32_t kTmemO = 2 * kMaxW;
   static constexpr uint32_t kCols = DC == 1 ? 256 : 512;
 };
-constexpr int kBars = 2 + 4 * kStages + 2 + 3;
+constexpr int kBars = 2 + 4 * kStages + 2 + 3 + 4;
 constexpr float kRescale = 8.f;
 }  // namespace fw
 
@@ -161,8 +168,12 @@ __device__ __forceinline__ Item forward_item(int item, const Geometry& g) {
 // Chunks [c0, c1) of an item.
 __device__ __forceinline__ void chunk_range(int len, const Item& it, const Geometry& g, int& c0, int& c1) {
   const int n = (len + g.width - 1) / g.width;
-  c0 = (int)((int64_t)n * it.split / g.splits);
-  c1 = (int)((int64_t)n * (it.split + 1) / g.splits);
+  c0 = 0;
+  c1 = n;
+  if (g.splits > 1) {  // n < 2^30 / 16 and splits <= 64 fit 32 bits
+    c0 = (int)((unsigned)n * (unsigned)it.split / (unsigned)g.splits);
+    c1 = (int)((unsigned)n * (unsigned)(it.split + 1) / (unsigned)g.splits);
+  }
 }
 
 template <typename T, int DC, bool DROP>
@@ -186,13 +197,16 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
   uint64_t* p_full = s_full + 2;
   uint64_t* o_done = p_full + 1;
   uint64_t* o_empty = o_done + 1;
+  uint64_t* pair = o_empty + 1;  // [4]: the two warps of a lane quarter
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
+  float* xs = reinterpret_cast<float*>(smem + Y::OFF_X);
   __shared__ int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gp_mask = (1 << g.gp_shift) - 1;
   if (threadIdx.x == 0) {
     umma::mbar_init(q_full, 1);
     umma::mbar_init(q_empty, 1);
+    for (int i = 0; i < 4; ++i) umma::mbar_init(&pair[i], 2);
     for (int s = 0; s < kStages; ++s) {
       umma::mbar_init(&k_full[s], 1);
       umma::mbar_init(&k_empty[s], 1);
@@ -201,9 +215,9 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
     }
     umma::mbar_init(&s_full[0], 1);
     umma::mbar_init(&s_full[1], 1);
-    umma::mbar_init(p_full, 4);
+    umma::mbar_init(p_full, kRowWarps);
     umma::mbar_init(o_done, 1);
-    umma::mbar_init(o_empty, 4);
+    umma::mbar_init(o_empty, kRowWarps);
     abort_flag = 0;
     umma::fence_barrier_init();
   }
@@ -313,11 +327,22 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
       if (!ok) abort_flag = 1;
     }
   } else {
-    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const float sl2 = sh.scale * kLog2e;
-    const Philox rng = DROP ? Philox(drop) : Philox(DropArgs{nullptr, 0, 0, 0.f});
-    uint32_t cc = 0, t = 0;
+    const Philox rng(DROP ? drop : DropArgs{});
+    uint32_t cc = 0, turn = 0;
+    // both threads of a row leave a value and take the other's
+    auto exchange = [&](float mine, float& other) -> bool {
+      float* slot = xs + (turn & 1) * 256;
+      slot[half * 128 + row] = mine;
+      __syncwarp();
+      if (lane == 0) umma::mbar_arrive(&pair[quarter]);
+      if (!umma::mbar_wait(&pair[quarter], turn & 1, 0x9d)) return false;
+      other = slot[(half ^ 1) * 128 + row];
+      ++turn;
+      return true;
+    };
     for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
       const Item it = forward_item(item, g);
       const int len = sh.keys(it.b);
@@ -326,16 +351,17 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
       const int R = it.blk * BM + row, pos = R >> g.gp_shift, head = (it.u << g.gp_shift) + (R & gp_mask);
       const bool valid = R < g.rows;
       const bool idle = it.blk * BM + quarter * 32 >= g.rows;  // no row of this warp exists
-      const int64_t stat = (int64_t)(it.b * g.units + it.u) * g.ldr + R;
-      const int64_t prow = ((int64_t)(it.b * g.units + it.u) * g.splits + it.split) * g.rows + R;
-      T* dst = o + it.b * po.s_b + pos * po.s_n + head * po.s_h;
+      // formed where they are used, not held in registers across the loop
+      auto stat = [&] { return (int64_t)(it.b * g.units + it.u) * g.ldr + R; };
+      auto prow = [&] { return ((int64_t)(it.b * g.units + it.u) * g.splits + it.split) * g.rows + R; };
+      auto dst = [&] { return o + it.b * po.s_b + pos * po.s_n + head * po.s_h; };
       if (c0 >= c1) {
         if (valid) {
-          if (g.splits > 1) {
-            part_lse[prow] = -INFINITY;
-          } else {
-            for (int d = 0; d < sh.dim; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
-            lse[stat] = INFINITY;
+          if (g.splits == 1)
+            for (int d = half * 8; d < sh.dim; d += 16) *reinterpret_cast<uint4*>(dst() + d) = make_uint4(0, 0, 0, 0);
+          if (half == 0) {
+            if (g.splits > 1) part_lse[prow()] = -INFINITY;
+            else lse[stat()] = -INFINITY;
           }
         }
         continue;
@@ -345,41 +371,38 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
       bool ok = true;
       for (int c = c0; c < c1; ++c, ++cc) {
         const int kc = c * g.width, keys = min(g.width, len - kc);
-        uint32_t keep[3];  // the chunk's dropout bits, drawn while its scores are formed
-        if (DROP && !idle) {
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            if (k * 32 < keys) keep[k] = keep_word(rng, drop.limit, kc + k * 32, pos, bh);
-          }
-        }
         if (!umma::mbar_wait(&s_full[cc & 1], (cc >> 1) & 1, 0x98)) {
           ok = false;
           break;
         }
         umma::tc_fence_after();
-        uint32_t s[3][32];
+        const uint32_t src = tmem + lane_off + (cc & 1) * kMaxW;
         if (!idle) {
-          const uint32_t src = tmem + lane_off + (cc & 1) * kMaxW;
+          float mx = -INFINITY, mo;
+#pragma unroll 1
+          for (int first = half * 16; first < keys; first += 32) {
+            uint32_t s[16];
+            tmem_ld16_nowait(src + first, s);
+            wait_ld();
+            tie16(s);
+            if (first + 16 > keys) {
 #pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            if (k * 32 < keys) tmem_ld32_nowait(src + k * 32, s[k]);
-          }
-          wait_ld();
-#pragma unroll
-          for (int k = 0; k < 3; ++k) tie32(s[k]);
-          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            if (k * 32 + 32 <= keys) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(s[k][e]));
-            } else if (k * 32 < keys) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (k * 32 + e < keys) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(s[k][e]));
+              for (int e = 1; e < 16; ++e)
+                if (first + e >= keys) s[e] = s[0];
             }
+            float m2[2] = {mx, mx};
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              m2[0] = max3(m2[0], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+              m2[1] = max3(m2[1], __uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
+            }
+            mx = fmaxf(m2[0], m2[1]);
           }
-          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
+          if (!exchange(mx, mo)) {
+            ok = false;
+            break;
+          }
+          mx = fmaxf(mx, mo) * sl2;
           if (c == c0) {
             m = mx;
           } else {
@@ -393,8 +416,8 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
               const float mn = grows ? mx : m, f = grows ? ex2(m - mn) : 1.f;
               l *= f;
               m = mn;
-#pragma unroll
-              for (int k = 0; k < 2 * DC; ++k) {
+#pragma unroll 1
+              for (int k = half; k < 2 * DC; k += 2) {
                 uint32_t a[32];
                 tmem_ld32_nowait(tmem + lane_off + Y::kTmemO + k * 32, a);
                 wait_ld();
@@ -405,30 +428,6 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
               }
             }
           }
-          float sum4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            if (k * 32 < keys) {
-              const bool tail = k * 32 + 32 > keys;
-#pragma unroll
-              for (int gr = 0; gr < 4; ++gr) {
-                float p[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  p[e] = ex2(fmaf(__uint_as_float(s[k][gr * 8 + e]), sl2, -m));
-                  if (tail && k * 32 + gr * 8 + e >= keys) p[e] = 0.f;
-                  sum4[e & 3] += p[e];
-                }
-                if (DROP) {
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) p[e] = (keep[k] >> (gr * 8 + e)) & 1u ? p[e] : 0.f;
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[k][gr * 4 + e] = pack2<T>(p[2 * e], p[2 * e + 1]);
-              }
-            }
-          }
-          l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
         }
         // the product of the previous chunk has read P (and, of the previous item, its O has been read)
         if (cc > 0 && !umma::mbar_wait(o_done, (cc - 1) & 1, 0x9a)) {
@@ -436,16 +435,49 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
           break;
         }
         if (!idle) {
+          uint64_t sum = pk2(0.f, 0.f);
+          const uint64_t sl22 = pk2(sl2, sl2), m22 = pk2(-m, -m);
+#pragma unroll 1
+          for (int first = half * 16; first < keys; first += 32) {
+            uint32_t s[16], p2[8];
+            tmem_ld16_nowait(src + first, s);
+            uint32_t mask[8];
+            if (DROP) {
 #pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            if (k * 32 < keys) {
-              uint8_t* tile = smem + Y::OFF_P + (k >> 1) * TILE;
-#pragma unroll
-              for (int gr = 0; gr < 4; ++gr)
-                *reinterpret_cast<uint4*>(tile + sw128(row, (k & 1) * 4 + gr)) =
-                    make_uint4(s[k][gr * 4], s[k][gr * 4 + 1], s[k][gr * 4 + 2], s[k][gr * 4 + 3]);
+              for (int gr = 0; gr < 2; ++gr) {  // drawn while the scores come
+                const uint4 r = rng((uint32_t)(kc + first) / 8 + gr, (uint32_t)pos, bh);
+                mask[gr * 4] = keep_mask2(r.x, drop.limit);
+                mask[gr * 4 + 1] = keep_mask2(r.y, drop.limit);
+                mask[gr * 4 + 2] = keep_mask2(r.z, drop.limit);
+                mask[gr * 4 + 3] = keep_mask2(r.w, drop.limit);
+              }
             }
+            wait_ld();
+            tie16(s);
+            if (first + 16 > keys) {  // keys behind the last: weights of zero
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (first + e >= keys) s[e] = 0xff800000u;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float a, b;
+              unpk2(fma2(pk2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sl22, m22), a, b);
+              a = ex2(a);
+              b = ex2(b);
+              sum = add2(sum, pk2(a, b));
+              p2[e] = pack2<T>(a, b);
+              if (DROP) p2[e] &= mask[e];
+            }
+            uint8_t* tile = smem + Y::OFF_P + (first >> 6) * TILE;
+#pragma unroll
+            for (int gr = 0; gr < 2; ++gr)
+              *reinterpret_cast<uint4*>(tile + sw128(row, ((first & 63) >> 3) + gr)) =
+                  make_uint4(p2[gr * 4], p2[gr * 4 + 1], p2[gr * 4 + 2], p2[gr * 4 + 3]);
           }
+          float a, b;
+          unpk2(sum, a, b);
+          l += a + b;
         }
         if (keys < g.width && sh.lengths != nullptr) {  // values behind the length: zeros, whatever they were
           const int st = cc % kStages;
@@ -457,48 +489,49 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
         }
         warp_arrive(p_full, true);
       }
-      if (!ok || !umma::mbar_wait(o_done, (cc - 1) & 1, 0x9c)) {
+      float lo = 0.f;
+      if (!ok || (!idle && !exchange(l, lo)) || !umma::mbar_wait(o_done, (cc - 1) & 1, 0x9c)) {
         abort_flag = 1;
         break;
       }
       umma::tc_fence_after();
+      // in one order for both threads, so that they agree to the last bit
+      l = half == 0 ? l + lo : lo + l;
       const float inv = (DROP ? drop.scale : 1.f) / l;
+#pragma unroll 1
+      for (int k = half; k < 2 * DC; k += 2) {
+        if (idle || k * 32 >= sh.dim) break;
+        uint32_t a[32];
+        tmem_ld32_nowait(tmem + lane_off + Y::kTmemO + k * 32, a);
+        wait_ld();
+        tie32(a);
+        const float* f = reinterpret_cast<const float*>(a);
+        if (valid) {
 #pragma unroll
-      for (int k = 0; k < 2 * DC; ++k) {
-        if (!idle && k * 32 < sh.dim) {
-          uint32_t a[32];
-          tmem_ld32_nowait(tmem + lane_off + Y::kTmemO + k * 32, a);
-          wait_ld();
-          tie32(a);
-          const float* f = reinterpret_cast<const float*>(a);
-          if (valid) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int d = k * 32 + i * 8;
-              if (d < sh.dim) {
-                if (g.splits > 1) {
-                  float4* out = reinterpret_cast<float4*>(part_o + prow * sh.dim + d);
-                  out[0] = make_float4(f[8 * i] * inv, f[8 * i + 1] * inv, f[8 * i + 2] * inv, f[8 * i + 3] * inv);
-                  out[1] = make_float4(f[8 * i + 4] * inv, f[8 * i + 5] * inv, f[8 * i + 6] * inv, f[8 * i + 7] * inv);
-                } else {
-                  *reinterpret_cast<uint4*>(dst + d) =
-                      make_uint4(pack2<T>(f[8 * i] * inv, f[8 * i + 1] * inv),
-                                 pack2<T>(f[8 * i + 2] * inv, f[8 * i + 3] * inv),
-                                 pack2<T>(f[8 * i + 4] * inv, f[8 * i + 5] * inv),
-                                 pack2<T>(f[8 * i + 6] * inv, f[8 * i + 7] * inv));
-                }
+          for (int i = 0; i < 4; ++i) {
+            const int d = k * 32 + i * 8;
+            if (d < sh.dim) {
+              if (g.splits > 1) {
+                float4* out = reinterpret_cast<float4*>(part_o + prow() * sh.dim + d);
+                out[0] = make_float4(f[8 * i] * inv, f[8 * i + 1] * inv, f[8 * i + 2] * inv, f[8 * i + 3] * inv);
+                out[1] = make_float4(f[8 * i + 4] * inv, f[8 * i + 5] * inv, f[8 * i + 6] * inv, f[8 * i + 7] * inv);
+              } else {
+                *reinterpret_cast<uint4*>(dst() + d) =
+                    make_uint4(pack2<T>(f[8 * i] * inv, f[8 * i + 1] * inv),
+                               pack2<T>(f[8 * i + 2] * inv, f[8 * i + 3] * inv),
+                               pack2<T>(f[8 * i + 4] * inv, f[8 * i + 5] * inv),
+                               pack2<T>(f[8 * i + 6] * inv, f[8 * i + 7] * inv));
               }
             }
           }
         }
       }
       warp_arrive(o_empty, false);
-      if (valid) {
+      if (valid && half == 0) {
         const float stat2 = m + log2f(l);
-        if (g.splits > 1) part_lse[prow] = stat2;
-        else lse[stat] = stat2;
+        if (g.splits > 1) part_lse[prow()] = stat2;
+        else lse[stat()] = -stat2;
       }
-      ++t;
     }
   }
   umma::tc_fence_before();
@@ -545,7 +578,7 @@ __global__ void __launch_bounds__(256)
   *reinterpret_cast<uint4*>(o + b * po.s_b + pos * po.s_n + head * po.s_h + d) =
       make_uint4(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv),
                  pack2<T>(acc[4] * inv, acc[5] * inv), pack2<T>(acc[6] * inv, acc[7] * inv));
-  if (d == 0) lse[bu * g.ldr + R] = any ? mx + log2f(w) : INFINITY;
+  if (d == 0) lse[bu * g.ldr + R] = any ? -(mx + log2f(w)) : -INFINITY;
 }
 
 // ------------------------------------------------------------ backward: dQ
@@ -722,7 +755,7 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
     const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const float sl2 = sh.scale * kLog2e, mult = DROP ? drop.scale : 1.f;
-    const Philox rng = DROP ? Philox(drop) : Philox(DropArgs{nullptr, 0, 0, 0.f});
+    const Philox rng(DROP ? drop : DropArgs{});
     uint32_t cc = 0, t = 0;
     for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
       const Item it = forward_item(item, g);
@@ -730,10 +763,10 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
       const int R = it.blk * BM + row, pos = R >> g.gp_shift, head = (it.u << g.gp_shift) + (R & gp_mask);
       const bool valid = R < g.rows, idle = it.blk * BM + quarter * 32 >= g.rows;
       const int64_t stat = (int64_t)(it.b * g.units + it.u) * g.ldr + R;
-      T* dst = dq + it.b * pdq.s_b + pos * pdq.s_n + head * pdq.s_h;
+      auto dst = [&] { return dq + it.b * pdq.s_b + pos * pdq.s_n + head * pdq.s_h; };
       if (nch == 0) {
         if (valid) {
-          for (int d = half * 8; d < sh.dim; d += 16) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
+          for (int d = half * 8; d < sh.dim; d += 16) *reinterpret_cast<uint4*>(dst() + d) = make_uint4(0, 0, 0, 0);
           if (half == 0) delta[stat] = 0.f;
         }
         continue;
@@ -746,7 +779,7 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
         const int d = (2 * i + half) * 8;
         orow[i] = valid && d < sh.dim ? *reinterpret_cast<const uint4*>(osrc + d) : make_uint4(0, 0, 0, 0);
       }
-      if (valid) lse2 = lse[stat];
+      if (valid) lse2 = -lse[stat];
       if (!umma::mbar_wait(qd_full, t & 1, 0xa8)) {
         abort_flag = 1;
         break;
@@ -769,46 +802,60 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
         break;
       }
       const float dsum = xs[row] + xs[BM + row];
-      if (valid && half == 0) delta[stat] = dsum;
+      if (valid && half == 0) delta[stat] = -dsum;
       warp_arrive(qd_empty, false);
       const uint32_t bh = (uint32_t)(it.b * sh.heads + head);
       bool ok = true;
       for (int c = 0; c < nch; ++c, ++cc) {
         const int kc = c * BC, keys = min(BC, len - kc), k0 = half * 32;
         const bool work = !idle && k0 < keys;
-        uint32_t keep = 0xffffffffu;  // drawn while the products run
-        if (DROP && work) keep = keep_word(rng, drop.limit, kc + k0, pos, bh);
         if (!umma::mbar_wait(sd_full, cc & 1, 0xaa)) {
           ok = false;
           break;
         }
         umma::tc_fence_after();
         uint32_t packed[16];
-        const bool tail = k0 + 32 > keys;
+        const uint64_t sl22 = pk2(sl2, sl2), lse22 = pk2(-lse2, -lse2), d22 = pk2(-dsum, -dsum), mult22 = pk2(mult, mult);
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {  // 16 columns at a time: 32 accumulator registers live
           uint32_t su[16], du[16];
           if (work) {
             tmem_ld16_nowait(tmem + lane_off + k0 + hh * 16, su);
             tmem_ld16_nowait(tmem + lane_off + Y::kTmemDP + k0 + hh * 16, du);
-            tmem_wait16(su, du);
-          }
-          if (hh == 1) warp_arrive(s_free, false);
-          if (work) {
+            uint32_t r[8];
+            if (DROP) {
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              float ds[2];
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int col = hh * 16 + i + e;
-                const float p = ex2(fmaf(__uint_as_float(su[i + e]), sl2, -lse2));
-                const float dp = (keep >> col) & 1u ? __uint_as_float(du[i + e]) * mult : 0.f;
-                ds[e] = p * (dp - dsum);
-                if (tail && k0 + col >= keys) ds[e] = 0.f;
+              for (int gr = 0; gr < 2; ++gr) {
+                const uint4 w = rng((uint32_t)(kc + k0) / 8 + hh * 2 + gr, (uint32_t)pos, bh);
+                r[gr * 4] = w.x;
+                r[gr * 4 + 1] = w.y;
+                r[gr * 4 + 2] = w.z;
+                r[gr * 4 + 3] = w.w;
               }
-              packed[hh * 8 + i / 2] = pack2<T>(ds[0], ds[1]);
+            }
+            tmem_wait16(su, du);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              float d0 = __uint_as_float(du[2 * i]), d1 = __uint_as_float(du[2 * i + 1]), p0, p1;
+              unpk2(fma2(pk2(__uint_as_float(su[2 * i]), __uint_as_float(su[2 * i + 1])), sl22, lse22), p0, p1);
+              uint64_t t;
+              if (DROP) {
+                d0 = kept(r[i], 0, drop.high) ? d0 : 0.f;
+                d1 = kept(r[i], 1, drop.high) ? d1 : 0.f;
+                t = fma2(pk2(d0, d1), mult22, d22);
+              } else {
+                t = add2(pk2(d0, d1), d22);
+              }
+              unpk2(mul2(pk2(ex2(p0), ex2(p1)), t), p0, p1);
+              packed[hh * 8 + i] = pack2<T>(p0, p1);
+            }
+            if (k0 + 32 > keys) {  // keys behind the last
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (k0 + hh * 16 + i >= keys) packed[hh * 8 + i / 2] &= i & 1 ? 0x0000ffffu : 0u;
             }
           }
+          if (hh == 1) warp_arrive(s_free, false);
         }
         if (!umma::mbar_wait(ds_free, (cc & 1) ^ 1, 0xab)) {
           ok = false;
@@ -842,7 +889,7 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               if (d0 + 8 * i < sh.dim)
-                *reinterpret_cast<uint4*>(dst + d0 + 8 * i) =
+                *reinterpret_cast<uint4*>(dst() + d0 + 8 * i) =
                     make_uint4(pack2<T>(f[8 * i] * sh.scale, f[8 * i + 1] * sh.scale),
                                pack2<T>(f[8 * i + 2] * sh.scale, f[8 * i + 3] * sh.scale),
                                pack2<T>(f[8 * i + 4] * sh.scale, f[8 * i + 5] * sh.scale),
@@ -1046,20 +1093,20 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
     const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const float sl2 = sh.scale * kLog2e, mult = DROP ? drop.scale : 1.f;
-    const Philox rng = DROP ? Philox(drop) : Philox(DropArgs{nullptr, 0, 0, 0.f});
+    const Philox rng(DROP ? drop : DropArgs{});
     uint32_t cc = 0, t = 0;
     for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
       int blk, kh, b;
       at(item, blk, kh, b);
       const int len = sh.keys(b), j = blk * BM + row;
       const bool exists = j < sh.nk, live = j < len, idle = blk * BM + quarter * 32 >= len;
-      T* out_k = dk + b * pdk.s_b + j * pdk.s_n + kh * pdk.s_h;
-      T* out_v = dv + b * pdv.s_b + j * pdv.s_n + kh * pdv.s_h;
+      auto out_k = [&] { return dk + b * pdk.s_b + j * pdk.s_n + kh * pdk.s_h; };
+      auto out_v = [&] { return dv + b * pdv.s_b + j * pdv.s_n + kh * pdv.s_h; };
       if (blk * BM >= len) {
         if (exists)
           for (int d = half * 8; d < sh.dim; d += 16) {
-            *reinterpret_cast<uint4*>(out_k + d) = make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(out_v + d) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(out_k() + d) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(out_v() + d) = make_uint4(0, 0, 0, 0);
           }
         continue;
       }
@@ -1084,45 +1131,59 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
         }
         umma::tc_fence_after();
         uint32_t pp[16], pd[16];
-        const bool tail = c0 + 32 > rows;
-        const float* ls = reinterpret_cast<const float*>(smem + Y::OFF_CH + s * Y::STAGE + Y::OFF_STAT) + c0;
-        const float* dl = ls + BC;
+        if (work) {
+          const uint64_t sl22 = pk2(sl2, sl2), mult22 = pk2(mult, mult);
+          const float* ls = reinterpret_cast<const float*>(smem + Y::OFF_CH + s * Y::STAGE + Y::OFF_STAT) + c0;
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {  // 16 columns at a time: 32 accumulator registers live
-          uint32_t su[16], du[16];
-          if (work) {
-            tmem_ld16_nowait(tmem + lane_off + c0 + hh * 16, su);
-            tmem_ld16_nowait(tmem + lane_off + Y::kTmemDP + c0 + hh * 16, du);
-            tmem_wait16(su, du);
-          }
-          if (hh == 1) warp_arrive(s_free, false);
-          if (work) {
+          for (int q8 = 0; q8 < 4; ++q8) {  // 8 columns at a time keep the registers under 96
+            uint32_t su[8], du[8];
+            tmem_ld8_nowait(tmem + lane_off + c0 + q8 * 8, su);
+            tmem_ld8_nowait(tmem + lane_off + Y::kTmemDP + c0 + q8 * 8, du);
+            tmem_wait8(su, du);
 #pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-              uint32_t bits = 0xffffffffu;
-              if (DROP) bits = __shfl_sync(0xffffffffu, word, (lane & 24) + hh * 4 + q4) >> (lane & 7);
-              const float4 l4 = *reinterpret_cast<const float4*>(ls + hh * 16 + 4 * q4);
-              const float4 d4 = *reinterpret_cast<const float4*>(dl + hh * 16 + 4 * q4);
-              const float lv[4] = {l4.x, l4.y, l4.z, l4.w}, dd[4] = {d4.x, d4.y, d4.z, d4.w};
-              float pt[4], ds[4];
+            for (int q4 = 0; q4 < 2; ++q4) {
+              uint32_t bits = 0;
+              if (DROP) bits = __shfl_sync(0xffffffffu, word, (lane & 24) + q8 * 2 + q4) >> (lane & 7);
+              const float4 l4 = *reinterpret_cast<const float4*>(ls + q8 * 8 + 4 * q4);
+              const float4 d4 = *reinterpret_cast<const float4*>(ls + BC + q8 * 8 + 4 * q4);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int i = 4 * q4 + e;
-                // queries behind the last: their statistics are someone else's, so select zeros outright
-                const bool dead = !live || (tail && c0 + hh * 16 + i >= rows);
-                const bool keep = (bits >> (8 * e)) & 1u;
-                const float p = ex2(fmaf(__uint_as_float(su[i]), sl2, -lv[e]));
-                const float dp = keep ? __uint_as_float(du[i]) * mult : 0.f;
-                pt[e] = dead || !keep ? 0.f : p;
-                ds[e] = dead ? 0.f : p * (dp - dd[e]);
+              for (int e = 0; e < 2; ++e) {
+                const int i = 4 * q4 + 2 * e;
+                // p = 2^(s - lse2), ds = p (dp - D); the statistics come negated
+                float p0, p1, d0 = __uint_as_float(du[i]), d1 = __uint_as_float(du[i + 1]);
+                unpk2(fma2(pk2(__uint_as_float(su[i]), __uint_as_float(su[i + 1])), sl22,
+                           e ? pk2(l4.z, l4.w) : pk2(l4.x, l4.y)), p0, p1);
+                p0 = ex2(p0);
+                p1 = ex2(p1);
+                const uint64_t nd = e ? pk2(d4.z, d4.w) : pk2(d4.x, d4.y);
+                uint64_t t;
+                float q0 = p0, q1 = p1;
+                if (DROP) {
+                  const bool k0 = bits & (1u << (16 * e)), k1 = bits & (1u << (16 * e + 8));
+                  d0 = k0 ? d0 : 0.f;
+                  d1 = k1 ? d1 : 0.f;
+                  q0 = k0 ? p0 : 0.f;
+                  q1 = k1 ? p1 : 0.f;
+                  t = fma2(pk2(d0, d1), mult22, nd);
+                } else {
+                  t = add2(pk2(d0, d1), nd);
+                }
+                unpk2(mul2(pk2(p0, p1), t), d0, d1);
+                pp[q8 * 4 + 2 * q4 + e] = pack2<T>(q0, q1);
+                pd[q8 * 4 + 2 * q4 + e] = pack2<T>(d0, d1);
               }
-              pp[hh * 8 + 2 * q4] = pack2<T>(pt[0], pt[1]);
-              pp[hh * 8 + 2 * q4 + 1] = pack2<T>(pt[2], pt[3]);
-              pd[hh * 8 + 2 * q4] = pack2<T>(ds[0], ds[1]);
-              pd[hh * 8 + 2 * q4 + 1] = pack2<T>(ds[2], ds[3]);
             }
           }
+          if (c0 + 32 > rows) {  // queries behind the last: their statistics are someone else's, so zeros outright
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c0 + i >= rows) {
+                pp[i / 2] &= i & 1 ? 0x0000ffffu : 0u;
+                pd[i / 2] &= i & 1 ? 0x0000ffffu : 0u;
+              }
+          }
         }
+        warp_arrive(s_free, false);
         if (!umma::mbar_wait(ps_free, (cc & 1) ^ 1, 0xba)) {
           ok = false;
           break;
@@ -1158,7 +1219,7 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
             }
             const float* f = reinterpret_cast<const float*>(a);
             const float by = which ? sh.scale : mult;
-            T* out = which ? out_k : out_v;
+            T* out = which ? out_k() : out_v();
             if (exists) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
@@ -1190,6 +1251,28 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
 // ------------------------------------------------------------------ host
 int64_t round_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
+// Key ranges per row tile: the count with the least estimated time, in
+// chunk times: waves of two CTAs per SM, each of its chunks and about two more
+// for a tile's start and end, and, with more than one range, the partial rows'
+// way out and back (about 5 GB a millisecond against 0.7 us per chunk) and the
+// second launch.
+int split_count(int64_t items, int nch, int64_t elements) {
+  if (items == 0) return 1;
+  const int64_t slots = (int64_t)num_sms() * 2;
+  int best = 1;
+  double least = 0.;
+  for (int s = 1; s <= kMaxSplits && (s == 1 || 2 * s <= nch); ++s) {
+    const int64_t waves = (items * s + slots - 1) / slots;
+    double t = (double)waves * ((nch + s - 1) / s + 2);
+    if (s > 1) t += (double)elements * s * 8 / 5e6 / 0.7 + 6.;
+    if (s == 1 || t < least) {
+      least = t;
+      best = s;
+    }
+  }
+  return best;
+}
+
 // Rows and tiles of a shape; `splits` from the tile count alone, so that the
 // workspace size, the forward and its join agree.
 Geometry geometry(const Shape& sh) {
@@ -1204,12 +1287,7 @@ Geometry geometry(const Shape& sh) {
   g.nblk = (g.rows + BM - 1) / BM;
   const int nch = (sh.nk + fw::kMaxW - 1) / fw::kMaxW;
   g.width = (int)round_up((sh.nk + nch - 1) / nch, 16);
-  // key ranges: enough items for two waves of two CTAs per SM, at least four chunks each
-  const int64_t items = (int64_t)sh.batch * g.units * g.nblk, want = (int64_t)num_sms() * 4;
-  int64_t s = items > 0 ? want / items : 1;
-  if (s > nch / 4) s = nch / 4;
-  if (s > kMaxSplits) s = kMaxSplits;
-  g.splits = s < 1 ? 1 : (int)s;
+  g.splits = split_count((int64_t)sh.batch * g.units * g.nblk, nch, (int64_t)sh.batch * g.units * g.rows * sh.dim);
   g.total = 0;
   return g;
 }

@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(kThreads)
   constexpr bool kTwo = MODE == kResidual || MODE == kGeluGrad;
   const int64_t stride = (int64_t)gridDim.x * kThreads;
   const int64_t groups = (n + 7) / 8, full = VEC ? n / 8 : 0;
-  const Philox rng = DROP ? Philox(drop) : Philox(DropArgs{nullptr, 0, 0, 0.f});
+  const Philox rng(DROP ? drop : DropArgs{});
   for (int64_t g0 = (int64_t)blockIdx.x * kThreads + threadIdx.x; g0 < groups; g0 += stride * kUnroll) {
     Pack8<T> pa[kUnroll], pb[kUnroll];
 #pragma unroll
@@ -64,13 +64,14 @@ __global__ void __launch_bounds__(kThreads)
     for (int u = 0; u < kUnroll; ++u) {
       const int64_t g = g0 + u * stride;
       if (g >= groups) break;
-      uint32_t keep = 0xffu;
-      if (DROP) keep = keep_bits(rng((uint32_t)g, (uint32_t)((uint64_t)g >> 32), 0xffffffffu), drop.limit);
+      uint4 r = make_uint4(0, 0, 0, 0);
+      if (DROP) r = rng((uint32_t)g, (uint32_t)((uint64_t)g >> 32), 0xffffffffu);
+      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
       Pack8<T> out;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         out.v[e] = Elem<T>::from_f(value<T, MODE>(Elem<T>::to_f(pa[u].v[e]), kTwo ? Elem<T>::to_f(pb[u].v[e]) : 0.f,
-                                                  (keep >> e) & 1u, DROP ? drop.scale : 1.f));
+                                                  !DROP || kept(w[e / 2], e & 1, drop.high), DROP ? drop.scale : 1.f));
       if (g < full) {
         reinterpret_cast<Pack8<T>*>(y)[g] = out;
       } else {

@@ -5,6 +5,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "f32x2.cuh"
 
 namespace pmb {
 namespace {
@@ -50,35 +51,6 @@ __device__ __forceinline__ float phi_cdf_fast(float x) {
 // phi(x) = exp(-x^2 / 2) / sqrt(2 pi) through ex2.approx
 __device__ __forceinline__ float phi_pdf_fast(float x) {
   return 0.39894228040143268f * ex2_approx(x * x * -0.72134752044448170f);  // -log2(e) / 2
-}
-
-// Pairs of fp32 values in one 64-bit register for the sm_100a packed
-// instructions fma / mul / add .rn.f32x2: each half is the IEEE fp32
-// operation of the scalar form, rounded the same way, so the paired
-// evaluation below gives the scalar functions' results bit for bit with half
-// the FMA-pipe instructions (the 16-bit GELU passes are issue-bound).
-__device__ __forceinline__ uint64_t pk2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpk2(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
 }
 
 // phi_cdf_fast of two values; t = x^2 is returned for the derivative's density term
