@@ -114,41 +114,52 @@ __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.
 // evenly): S (two buffers of 96 columns) and O (64 columns per 64 head
 // elements) then fill 256 tensor memory columns and two CTAs fit an SM.
 //
-// Eight row warps: two threads per row share its scores by blocks of 16
-// columns (even blocks, odd blocks), so four row warps per scheduler hide one
-// another's latencies.  They agree on the running maximum through shared
-// memory once per chunk; sums stay apart until the end.
+// A row thread owns a row: no exchange between threads.  It takes the row's
+// maximum, then turns 32 scores at a time into probabilities and writes them,
+// as 16-bit pairs, over the scores just read: P is the product's A operand
+// straight from tensor memory (no shared memory and no proxy fence between
+// the two products), and S of the next chunk sits in the other buffer, so the
+// row warps wait for neither product.  Measured per chunk and CTA before this
+// form, with P in shared memory and two threads per row: 4000 cycles, of
+// which 1500 arithmetic, 550 the threads' exchange, 550 waiting for the
+// previous product to release P, 360 fences.
 //
-// The MMA lane issues S of chunk c + 1 before O += P V of chunk c, so scores
-// are ready while the row warps work.  O stays in tensor memory; the running
-// maximum moves only when a row's grows by more than 8 (a factor 256 in P,
-// harmless in fp32 sums and 16-bit P), which after the first chunks is rare,
-// and then the row threads rescale O themselves.  P is rounded to the input
-// type (as in attention.cu); the row sums add the unrounded values before
-// dropout, whose scale is applied once at the end.
-//
-// K and V have separate rings: a K stage is free as soon as its scores are
-// formed.
+// O stays in tensor memory; the running maximum moves only when a row's grows
+// by more than 8 (a factor 256 in P, harmless in fp32 sums and 16-bit P),
+// which after the first chunks is rare, and then the row threads rescale O
+// themselves.  P is rounded to the input type (as in attention.cu); the row
+// sums add the unrounded values before dropout, whose scale is applied once
+// at the end.
 namespace fw {
-constexpr int kRowWarps = 8;
-constexpr int kThreads = 64 + 32 * kRowWarps;
+constexpr int kThreads = 192;
 constexpr int kMaxW = 96;
-constexpr int kStages = 2;
+constexpr int kStages = 3;        // K and V rings
 constexpr int SUB = kMaxW * 128;  // one 64-element sub-tile of a K or V stage
 template <int DC>
 struct L {
-  static constexpr int OFF_K = DC * TILE;
+  static constexpr int OFF_K = 2 * DC * TILE;               // two Q tiles
   static constexpr int OFF_V = OFF_K + kStages * DC * SUB;
-  static constexpr int OFF_P = OFF_V + kStages * DC * SUB;  // 128 rows x 96 keys: two sub-tiles
-  static constexpr int OFF_X = OFF_P + 2 * TILE;            // [2 turns][2 halves][128] row values exchanged
-  static constexpr int OFF_BAR = OFF_X + 2048;
+  static constexpr int OFF_BAR = OFF_V + kStages * DC * SUB;
   static constexpr int SMEM = OFF_BAR + 256 + 1024;
   static constexpr uint32_t kTmemO = 2 * kMaxW;
   static constexpr uint32_t kCols = DC == 1 ? 256 : 512;
 };
-constexpr int kBars = 2 + 4 * kStages + 2 + 3 + 4;
+constexpr int kBars = 4 + 4 * kStages + 2 + 5;
 constexpr float kRescale = 8.f;
 }  // namespace fw
+
+// Position in a ring of N stages.
+template <int N>
+struct Ring {
+  int s = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++s == N) {
+      s = 0;
+      phase ^= 1;
+    }
+  }
+};
 
 struct Item {
   int b, u, blk, split;
@@ -187,37 +198,35 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Y::OFF_BAR);
-  uint64_t* q_full = bars;
-  uint64_t* q_empty = bars + 1;
-  uint64_t* k_full = bars + 2;
+  uint64_t* q_full = bars;         // [2]
+  uint64_t* q_empty = q_full + 2;  // [2]
+  uint64_t* k_full = q_empty + 2;
   uint64_t* k_empty = k_full + kStages;
   uint64_t* v_full = k_empty + kStages;
   uint64_t* v_empty = v_full + kStages;
   uint64_t* s_full = v_empty + kStages;  // [2]
-  uint64_t* p_full = s_full + 2;
-  uint64_t* o_done = p_full + 1;
-  uint64_t* o_empty = o_done + 1;
-  uint64_t* pair = o_empty + 1;  // [4]: the two warps of a lane quarter
+  uint64_t* p_full = s_full + 2;         // [2]: a warp may be one chunk ahead of another
+  uint64_t* o_done = p_full + 2;         // [2], for the same reason
+  uint64_t* o_empty = o_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
-  float* xs = reinterpret_cast<float*>(smem + Y::OFF_X);
   __shared__ int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gp_mask = (1 << g.gp_shift) - 1;
   if (threadIdx.x == 0) {
-    umma::mbar_init(q_full, 1);
-    umma::mbar_init(q_empty, 1);
-    for (int i = 0; i < 4; ++i) umma::mbar_init(&pair[i], 2);
+    for (int i = 0; i < 2; ++i) {
+      umma::mbar_init(&q_full[i], 1);
+      umma::mbar_init(&q_empty[i], 1);
+      umma::mbar_init(&s_full[i], 1);
+      umma::mbar_init(&p_full[i], 4);
+      umma::mbar_init(&o_done[i], 1);
+    }
     for (int s = 0; s < kStages; ++s) {
       umma::mbar_init(&k_full[s], 1);
       umma::mbar_init(&k_empty[s], 1);
       umma::mbar_init(&v_full[s], 1);
       umma::mbar_init(&v_empty[s], 1);
     }
-    umma::mbar_init(&s_full[0], 1);
-    umma::mbar_init(&s_full[1], 1);
-    umma::mbar_init(p_full, kRowWarps);
-    umma::mbar_init(o_done, 1);
-    umma::mbar_init(o_empty, kRowWarps);
+    umma::mbar_init(o_empty, 4);
     abort_flag = 0;
     umma::fence_barrier_init();
   }
@@ -228,68 +237,68 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
-    if (lane == 0) {  // Q tiles
+    if (lane == 0) {
       umma::tma_prefetch(&tmQ);
-      uint32_t t = 0;
-      for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
+      umma::tma_prefetch(&tmK);
+      umma::tma_prefetch(&tmV);
+      Ring<kStages> kv;
+      Ring<2> q;
+      bool ok = true;
+      auto load = [&](const CUtensorMap* map, uint64_t* full, uint64_t* empty, int off, int c, const Item& it) -> bool {
+        if (!umma::mbar_wait(&empty[kv.s], kv.phase ^ 1, 0x92)) return false;
+        umma::mbar_arrive_expect_tx(&full[kv.s], DC * g.width * 128);
+#pragma unroll
+        for (int dc = 0; dc < DC; ++dc)
+          umma::tma_load_4d(smem + off + (kv.s * DC + dc) * SUB, map, &full[kv.s], dc * 64, c * g.width,
+                            it.u / g.kv_units, it.b);
+        return true;
+      };
+      for (int item = blockIdx.x; item < g.total && ok && !abort_flag; item += gridDim.x) {
         const Item it = forward_item(item, g);
         int c0, c1;
         chunk_range(sh.keys(it.b), it, g, c0, c1);
         if (c0 >= c1) continue;
-        if (!umma::mbar_wait(q_empty, (t & 1) ^ 1, 0x91)) {
-          abort_flag = 1;
+        if (!umma::mbar_wait(&q_empty[q.s], q.phase ^ 1, 0x91)) {
+          ok = false;
           break;
         }
-        umma::mbar_arrive_expect_tx(q_full, DC * TILE);
+        umma::mbar_arrive_expect_tx(&q_full[q.s], DC * TILE);
 #pragma unroll
         for (int dc = 0; dc < DC; ++dc)
-          umma::tma_load_5d(smem + dc * TILE, &tmQ, q_full, dc * 64, 0, (it.blk * BM) >> g.gp_shift, it.u, it.b);
-        ++t;
+          umma::tma_load_5d(smem + (q.s * DC + dc) * TILE, &tmQ, &q_full[q.s], dc * 64, 0, (it.blk * BM) >> g.gp_shift,
+                            it.u, it.b);
+        for (int c = c0; c < c1 && ok; ++c, kv.next())
+          ok = load(&tmK, k_full, k_empty, Y::OFF_K, c, it) && load(&tmV, v_full, v_empty, Y::OFF_V, c, it);
+        q.next();
       }
-    } else if (lane <= 2) {  // K chunks (lane 1), V chunks (lane 2)
-      const CUtensorMap* map = lane == 1 ? &tmK : &tmV;
-      uint64_t* full = lane == 1 ? k_full : v_full;
-      uint64_t* empty = lane == 1 ? k_empty : v_empty;
-      uint8_t* ring = smem + (lane == 1 ? Y::OFF_K : Y::OFF_V);
-      umma::tma_prefetch(map);
-      uint32_t cc = 0;
-      for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
-        const Item it = forward_item(item, g);
-        int c0, c1;
-        chunk_range(sh.keys(it.b), it, g, c0, c1);
-        for (int c = c0; c < c1; ++c, ++cc) {
-          const int s = cc % kStages;
-          if (!umma::mbar_wait(&empty[s], ((cc / kStages) & 1) ^ 1, 0x92)) {
-            abort_flag = 1;
-            break;
-          }
-          umma::mbar_arrive_expect_tx(&full[s], DC * g.width * 128);
-#pragma unroll
-          for (int dc = 0; dc < DC; ++dc)
-            umma::tma_load_4d(ring + (s * DC + dc) * SUB, map, &full[s], dc * 64, c * g.width, it.u / g.kv_units,
-                              it.b);
-        }
-      }
+      if (!ok) abort_flag = 1;
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      // O += P V of the chunk issued last; first / number of an item decide the accumulator
+      // O += P V of the chunk whose scores were issued last
       struct Pending {
         bool live, first;
         int keys;
         uint32_t t;
       } prev{false, false, 0, 0};
-      uint32_t cc = 0, t = 0;
+      uint32_t cc = 0, t = 0;  // chunks and items so far
+      Ring<kStages> kr, vr;
+      Ring<2> q;
       auto issue_o = [&](uint32_t c) -> bool {
-        const int s = c % kStages;
-        if (!umma::mbar_wait(p_full, c & 1, 0x94) || !umma::mbar_wait(&v_full[s], (c / kStages) & 1, 0x95)) return false;
+        if (!umma::mbar_wait(&p_full[c & 1], (c >> 1) & 1, 0x94) || !umma::mbar_wait(&v_full[vr.s], vr.phase, 0x95)) return false;
         if (prev.first && !umma::mbar_wait(o_empty, (prev.t & 1) ^ 1, 0x96)) return false;
         umma::tc_fence_after();
-        mma_rows<DC>(tmem + Y::kTmemO, umma::smem_u32(smem + Y::OFF_P),
-                     umma::smem_u32(smem + Y::OFF_V + s * DC * SUB), SUB, Desc<T>::MN, (prev.keys + 15) >> 4,
-                     !prev.first);
-        umma::mma_commit(o_done);
-        umma::mma_commit(&v_empty[s]);
+        const uint32_t v = umma::smem_u32(smem + Y::OFF_V + vr.s * DC * SUB), p = tmem + (c & 1) * kMaxW;
+        const int ksteps = (prev.keys + 15) >> 4;
+        for (int ks = 0; ks < ksteps; ++ks)
+#pragma unroll
+          for (int dc = 0; dc < DC; ++dc)
+            umma::mma_f16_ts(tmem + Y::kTmemO + dc * 64, p + ks * 8,
+                             umma::smem_desc_sw128(v + dc * SUB + ks * 2048, 16, 1024), Desc<T>::MN,
+                             (!prev.first || ks) ? 1u : 0u);
+        umma::mma_commit(&o_done[c & 1]);
+        umma::mma_commit(&v_empty[vr.s]);
+        vr.next();
         return true;
       };
       bool ok = true;
@@ -299,50 +308,43 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
         int c0, c1;
         chunk_range(len, it, g, c0, c1);
         if (c0 >= c1) continue;
-        if (!umma::mbar_wait(q_full, t & 1, 0x93)) {
+        if (!umma::mbar_wait(&q_full[q.s], q.phase, 0x93)) {
           ok = false;
           break;
         }
         for (int c = c0; c < c1; ++c, ++cc) {
-          const int s = cc % kStages, keys = min(g.width, len - c * g.width);
-          if (!umma::mbar_wait(&k_full[s], (cc / kStages) & 1, 0x97)) {
+          const int keys = min(g.width, len - c * g.width);
+          // the buffer still holds P of the chunk before the previous one until its product is done
+          if (!umma::mbar_wait(&k_full[kr.s], kr.phase, 0x97) || (cc > 1 && !umma::mbar_wait(&o_done[cc & 1], ((cc >> 1) - 1) & 1, 0x9a))) {
             ok = false;
             break;
           }
           umma::tc_fence_after();
-          mma_scores<DC>(tmem + (cc & 1) * kMaxW, umma::smem_u32(smem), TILE,
-                         umma::smem_u32(smem + Y::OFF_K + s * DC * SUB), SUB, Desc<T>::kk((keys + 15) & ~15));
+          mma_scores<DC>(tmem + (cc & 1) * kMaxW, umma::smem_u32(smem + q.s * DC * TILE), TILE,
+                         umma::smem_u32(smem + Y::OFF_K + kr.s * DC * SUB), SUB, Desc<T>::kk((keys + 15) & ~15));
           umma::mma_commit(&s_full[cc & 1]);
-          umma::mma_commit(&k_empty[s]);
-          if (c == c1 - 1) umma::mma_commit(q_empty);
+          umma::mma_commit(&k_empty[kr.s]);
+          kr.next();
+          if (c == c1 - 1) umma::mma_commit(&q_empty[q.s]);
           if (prev.live && !issue_o(cc - 1)) {
             ok = false;
             break;
           }
           prev = Pending{true, c == c0, keys, t};
         }
+        q.next();
         ++t;
       }
       if (ok && prev.live) ok = issue_o(cc - 1);
       if (!ok) abort_flag = 1;
     }
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane;
-    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     const float sl2 = sh.scale * kLog2e;
     const Philox rng(DROP ? drop : DropArgs{});
-    uint32_t cc = 0, turn = 0;
-    // both threads of a row leave a value and take the other's
-    auto exchange = [&](float mine, float& other) -> bool {
-      float* slot = xs + (turn & 1) * 256;
-      slot[half * 128 + row] = mine;
-      __syncwarp();
-      if (lane == 0) umma::mbar_arrive(&pair[quarter]);
-      if (!umma::mbar_wait(&pair[quarter], turn & 1, 0x9d)) return false;
-      other = slot[(half ^ 1) * 128 + row];
-      ++turn;
-      return true;
-    };
+    uint32_t cc = 0;
+    Ring<kStages> vr;
     for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
       const Item it = forward_item(item, g);
       const int len = sh.keys(it.b);
@@ -357,11 +359,11 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
       auto dst = [&] { return o + it.b * po.s_b + pos * po.s_n + head * po.s_h; };
       if (c0 >= c1) {
         if (valid) {
-          if (g.splits == 1)
-            for (int d = half * 8; d < sh.dim; d += 16) *reinterpret_cast<uint4*>(dst() + d) = make_uint4(0, 0, 0, 0);
-          if (half == 0) {
-            if (g.splits > 1) part_lse[prow()] = -INFINITY;
-            else lse[stat()] = -INFINITY;
+          if (g.splits > 1) {
+            part_lse[prow()] = -INFINITY;
+          } else {
+            for (int d = 0; d < sh.dim; d += 8) *reinterpret_cast<uint4*>(dst() + d) = make_uint4(0, 0, 0, 0);
+            lse[stat()] = -INFINITY;
           }
         }
         continue;
@@ -369,46 +371,40 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
       const uint32_t bh = (uint32_t)(it.b * sh.heads + head);
       float m = -INFINITY, l = 0.f;
       bool ok = true;
-      for (int c = c0; c < c1; ++c, ++cc) {
+      for (int c = c0; c < c1; ++c, ++cc, vr.next()) {
         const int kc = c * g.width, keys = min(g.width, len - kc);
         if (!umma::mbar_wait(&s_full[cc & 1], (cc >> 1) & 1, 0x98)) {
           ok = false;
           break;
         }
         umma::tc_fence_after();
-        const uint32_t src = tmem + lane_off + (cc & 1) * kMaxW;
+        const uint32_t src = lanes + (cc & 1) * kMaxW;
         if (!idle) {
-          float mx = -INFINITY, mo;
+          float mx = -INFINITY;
 #pragma unroll 1
-          for (int first = half * 16; first < keys; first += 32) {
-            uint32_t s[16];
-            tmem_ld16_nowait(src + first, s);
+          for (int first = 0; first < keys; first += 32) {
+            uint32_t s[32];
+            tmem_ld32_nowait(src + first, s);
             wait_ld();
-            tie16(s);
-            if (first + 16 > keys) {
+            tie32(s);
+            if (first + 32 > keys) {
 #pragma unroll
-              for (int e = 1; e < 16; ++e)
+              for (int e = 1; e < 32; ++e)
                 if (first + e >= keys) s[e] = s[0];
             }
-            float m2[2] = {mx, mx};
+            float m4[4] = {mx, mx, mx, mx};
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-              m2[0] = max3(m2[0], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-              m2[1] = max3(m2[1], __uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
-            }
-            mx = fmaxf(m2[0], m2[1]);
+            for (int e = 0; e < 32; e += 2)
+              m4[(e >> 1) & 3] = max3(m4[(e >> 1) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+            mx = max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);
           }
-          if (!exchange(mx, mo)) {
-            ok = false;
-            break;
-          }
-          mx = fmaxf(mx, mo) * sl2;
+          mx *= sl2;
           if (c == c0) {
             m = mx;
           } else {
             const bool grows = mx > m + kRescale;
             if (__any_sync(0xffffffffu, grows)) {
-              if (!umma::mbar_wait(o_done, (cc - 1) & 1, 0x99)) {
+              if (!umma::mbar_wait(&o_done[(cc - 1) & 1], ((cc - 1) >> 1) & 1, 0x99)) {
                 ok = false;
                 break;
               }
@@ -417,34 +413,27 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
               l *= f;
               m = mn;
 #pragma unroll 1
-              for (int k = half; k < 2 * DC; k += 2) {
-                uint32_t a[32];
-                tmem_ld32_nowait(tmem + lane_off + Y::kTmemO + k * 32, a);
+              for (int k = 0; k < 4 * DC; ++k) {
+                uint32_t a[16];
+                tmem_ld16_nowait(lanes + Y::kTmemO + k * 16, a);
                 wait_ld();
-                tie32(a);
+                tie16(a);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(__uint_as_float(a[e]) * f);
-                umma::tmem_st32(tmem + lane_off + Y::kTmemO + k * 32, a);
+                for (int e = 0; e < 16; ++e) a[e] = __float_as_uint(__uint_as_float(a[e]) * f);
+                umma::tmem_st16(lanes + Y::kTmemO + k * 16, a);
               }
             }
           }
-        }
-        // the product of the previous chunk has read P (and, of the previous item, its O has been read)
-        if (cc > 0 && !umma::mbar_wait(o_done, (cc - 1) & 1, 0x9a)) {
-          ok = false;
-          break;
-        }
-        if (!idle) {
           uint64_t sum = pk2(0.f, 0.f);
           const uint64_t sl22 = pk2(sl2, sl2), m22 = pk2(-m, -m);
 #pragma unroll 1
-          for (int first = half * 16; first < keys; first += 32) {
-            uint32_t s[16], p2[8];
-            tmem_ld16_nowait(src + first, s);
-            uint32_t mask[8];
+          for (int first = 0; first < keys; first += 32) {
+            uint32_t s[32], p2[16];
+            tmem_ld32_nowait(src + first, s);
+            uint32_t mask[16];
             if (DROP) {
 #pragma unroll
-              for (int gr = 0; gr < 2; ++gr) {  // drawn while the scores come
+              for (int gr = 0; gr < 4; ++gr) {  // drawn while the scores come
                 const uint4 r = rng((uint32_t)(kc + first) / 8 + gr, (uint32_t)pos, bh);
                 mask[gr * 4] = keep_mask2(r.x, drop.limit);
                 mask[gr * 4 + 1] = keep_mask2(r.y, drop.limit);
@@ -453,14 +442,14 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
               }
             }
             wait_ld();
-            tie16(s);
-            if (first + 16 > keys) {  // keys behind the last: weights of zero
+            tie32(s);
+            if (first + 32 > keys) {  // keys behind the last: weights of zero
 #pragma unroll
-              for (int e = 0; e < 16; ++e)
+              for (int e = 0; e < 32; ++e)
                 if (first + e >= keys) s[e] = 0xff800000u;
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < 16; ++e) {
               float a, b;
               unpk2(fma2(pk2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sl22, m22), a, b);
               a = ex2(a);
@@ -469,40 +458,35 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
               p2[e] = pack2<T>(a, b);
               if (DROP) p2[e] &= mask[e];
             }
-            uint8_t* tile = smem + Y::OFF_P + (first >> 6) * TILE;
-#pragma unroll
-            for (int gr = 0; gr < 2; ++gr)
-              *reinterpret_cast<uint4*>(tile + sw128(row, ((first & 63) >> 3) + gr)) =
-                  make_uint4(p2[gr * 4], p2[gr * 4 + 1], p2[gr * 4 + 2], p2[gr * 4 + 3]);
+            umma::tmem_st16(src + first / 2, p2);  // over scores this warp has read
           }
+          umma::tmem_wait_st();
           float a, b;
           unpk2(sum, a, b);
           l += a + b;
         }
+        bool zeroed = false;
         if (keys < g.width && sh.lengths != nullptr) {  // values behind the length: zeros, whatever they were
-          const int st = cc % kStages;
-          if (!umma::mbar_wait(&v_full[st], (cc / kStages) & 1, 0x9b)) {
+          if (!umma::mbar_wait(&v_full[vr.s], vr.phase, 0x9b)) {
             ok = false;
             break;
           }
-          zero_rows<DC>(smem + Y::OFF_V + st * DC * SUB, SUB, keys, (keys + 15) & ~15, threadIdx.x - 64);
+          zero_rows<DC>(smem + Y::OFF_V + vr.s * DC * SUB, SUB, keys, (keys + 15) & ~15, threadIdx.x - 64);
+          zeroed = true;
         }
-        warp_arrive(p_full, true);
+        warp_arrive(&p_full[cc & 1], zeroed);
       }
-      float lo = 0.f;
-      if (!ok || (!idle && !exchange(l, lo)) || !umma::mbar_wait(o_done, (cc - 1) & 1, 0x9c)) {
+      if (!ok || !umma::mbar_wait(&o_done[(cc - 1) & 1], ((cc - 1) >> 1) & 1, 0x9c)) {
         abort_flag = 1;
         break;
       }
       umma::tc_fence_after();
-      // in one order for both threads, so that they agree to the last bit
-      l = half == 0 ? l + lo : lo + l;
       const float inv = (DROP ? drop.scale : 1.f) / l;
 #pragma unroll 1
-      for (int k = half; k < 2 * DC; k += 2) {
+      for (int k = 0; k < 2 * DC; ++k) {
         if (idle || k * 32 >= sh.dim) break;
         uint32_t a[32];
-        tmem_ld32_nowait(tmem + lane_off + Y::kTmemO + k * 32, a);
+        tmem_ld32_nowait(lanes + Y::kTmemO + k * 32, a);
         wait_ld();
         tie32(a);
         const float* f = reinterpret_cast<const float*>(a);
@@ -527,7 +511,7 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
         }
       }
       warp_arrive(o_empty, false);
-      if (valid && half == 0) {
+      if (valid) {
         const float stat2 = m + log2f(l);
         if (g.splits > 1) part_lse[prow()] = stat2;
         else lse[stat()] = -stat2;
