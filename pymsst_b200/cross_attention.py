@@ -9,6 +9,7 @@ several positions (frame, band, channel).
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Sequence
 
 import torch
@@ -22,7 +23,7 @@ MAX_HEAD_DIM = 256
 
 def _plane_empty(b, h, n, d, dtype, device) -> torch.Tensor:
     """[b, h, n, d] view of a new [b, n, h, d] plane."""
-    return torch.empty(b, n, h, d, dtype=dtype, device=device).transpose(1, 2)
+    return torch.empty_strided((b, h, n, d), (n * h * d, d, h * d, 1), dtype=dtype, device=device)
 
 
 def _copy_plane(t: torch.Tensor) -> torch.Tensor:
@@ -43,12 +44,15 @@ def _plane(t: torch.Tensor) -> torch.Tensor:
     return t if ok else _copy_plane(t)
 
 
+_I64x12, _I64x24 = ctypes.c_int64 * 12, ctypes.c_int64 * 24
+
+
 def _strides(*planes: torch.Tensor):
     out: list[int] = []
     for t in planes:
         sb, sh, sn, _ = t.stride()
         out += (sb, sn, sh)
-    return nat.i64_array(out)
+    return (_I64x12 if len(out) == 12 else _I64x24)(*out)
 
 
 # ------------------------------------------------------------------- attention

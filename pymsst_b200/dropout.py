@@ -90,8 +90,8 @@ def _as_int64(value: int) -> int:
     return value - 2**64 if value >= 2**63 else value
 
 
-def _dropout(x, residual, threshold, key, site, name):
-    device = nat.require_cuda(x, residual, name=name)
+def _dropout(x, residual, threshold, key, site):
+    device = x.device
     x = x.contiguous()
     y = torch.empty_like(x)
     if residual is not None:
@@ -109,7 +109,7 @@ class DropoutFn(torch.autograd.Function):
     def forward(ctx, x, residual, threshold, key, site):
         ctx.threshold, ctx.site = threshold, site
         ctx.save_for_backward(key)
-        return _dropout(x, residual, threshold, key, site, "dropout")
+        return _dropout(x, residual, threshold, key, site)
 
     @staticmethod
     @once_differentiable
@@ -117,7 +117,7 @@ class DropoutFn(torch.autograd.Function):
         (key,) = ctx.saved_tensors
         gx = None
         if ctx.needs_input_grad[0]:
-            gx = _dropout(grad, None, ctx.threshold, key, ctx.site, "dropout.backward")
+            gx = _dropout(grad, None, ctx.threshold, key, ctx.site)
         return gx, grad if ctx.needs_input_grad[1] else None, None, None, None
 
 
@@ -132,13 +132,15 @@ def dropout(x: torch.Tensor, p: float, key: torch.Tensor | None = None, site: in
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError(f"dropout: residual must be {tuple(x.shape)} {x.dtype}, got {tuple(residual.shape)} "
                          f"{residual.dtype}")
+    nat.require_cuda(x, residual, name="dropout")
+    nat.dtype_code(x.dtype)
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
         return DropoutFn.apply(x, residual, threshold, key, site)
-    return _dropout(x, residual, threshold, key, site, "dropout")
+    return _dropout(x, residual, threshold, key, site)
 
 
 def _gelu_dropout(x, threshold, key, site):
-    device = nat.require_cuda(x, name="gelu_dropout")
+    device = x.device
     y = torch.empty_like(x)
     with on_device(device):
         nat.call("pmb_gelu_dropout_forward", x.data_ptr(), y.data_ptr(), x.numel(), threshold, nat.ptr(key), site,
@@ -174,6 +176,8 @@ def gelu_dropout(x: torch.Tensor, p: float, key: torch.Tensor | None = None, sit
     fp32, bf16 and fp16; see :func:`dropout` for the key."""
     threshold = drop_threshold(p)
     check_key(key, threshold, site, x.device, "gelu_dropout")
+    nat.require_cuda(x, name="gelu_dropout")
+    nat.dtype_code(x.dtype)
     if torch.is_grad_enabled() and x.requires_grad:
         return GeluDropoutFn.apply(x, threshold, key, site)
     return _gelu_dropout(x.contiguous(), threshold, key, site)
