@@ -76,16 +76,38 @@ __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t a_su
                     umma::smem_desc_sw128(b + dc * b_sub + kk * 32, 16, 1024), idesc, (dc || kk) ? 1u : 0u);
 }
 
-// D (+)= A B with A K-major (64-element sub-tiles TILE bytes apart) and B MN-major: its rows are the K index, its 64
-// head elements the N index, DC sub-tiles b_sub bytes apart into accumulators 64 columns apart.
+// D (+)= A B with A in tensor memory, 16-bit pairs in 32-bit columns, and B MN-major: its rows are the K index, its
+// 64 head elements the N index, DC sub-tiles b_sub bytes apart into accumulators 64 columns apart.
 template <int DC>
-__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t b_sub, uint32_t idesc, int ksteps,
-                                         bool accumulate) {
+__device__ __forceinline__ void mma_rows_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t b_sub, uint32_t idesc,
+                                            int ksteps, bool accumulate) {
   for (int ks = 0; ks < ksteps; ++ks)
 #pragma unroll
     for (int dc = 0; dc < DC; ++dc)
-      umma::mma_f16(d + dc * 64, umma::smem_desc_sw128(a + (ks >> 2) * TILE + (ks & 3) * 32, 16, 1024),
-                    umma::smem_desc_sw128(b + dc * b_sub + ks * 2048, 16, 1024), idesc, (accumulate || ks) ? 1u : 0u);
+      umma::mma_f16_ts(d + dc * 64, a + ks * 8, umma::smem_desc_sw128(b + dc * b_sub + ks * 2048, 16, 1024), idesc,
+                       (accumulate || ks) ? 1u : 0u);
+}
+
+// Elements [n, 32) of 16 packed pairs to zero.
+__device__ __forceinline__ void zero_tail(uint32_t (&p)[16], int n) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if (2 * i + 1 >= n) p[i] &= 0x0000ffffu;
+    if (2 * i >= n) p[i] = 0;
+  }
+}
+
+// 32 accumulator columns (times mul) to head elements [d0, d0 + 32) of a global row, as far as the head goes.
+template <typename T>
+__device__ __forceinline__ void store_row(T* row, int d0, int dim, const uint32_t (&a)[32], float mul) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float* f = reinterpret_cast<const float*>(a) + 8 * i;
+    if (d0 + 8 * i < dim)
+      *reinterpret_cast<uint4*>(row + d0 + 8 * i) =
+          make_uint4(pack2<T>(f[0] * mul, f[1] * mul), pack2<T>(f[2] * mul, f[3] * mul),
+                     pack2<T>(f[4] * mul, f[5] * mul), pack2<T>(f[6] * mul, f[7] * mul));
+  }
 }
 
 // Zero the 128-byte rows [first, rows) of DC sub-tiles, one row per thread.
@@ -318,14 +340,8 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
         if (!umma::mbar_wait(&p_full[c & 1], (c >> 1) & 1, 0x94) || !umma::mbar_wait(&v_full[vr.s], vr.phase, 0x95)) return false;
         if (prev.first && !umma::mbar_wait(o_empty, (prev.t & 1) ^ 1, 0x96)) return false;
         umma::tc_fence_after();
-        const uint32_t v = umma::smem_u32(smem + Y::OFF_V + vr.s * DC * SUB), p = tmem + (c & 1) * kMaxW;
-        const int ksteps = (prev.keys + 15) >> 4;
-        for (int ks = 0; ks < ksteps; ++ks)
-#pragma unroll
-          for (int dc = 0; dc < DC; ++dc)
-            umma::mma_f16_ts(tmem + Y::kTmemO + dc * 64, p + ks * 8,
-                             umma::smem_desc_sw128(v + dc * SUB + ks * 2048, 16, 1024), Desc<T>::MN,
-                             (!prev.first || ks) ? 1u : 0u);
+        mma_rows_ts<DC>(tmem + Y::kTmemO, tmem + (c & 1) * kMaxW, umma::smem_u32(smem + Y::OFF_V + vr.s * DC * SUB), SUB,
+                        Desc<T>::MN, (prev.keys + 15) >> 4, !prev.first);
         umma::mma_commit(&o_done[c & 1]);
         umma::mma_commit(&v_empty[vr.s]);
         vr.next();
@@ -524,25 +540,14 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
         tmem_ld32_nowait(lanes + Y::kTmemO + k * 32, a);
         wait_ld();
         tie32(a);
-        const float* f = reinterpret_cast<const float*>(a);
-        if (valid) {
+        if (valid && g.splits == 1) store_row<T>(dst(), k * 32, sh.dim, a, inv);
+        if (valid && g.splits > 1) {
+          const float* f = reinterpret_cast<const float*>(a);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int d = k * 32 + i * 8;
-            if (d < sh.dim) {
-              if (g.splits > 1) {
-                float4* out = reinterpret_cast<float4*>(part_o + prow() * sh.dim + d);
-                out[0] = make_float4(f[8 * i] * inv, f[8 * i + 1] * inv, f[8 * i + 2] * inv, f[8 * i + 3] * inv);
-                out[1] = make_float4(f[8 * i + 4] * inv, f[8 * i + 5] * inv, f[8 * i + 6] * inv, f[8 * i + 7] * inv);
-              } else {
-                *reinterpret_cast<uint4*>(dst() + d) =
-                    make_uint4(pack2<T>(f[8 * i] * inv, f[8 * i + 1] * inv),
-                               pack2<T>(f[8 * i + 2] * inv, f[8 * i + 3] * inv),
-                               pack2<T>(f[8 * i + 4] * inv, f[8 * i + 5] * inv),
-                               pack2<T>(f[8 * i + 6] * inv, f[8 * i + 7] * inv));
-              }
-            }
-          }
+          for (int i = 0; i < 8; ++i)
+            if (k * 32 + i * 4 < sh.dim)
+              *reinterpret_cast<float4*>(part_o + prow() * sh.dim + k * 32 + i * 4) =
+                  make_float4(f[4 * i] * inv, f[4 * i + 1] * inv, f[4 * i + 2] * inv, f[4 * i + 3] * inv);
         }
       }
       warp_arrive(o_empty, false);
@@ -601,32 +606,31 @@ __global__ void __launch_bounds__(256)
 }
 
 // ------------------------------------------------------------ backward: dQ
-// Item = 128 packed rows of a unit; keys in chunks of 64.  The MMA lane forms
-// S = Q K^T and dP = dO V^T of chunk c + 1 as soon as the row warps hold
-// chunk c's in registers, and dQ += dS K once dS is in shared memory.  Eight
-// row warps, two threads per row with 32 columns each, two CTAs per SM.
-// D = rowsum(dO * O) is formed once per item and kept for the dK / dV kernel.
+// Item = 128 packed rows of a unit; keys in chunks of 96.  S = Q K^T, dP =
+// dO V^T; the row threads (one per row) write dS, as 16-bit pairs, over the
+// scores they have read, and dQ += dS K takes it from there.  S of the next
+// chunk waits for that product (it overwrites dS); two CTAs per SM fill the
+// gap.  D = rowsum(dO * O) is formed once per item and kept for the dK / dV
+// kernel.
 namespace bw {
-constexpr int kRowWarps = 8;
-constexpr int kThreads = 64 + 32 * kRowWarps;
-constexpr int BC = 64;                 // chunk rows
-constexpr int CT = BC * 128;           // bytes of a chunk's 64-element sub-tile
+constexpr int kThreads = 192;
 }  // namespace bw
 
 namespace bq {
 constexpr int kStages = 3;
+constexpr int BC = 96;                 // keys per chunk
+constexpr int CT = BC * 128;           // bytes of a chunk's 64-element sub-tile
 template <int DC>
 struct L {
   static constexpr int OFF_DO = DC * TILE;
   static constexpr int OFF_KV = 2 * DC * TILE;             // stages of DC K sub-tiles, DC V sub-tiles
-  static constexpr int STAGE = 2 * DC * bw::CT;
-  static constexpr int OFF_DS = OFF_KV + kStages * STAGE;
-  static constexpr int OFF_X = OFF_DS + TILE;              // [2][128] fp32 halves of D
-  static constexpr int OFF_BAR = OFF_X + 1024;
+  static constexpr int STAGE = 2 * DC * CT;
+  static constexpr int OFF_BAR = OFF_KV + (DC == 1 ? kStages : kStages - 1) * STAGE;
+  static constexpr int kN = DC == 1 ? kStages : kStages - 1;
   static constexpr int SMEM = OFF_BAR + 256 + 1024;
-  static constexpr uint32_t kTmemDP = 64, kTmemDQ = 128, kCols = 256;
+  static constexpr uint32_t kTmemDP = BC, kTmemDQ = 2 * BC, kCols = DC == 1 ? 256 : 512;
 };
-constexpr int kBars = 2 + 2 * kStages + 7;
+constexpr int kBars = 2 + 2 * kStages + 5;
 }  // namespace bq
 
 template <typename T, int DC, bool DROP>
@@ -635,7 +639,6 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
                  const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                  const T* __restrict__ o, const float* __restrict__ lse, float* __restrict__ delta, T* __restrict__ dq,
                  Plane po, Plane pdq, Shape sh, Geometry g, DropArgs drop) {
-  using namespace bw;
   using namespace bq;
   using Y = bq::L<DC>;
   extern __shared__ uint8_t smem_raw[];
@@ -646,31 +649,26 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
   uint64_t* kv_full = bars + 2;
   uint64_t* kv_empty = kv_full + kStages;
   uint64_t* sd_full = kv_empty + kStages;
-  uint64_t* s_free = sd_full + 1;
-  uint64_t* ds_full = s_free + 1;
-  uint64_t* ds_free = ds_full + 1;
-  uint64_t* dq_full = ds_free + 1;
+  uint64_t* ds_full = sd_full + 1;
+  uint64_t* ds_done = ds_full + 1;
+  uint64_t* dq_full = ds_done + 1;
   uint64_t* dq_empty = dq_full + 1;
-  uint64_t* x_full = dq_empty + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
-  float* xs = reinterpret_cast<float*>(smem + Y::OFF_X);
   __shared__ int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gp_mask = (1 << g.gp_shift) - 1;
   if (threadIdx.x == 0) {
     umma::mbar_init(qd_full, 1);
-    umma::mbar_init(qd_empty, 1 + kRowWarps);
+    umma::mbar_init(qd_empty, 1 + 4);  // the products' commit and the row warps' reads of dO
     for (int s = 0; s < kStages; ++s) {
       umma::mbar_init(&kv_full[s], 1);
       umma::mbar_init(&kv_empty[s], 1);
     }
     umma::mbar_init(sd_full, 1);
-    umma::mbar_init(s_free, kRowWarps);
-    umma::mbar_init(ds_full, kRowWarps);
-    umma::mbar_init(ds_free, 1);
+    umma::mbar_init(ds_full, 4);
+    umma::mbar_init(ds_done, 1);
     umma::mbar_init(dq_full, 1);
-    umma::mbar_init(dq_empty, kRowWarps);
-    umma::mbar_init(x_full, kRowWarps);
+    umma::mbar_init(dq_empty, 4);
     abort_flag = 0;
     umma::fence_barrier_init();
   }
@@ -681,15 +679,20 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
-    if (lane == 0) {  // Q and dO tiles
+    if (lane == 0) {  // tiles of an item, then its chunks
       umma::tma_prefetch(&tmQ);
       umma::tma_prefetch(&tmDO);
+      umma::tma_prefetch(&tmK);
+      umma::tma_prefetch(&tmV);
       uint32_t t = 0;
-      for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
+      Ring<Y::kN> kv;
+      bool ok = true;
+      for (int item = blockIdx.x; item < g.total && ok && !abort_flag; item += gridDim.x) {
         const Item it = forward_item(item, g);
-        if (sh.keys(it.b) == 0) continue;
+        const int nch = (sh.keys(it.b) + BC - 1) / BC;
+        if (nch == 0) continue;
         if (!umma::mbar_wait(qd_empty, (t & 1) ^ 1, 0xa1)) {
-          abort_flag = 1;
+          ok = false;
           break;
         }
         umma::mbar_arrive_expect_tx(qd_full, 2 * DC * TILE);
@@ -699,71 +702,58 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
           umma::tma_load_5d(smem + dc * TILE, &tmQ, qd_full, dc * 64, 0, pos, it.u, it.b);
           umma::tma_load_5d(smem + Y::OFF_DO + dc * TILE, &tmDO, qd_full, dc * 64, 0, pos, it.u, it.b);
         }
-        ++t;
-      }
-    } else if (lane == 1) {  // K / V chunks
-      umma::tma_prefetch(&tmK);
-      umma::tma_prefetch(&tmV);
-      uint32_t cc = 0;
-      for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
-        const Item it = forward_item(item, g);
-        const int nch = (sh.keys(it.b) + BC - 1) / BC;
-        for (int c = 0; c < nch; ++c, ++cc) {
-          const int s = cc % kStages;
-          if (!umma::mbar_wait(&kv_empty[s], ((cc / kStages) & 1) ^ 1, 0xa2)) {
-            abort_flag = 1;
+        for (int c = 0; c < nch; ++c, kv.next()) {
+          if (!umma::mbar_wait(&kv_empty[kv.s], kv.phase ^ 1, 0xa2)) {
+            ok = false;
             break;
           }
-          uint8_t* dst = smem + Y::OFF_KV + s * Y::STAGE;
-          umma::mbar_arrive_expect_tx(&kv_full[s], Y::STAGE);
+          uint8_t* dst = smem + Y::OFF_KV + kv.s * Y::STAGE;
+          umma::mbar_arrive_expect_tx(&kv_full[kv.s], Y::STAGE);
 #pragma unroll
           for (int dc = 0; dc < DC; ++dc) {
-            umma::tma_load_4d(dst + dc * CT, &tmK, &kv_full[s], dc * 64, c * BC, it.u / g.kv_units, it.b);
-            umma::tma_load_4d(dst + (DC + dc) * CT, &tmV, &kv_full[s], dc * 64, c * BC, it.u / g.kv_units, it.b);
+            umma::tma_load_4d(dst + dc * CT, &tmK, &kv_full[kv.s], dc * 64, c * BC, it.u / g.kv_units, it.b);
+            umma::tma_load_4d(dst + (DC + dc) * CT, &tmV, &kv_full[kv.s], dc * 64, c * BC, it.u / g.kv_units, it.b);
           }
         }
+        ++t;
       }
+      if (!ok) abort_flag = 1;
     }
   } else if (warp == 1) {
     if (lane == 0) {
       uint32_t cc = 0, t = 0;
-      auto issue_s = [&](uint32_t c, int keys, bool last) -> bool {
-        const int s = c % kStages;
-        if (!umma::mbar_wait(&kv_full[s], (c / kStages) & 1, 0xa4)) return false;
-        if (!umma::mbar_wait(s_free, (c & 1) ^ 1, 0xa5)) return false;
-        umma::tc_fence_after();
-        const uint32_t k = umma::smem_u32(smem + Y::OFF_KV + s * Y::STAGE), idesc = Desc<T>::kk((keys + 15) & ~15);
-        mma_scores<DC>(tmem, umma::smem_u32(smem), TILE, k, CT, idesc);
-        mma_scores<DC>(tmem + Y::kTmemDP, umma::smem_u32(smem + Y::OFF_DO), TILE, k + DC * CT, CT, idesc);
-        umma::mma_commit(sd_full);
-        if (last) umma::mma_commit(qd_empty);
-        return true;
-      };
+      Ring<Y::kN> kv;
       bool ok = true;
       for (int item = blockIdx.x; item < g.total && ok && !abort_flag; item += gridDim.x) {
         const Item it = forward_item(item, g);
         const int len = sh.keys(it.b), nch = (len + BC - 1) / BC;
         if (nch == 0) continue;
-        if (!umma::mbar_wait(qd_full, t & 1, 0xa3) || !issue_s(cc, min(BC, len), nch == 1)) {
+        if (!umma::mbar_wait(qd_full, t & 1, 0xa3)) {
           ok = false;
           break;
         }
-        for (int c = 0; c < nch; ++c, ++cc) {
-          if (c + 1 < nch && !issue_s(cc + 1, min(BC, len - (c + 1) * BC), c + 2 == nch)) {
+        for (int c = 0; c < nch; ++c, ++cc, kv.next()) {
+          const int keys = min(BC, len - c * BC), ksteps = (keys + 15) >> 4;
+          if (!umma::mbar_wait(&kv_full[kv.s], kv.phase, 0xa4) ||
+              (cc > 0 && !umma::mbar_wait(ds_done, (cc - 1) & 1, 0xa5))) {
             ok = false;
             break;
           }
+          umma::tc_fence_after();
+          const uint32_t k = umma::smem_u32(smem + Y::OFF_KV + kv.s * Y::STAGE), idesc = Desc<T>::kk(ksteps * 16);
+          mma_scores<DC>(tmem, umma::smem_u32(smem), TILE, k, CT, idesc);
+          mma_scores<DC>(tmem + Y::kTmemDP, umma::smem_u32(smem + Y::OFF_DO), TILE, k + DC * CT, CT, idesc);
+          umma::mma_commit(sd_full);
+          if (c == nch - 1) umma::mma_commit(qd_empty);
           if (!umma::mbar_wait(ds_full, cc & 1, 0xa6) ||
               (c == 0 && !umma::mbar_wait(dq_empty, (t & 1) ^ 1, 0xa7))) {
             ok = false;
             break;
           }
           umma::tc_fence_after();
-          mma_rows<DC>(tmem + Y::kTmemDQ, umma::smem_u32(smem + Y::OFF_DS),
-                       umma::smem_u32(smem + Y::OFF_KV + (cc % kStages) * Y::STAGE), CT, Desc<T>::MN,
-                       (min(BC, len - c * BC) + 15) >> 4, c > 0);
-          umma::mma_commit(ds_free);
-          umma::mma_commit(&kv_empty[cc % kStages]);
+          mma_rows_ts<DC>(tmem + Y::kTmemDQ, tmem, k, CT, Desc<T>::MN, ksteps, c > 0);
+          umma::mma_commit(ds_done);
+          umma::mma_commit(&kv_empty[kv.s]);
           if (c == nch - 1) umma::mma_commit(dq_full);
         }
         ++t;
@@ -771,11 +761,12 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
       if (!ok) abort_flag = 1;
     }
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane;
-    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     const float sl2 = sh.scale * kLog2e, mult = DROP ? drop.scale : 1.f;
     const Philox rng(DROP ? drop : DropArgs{});
     uint32_t cc = 0, t = 0;
+    Ring<Y::kN> kv;
     for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
       const Item it = forward_item(item, g);
       const int len = sh.keys(it.b), nch = (len + BC - 1) / BC;
@@ -785,137 +776,101 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
       auto dst = [&] { return dq + it.b * pdq.s_b + pos * pdq.s_n + head * pdq.s_h; };
       if (nch == 0) {
         if (valid) {
-          for (int d = half * 8; d < sh.dim; d += 16) *reinterpret_cast<uint4*>(dst() + d) = make_uint4(0, 0, 0, 0);
-          if (half == 0) delta[stat] = 0.f;
+          for (int d = 0; d < sh.dim; d += 8) *reinterpret_cast<uint4*>(dst() + d) = make_uint4(0, 0, 0, 0);
+          delta[stat] = 0.f;
         }
         continue;
       }
-      uint4 orow[4 * DC];
-      float lse2 = 0.f;
+      // this row of O and its statistics, fetched while the tiles are in flight
+      uint4 orow[8 * DC];
+      float nlse = 0.f;
       const T* osrc = o + it.b * po.s_b + pos * po.s_n + head * po.s_h;
 #pragma unroll
-      for (int i = 0; i < 4 * DC; ++i) {
-        const int d = (2 * i + half) * 8;
-        orow[i] = valid && d < sh.dim ? *reinterpret_cast<const uint4*>(osrc + d) : make_uint4(0, 0, 0, 0);
-      }
-      if (valid) lse2 = -lse[stat];
+      for (int i = 0; i < 8 * DC; ++i)
+        orow[i] = valid && i * 8 < sh.dim ? *reinterpret_cast<const uint4*>(osrc + i * 8) : make_uint4(0, 0, 0, 0);
+      if (valid) nlse = lse[stat];
       if (!umma::mbar_wait(qd_full, t & 1, 0xa8)) {
         abort_flag = 1;
         break;
       }
-      float part = 0.f;
+      float ndsum = 0.f;  // -D
 #pragma unroll
-      for (int i = 0; i < 4 * DC; ++i) {
-        const int ch = 2 * i + half;
-        const uint4 d4 =
-            *reinterpret_cast<const uint4*>(smem + Y::OFF_DO + (ch >> 3) * TILE + sw128(row, ch & 7));
+      for (int i = 0; i < 8 * DC; ++i) {
+        const uint4 d4 = *reinterpret_cast<const uint4*>(smem + Y::OFF_DO + (i >> 3) * TILE + sw128(row, i & 7));
         const T* oe = reinterpret_cast<const T*>(&orow[i]);
         const T* de = reinterpret_cast<const T*>(&d4);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) part = fmaf(Elem<T>::to_f(oe[e]), Elem<T>::to_f(de[e]), part);
+        for (int e = 0; e < 8; ++e) ndsum = fmaf(-Elem<T>::to_f(oe[e]), Elem<T>::to_f(de[e]), ndsum);
       }
-      xs[half * BM + row] = part;
-      warp_arrive(x_full, false);
-      if (!umma::mbar_wait(x_full, t & 1, 0xa9)) {
-        abort_flag = 1;
-        break;
-      }
-      const float dsum = xs[row] + xs[BM + row];
-      if (valid && half == 0) delta[stat] = -dsum;
+      if (valid) delta[stat] = ndsum;
       warp_arrive(qd_empty, false);
       const uint32_t bh = (uint32_t)(it.b * sh.heads + head);
+      const uint64_t sl22 = pk2(sl2, sl2), nlse2 = pk2(nlse, nlse), nd2 = pk2(ndsum, ndsum), mult2 = pk2(mult, mult);
       bool ok = true;
-      for (int c = 0; c < nch; ++c, ++cc) {
-        const int kc = c * BC, keys = min(BC, len - kc), k0 = half * 32;
-        const bool work = !idle && k0 < keys;
+      for (int c = 0; c < nch; ++c, ++cc, kv.next()) {
+        const int kc = c * BC, keys = min(BC, len - kc);
         if (!umma::mbar_wait(sd_full, cc & 1, 0xaa)) {
           ok = false;
           break;
         }
         umma::tc_fence_after();
-        uint32_t packed[16];
-        const uint64_t sl22 = pk2(sl2, sl2), lse22 = pk2(-lse2, -lse2), d22 = pk2(-dsum, -dsum), mult22 = pk2(mult, mult);
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {  // 16 columns at a time: 32 accumulator registers live
-          uint32_t su[16], du[16];
-          if (work) {
-            tmem_ld16_nowait(tmem + lane_off + k0 + hh * 16, su);
-            tmem_ld16_nowait(tmem + lane_off + Y::kTmemDP + k0 + hh * 16, du);
-            uint32_t r[8];
+        if (!idle) {
+#pragma unroll 1
+          for (int first = 0; first < keys; first += 32) {
+            uint32_t su[32], du[32];
+            tmem_ld32_nowait(lanes + first, su);
+            tmem_ld32_nowait(lanes + Y::kTmemDP + first, du);
+            uint32_t w[16];
             if (DROP) {
 #pragma unroll
-              for (int gr = 0; gr < 2; ++gr) {
-                const uint4 w = rng((uint32_t)(kc + k0) / 8 + hh * 2 + gr, (uint32_t)pos, bh);
-                r[gr * 4] = w.x;
-                r[gr * 4 + 1] = w.y;
-                r[gr * 4 + 2] = w.z;
-                r[gr * 4 + 3] = w.w;
+              for (int gr = 0; gr < 4; ++gr) {  // drawn while the products come
+                const uint4 r = rng((uint32_t)(kc + first) / 8 + gr, (uint32_t)pos, bh);
+                w[gr * 4] = r.x;
+                w[gr * 4 + 1] = r.y;
+                w[gr * 4 + 2] = r.z;
+                w[gr * 4 + 3] = r.w;
               }
             }
-            tmem_wait16(su, du);
+            tmem_wait2(su, du);
+            uint32_t p2[16];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 16; ++i) {
               float d0 = __uint_as_float(du[2 * i]), d1 = __uint_as_float(du[2 * i + 1]), p0, p1;
-              unpk2(fma2(pk2(__uint_as_float(su[2 * i]), __uint_as_float(su[2 * i + 1])), sl22, lse22), p0, p1);
-              uint64_t t;
+              unpk2(fma2(pk2(__uint_as_float(su[2 * i]), __uint_as_float(su[2 * i + 1])), sl22, nlse2), p0, p1);
+              uint64_t x;
               if (DROP) {
-                d0 = kept(r[i], 0, drop.high) ? d0 : 0.f;
-                d1 = kept(r[i], 1, drop.high) ? d1 : 0.f;
-                t = fma2(pk2(d0, d1), mult22, d22);
+                d0 = kept(w[i], 0, drop.high) ? d0 : 0.f;
+                d1 = kept(w[i], 1, drop.high) ? d1 : 0.f;
+                x = fma2(pk2(d0, d1), mult2, nd2);
               } else {
-                t = add2(pk2(d0, d1), d22);
+                x = add2(pk2(d0, d1), nd2);
               }
-              unpk2(mul2(pk2(ex2(p0), ex2(p1)), t), p0, p1);
-              packed[hh * 8 + i] = pack2<T>(p0, p1);
+              unpk2(mul2(pk2(ex2(p0), ex2(p1)), x), p0, p1);
+              p2[i] = pack2<T>(p0, p1);
             }
-            if (k0 + 32 > keys) {  // keys behind the last
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (k0 + hh * 16 + i >= keys) packed[hh * 8 + i / 2] &= i & 1 ? 0x0000ffffu : 0u;
-            }
+            if (first + 32 > keys) zero_tail(p2, keys - first);
+            umma::tmem_st16(lanes + first / 2, p2);  // over scores this warp has read
           }
-          if (hh == 1) warp_arrive(s_free, false);
+          umma::tmem_wait_st();
         }
-        if (!umma::mbar_wait(ds_free, (cc & 1) ^ 1, 0xab)) {
-          ok = false;
-          break;
-        }
-        if (work) {
-#pragma unroll
-          for (int gr = 0; gr < 4; ++gr)
-            *reinterpret_cast<uint4*>(smem + Y::OFF_DS + sw128(row, half * 4 + gr)) =
-                make_uint4(packed[gr * 4], packed[gr * 4 + 1], packed[gr * 4 + 2], packed[gr * 4 + 3]);
-        }
-        if (keys < BC && sh.lengths != nullptr)  // S of this chunk is formed: its keys behind the length become zeros
-          zero_rows<DC>(smem + Y::OFF_KV + (cc % kStages) * Y::STAGE, CT, keys, (keys + 15) & ~15, threadIdx.x - 64);
-        warp_arrive(ds_full, true);
+        const bool pad = keys < BC && sh.lengths != nullptr;
+        if (pad)  // S of this chunk is formed: its keys behind the length become zeros
+          zero_rows<DC>(smem + Y::OFF_KV + kv.s * Y::STAGE, CT, keys, (keys + 15) & ~15, threadIdx.x - 64);
+        warp_arrive(ds_full, pad);
       }
       if (!ok || !umma::mbar_wait(dq_full, t & 1, 0xac)) {
         abort_flag = 1;
         break;
       }
       umma::tc_fence_after();
-#pragma unroll
-      for (int dc = 0; dc < DC; ++dc) {
-        const int d0 = dc * 64 + half * 32;
-        if (!idle && d0 < sh.dim) {
-          uint32_t a[32];
-          tmem_ld32_nowait(tmem + lane_off + Y::kTmemDQ + d0, a);
-          wait_ld();
-          tie32(a);
-          const float* f = reinterpret_cast<const float*>(a);
-          if (valid) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (d0 + 8 * i < sh.dim)
-                *reinterpret_cast<uint4*>(dst() + d0 + 8 * i) =
-                    make_uint4(pack2<T>(f[8 * i] * sh.scale, f[8 * i + 1] * sh.scale),
-                               pack2<T>(f[8 * i + 2] * sh.scale, f[8 * i + 3] * sh.scale),
-                               pack2<T>(f[8 * i + 4] * sh.scale, f[8 * i + 5] * sh.scale),
-                               pack2<T>(f[8 * i + 6] * sh.scale, f[8 * i + 7] * sh.scale));
-            }
-          }
-        }
+#pragma unroll 1
+      for (int k = 0; k < 2 * DC; ++k) {
+        if (idle || k * 32 >= sh.dim) break;
+        uint32_t a[32];
+        tmem_ld32_nowait(lanes + Y::kTmemDQ + k * 32, a);
+        wait_ld();
+        tie32(a);
+        if (valid) store_row<T>(dst(), k * 32, sh.dim, a, sh.scale);
       }
       warp_arrive(dq_empty, false);
       ++t;
@@ -932,27 +887,29 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
 // -------------------------------------------------------- backward: dK, dV
 // Item = 128 keys of a key / value head; the packed rows of all its units
 // come in chunks of 64 with their lse2 and D.  S^T = K Q^T and dP^T = V dO^T
-// put a key in each tensor memory lane; dV += P^T dO and dK += dS^T Q take
-// the row threads' 16-bit P^T and dS^T from shared memory.  The dropout bits
-// come in groups of eight keys of one query, that is of eight lanes: each
-// lane draws the groups of four of its 32 columns and the eight exchange the
-// keep bits by shuffles, so a group is still drawn once.
+// put a key in each tensor memory lane; the row threads write P^T and dS^T,
+// as 16-bit pairs, over the accumulators they have read, where dV += P^T dO
+// and dK += dS^T Q take them.  The dropout bits come in groups of eight keys
+// of one query, that is of eight lanes: each lane draws the groups of four of
+// 32 columns and the eight exchange the keep bits by shuffles, so a group is
+// still drawn once.
 namespace bk {
-constexpr int kStages = 2;
+constexpr int kStages = 4;
+constexpr int BC = 64;                 // packed rows per chunk
+constexpr int CT = BC * 128;
 template <int DC>
 struct L {
   static constexpr int OFF_V = DC * TILE;
   static constexpr int OFF_CH = 2 * DC * TILE;
-  static constexpr int OFF_STAT = 2 * DC * bw::CT;              // within a stage: lse2[64], D[64]
+  static constexpr int OFF_STAT = 2 * DC * CT;              // within a stage: -lse2[64], -D[64]
   static constexpr int STAGE = OFF_STAT + 1024;
-  static constexpr int OFF_PT = OFF_CH + kStages * STAGE;
-  static constexpr int OFF_DST = OFF_PT + TILE;
-  static constexpr int OFF_BAR = OFF_DST + TILE;
+  static constexpr int kN = DC == 1 ? kStages : kStages - 1;
+  static constexpr int OFF_BAR = OFF_CH + kN * STAGE;
   static constexpr int SMEM = OFF_BAR + 256 + 1024;
   static constexpr uint32_t kTmemDP = 64, kTmemDV = 128, kTmemDK = 128 + 64 * DC;
   static constexpr uint32_t kCols = DC == 1 ? 256 : 512;
 };
-constexpr int kBars = 2 + 2 * kStages + 6;
+constexpr int kBars = 2 + 2 * kStages + 5;
 }  // namespace bk
 
 template <typename T, int DC, bool DROP>
@@ -961,7 +918,6 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
                    const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
                    const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk,
                    T* __restrict__ dv, Plane pdk, Plane pdv, Shape sh, Geometry g, int kblk, DropArgs drop) {
-  using namespace bw;
   using namespace bk;
   using Y = bk::L<DC>;
   extern __shared__ uint8_t smem_raw[];
@@ -972,16 +928,15 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
   uint64_t* ch_full = bars + 2;
   uint64_t* ch_empty = ch_full + kStages;
   uint64_t* sd_full = ch_empty + kStages;
-  uint64_t* s_free = sd_full + 1;
-  uint64_t* ps_full = s_free + 1;
-  uint64_t* ps_free = ps_full + 1;
-  uint64_t* acc_full = ps_free + 1;
+  uint64_t* ps_full = sd_full + 1;
+  uint64_t* ps_done = ps_full + 1;
+  uint64_t* acc_full = ps_done + 1;
   uint64_t* acc_empty = acc_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
   __shared__ int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gp_mask = (1 << g.gp_shift) - 1;
-  const int per_unit = (g.rows + BC - 1) / BC, nch = per_unit * g.kv_units;
+  const int per_unit = (g.rows + BC - 1) / BC;
   if (threadIdx.x == 0) {
     umma::mbar_init(kv_full, 1);
     umma::mbar_init(kv_empty, 1);
@@ -990,11 +945,10 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
       umma::mbar_init(&ch_empty[s], 1);
     }
     umma::mbar_init(sd_full, 1);
-    umma::mbar_init(s_free, kRowWarps);
-    umma::mbar_init(ps_full, kRowWarps);
-    umma::mbar_init(ps_free, 1);
+    umma::mbar_init(ps_full, 4);
+    umma::mbar_init(ps_done, 1);
     umma::mbar_init(acc_full, 1);
-    umma::mbar_init(acc_empty, kRowWarps);
+    umma::mbar_init(acc_empty, 4);
     abort_flag = 0;
     umma::fence_barrier_init();
   }
@@ -1013,16 +967,20 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
   };
 
   if (warp == 0) {
-    if (lane == 0) {  // K and V tiles
+    if (lane == 0) {  // K and V tiles of an item, then the query chunks
       umma::tma_prefetch(&tmK);
       umma::tma_prefetch(&tmV);
+      umma::tma_prefetch(&tmQ);
+      umma::tma_prefetch(&tmDO);
       uint32_t t = 0;
-      for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
+      Ring<Y::kN> ch;
+      bool ok = true;
+      for (int item = blockIdx.x; item < g.total && ok && !abort_flag; item += gridDim.x) {
         int blk, kh, b;
         at(item, blk, kh, b);
         if (blk * BM >= sh.keys(b)) continue;
         if (!umma::mbar_wait(kv_empty, (t & 1) ^ 1, 0xb1)) {
-          abort_flag = 1;
+          ok = false;
           break;
         }
         umma::mbar_arrive_expect_tx(kv_full, 2 * DC * TILE);
@@ -1031,89 +989,82 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
           umma::tma_load_4d(smem + dc * TILE, &tmK, kv_full, dc * 64, blk * BM, kh, b);
           umma::tma_load_4d(smem + Y::OFF_V + dc * TILE, &tmV, kv_full, dc * 64, blk * BM, kh, b);
         }
+        for (int u = kh * g.kv_units; u < (kh + 1) * g.kv_units && ok; ++u) {
+          for (int r0 = 0; r0 < g.rows; r0 += BC, ch.next()) {
+            if (!umma::mbar_wait(&ch_empty[ch.s], ch.phase ^ 1, 0xb2)) {
+              ok = false;
+              break;
+            }
+            uint8_t* dst = smem + Y::OFF_CH + ch.s * Y::STAGE;
+            umma::mbar_arrive_expect_tx(&ch_full[ch.s], 2 * DC * CT + 2 * BC * 4);
+#pragma unroll
+            for (int dc = 0; dc < DC; ++dc) {
+              umma::tma_load_5d(dst + dc * CT, &tmQ, &ch_full[ch.s], dc * 64, 0, r0 >> g.gp_shift, u, b);
+              umma::tma_load_5d(dst + (DC + dc) * CT, &tmDO, &ch_full[ch.s], dc * 64, 0, r0 >> g.gp_shift, u, b);
+            }
+            const int64_t stat = (int64_t)(b * g.units + u) * g.ldr + r0;  // both end 64 values behind the last row
+            umma::bulk_load(dst + Y::OFF_STAT, lse + stat, BC * 4, &ch_full[ch.s]);
+            umma::bulk_load(dst + Y::OFF_STAT + BC * 4, delta + stat, BC * 4, &ch_full[ch.s]);
+          }
+        }
         ++t;
       }
-    } else if (lane == 1) {  // query chunks
-      umma::tma_prefetch(&tmQ);
-      umma::tma_prefetch(&tmDO);
-      uint32_t cc = 0;
-      for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
-        int blk, kh, b;
-        at(item, blk, kh, b);
-        if (blk * BM >= sh.keys(b)) continue;
-        for (int c = 0; c < nch; ++c, ++cc) {
-          const int s = cc % kStages, u = kh * g.kv_units + c / per_unit, r0 = (c % per_unit) * BC;
-          if (!umma::mbar_wait(&ch_empty[s], ((cc / kStages) & 1) ^ 1, 0xb2)) {
-            abort_flag = 1;
-            break;
-          }
-          uint8_t* dst = smem + Y::OFF_CH + s * Y::STAGE;
-          umma::mbar_arrive_expect_tx(&ch_full[s], 2 * DC * CT + 2 * BC * 4);
-#pragma unroll
-          for (int dc = 0; dc < DC; ++dc) {
-            umma::tma_load_5d(dst + dc * CT, &tmQ, &ch_full[s], dc * 64, 0, r0 >> g.gp_shift, u, b);
-            umma::tma_load_5d(dst + (DC + dc) * CT, &tmDO, &ch_full[s], dc * 64, 0, r0 >> g.gp_shift, u, b);
-          }
-          const int64_t stat = (int64_t)(b * g.units + u) * g.ldr + r0;  // both buffers end 64 values behind the last row
-          umma::bulk_load(dst + Y::OFF_STAT, lse + stat, BC * 4, &ch_full[s]);
-          umma::bulk_load(dst + Y::OFF_STAT + BC * 4, delta + stat, BC * 4, &ch_full[s]);
-        }
-      }
+      if (!ok) abort_flag = 1;
     }
   } else if (warp == 1) {
     if (lane == 0) {
       uint32_t cc = 0, t = 0;
-      auto issue_s = [&](uint32_t c, int rows, bool last) -> bool {
-        const int s = c % kStages;
-        if (!umma::mbar_wait(&ch_full[s], (c / kStages) & 1, 0xb4)) return false;
-        if (!umma::mbar_wait(s_free, (c & 1) ^ 1, 0xb5)) return false;
-        umma::tc_fence_after();
-        const uint32_t q = umma::smem_u32(smem + Y::OFF_CH + s * Y::STAGE), idesc = Desc<T>::kk((rows + 15) & ~15);
-        mma_scores<DC>(tmem, umma::smem_u32(smem), TILE, q, CT, idesc);
-        mma_scores<DC>(tmem + Y::kTmemDP, umma::smem_u32(smem + Y::OFF_V), TILE, q + DC * CT, CT, idesc);
-        umma::mma_commit(sd_full);
-        if (last) umma::mma_commit(kv_empty);
-        return true;
-      };
-      auto rows_of = [&](int c) { return min(BC, g.rows - (c % per_unit) * BC); };
+      Ring<Y::kN> ch;
+      const int nch = per_unit * g.kv_units;
       bool ok = true;
       for (int item = blockIdx.x; item < g.total && ok && !abort_flag; item += gridDim.x) {
         int blk, kh, b;
         at(item, blk, kh, b);
         if (blk * BM >= sh.keys(b)) continue;
-        if (!umma::mbar_wait(kv_full, t & 1, 0xb3) || !issue_s(cc, rows_of(0), nch == 1)) {
+        if (!umma::mbar_wait(kv_full, t & 1, 0xb3)) {
           ok = false;
           break;
         }
-        for (int c = 0; c < nch; ++c, ++cc) {
-          if (c + 1 < nch && !issue_s(cc + 1, rows_of(c + 1), c + 2 == nch)) {
+        int r0 = 0;  // first row of the chunk in its unit
+        for (int c = 0; c < nch; ++c, ++cc, ch.next()) {
+          const int ksteps = (min(BC, g.rows - r0) + 15) >> 4;
+          if (!umma::mbar_wait(&ch_full[ch.s], ch.phase, 0xb4) ||
+              (cc > 0 && !umma::mbar_wait(ps_done, (cc - 1) & 1, 0xb5))) {
             ok = false;
             break;
           }
+          umma::tc_fence_after();
+          const uint32_t q = umma::smem_u32(smem + Y::OFF_CH + ch.s * Y::STAGE), idesc = Desc<T>::kk(ksteps * 16);
+          mma_scores<DC>(tmem, umma::smem_u32(smem), TILE, q, CT, idesc);
+          mma_scores<DC>(tmem + Y::kTmemDP, umma::smem_u32(smem + Y::OFF_V), TILE, q + DC * CT, CT, idesc);
+          umma::mma_commit(sd_full);
+          if (c == nch - 1) umma::mma_commit(kv_empty);
           if (!umma::mbar_wait(ps_full, cc & 1, 0xb6) ||
               (c == 0 && !umma::mbar_wait(acc_empty, (t & 1) ^ 1, 0xb7))) {
             ok = false;
             break;
           }
           umma::tc_fence_after();
-          const uint32_t q = umma::smem_u32(smem + Y::OFF_CH + (cc % kStages) * Y::STAGE);
-          const int ksteps = (rows_of(c) + 15) >> 4;
-          mma_rows<DC>(tmem + Y::kTmemDV, umma::smem_u32(smem + Y::OFF_PT), q + DC * CT, CT, Desc<T>::MN, ksteps, c > 0);
-          mma_rows<DC>(tmem + Y::kTmemDK, umma::smem_u32(smem + Y::OFF_DST), q, CT, Desc<T>::MN, ksteps, c > 0);
-          umma::mma_commit(ps_free);
-          umma::mma_commit(&ch_empty[cc % kStages]);
+          mma_rows_ts<DC>(tmem + Y::kTmemDV, tmem, q + DC * CT, CT, Desc<T>::MN, ksteps, c > 0);
+          mma_rows_ts<DC>(tmem + Y::kTmemDK, tmem + Y::kTmemDP, q, CT, Desc<T>::MN, ksteps, c > 0);
+          umma::mma_commit(ps_done);
+          umma::mma_commit(&ch_empty[ch.s]);
           if (c == nch - 1) umma::mma_commit(acc_full);
+          r0 += BC;
+          if (r0 >= g.rows) r0 = 0;
         }
         ++t;
       }
       if (!ok) abort_flag = 1;
     }
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane;
-    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     const float sl2 = sh.scale * kLog2e, mult = DROP ? drop.scale : 1.f;
+    const uint64_t sl22 = pk2(sl2, sl2), mult2 = pk2(mult, mult);
     const Philox rng(DROP ? drop : DropArgs{});
     uint32_t cc = 0, t = 0;
+    Ring<Y::kN> ch;
     for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
       int blk, kh, b;
       at(item, blk, kh, b);
@@ -1121,140 +1072,105 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
       const bool exists = j < sh.nk, live = j < len, idle = blk * BM + quarter * 32 >= len;
       auto out_k = [&] { return dk + b * pdk.s_b + j * pdk.s_n + kh * pdk.s_h; };
       auto out_v = [&] { return dv + b * pdv.s_b + j * pdv.s_n + kh * pdv.s_h; };
+      auto zeros = [&] {
+        for (int d = 0; d < sh.dim; d += 8) {
+          *reinterpret_cast<uint4*>(out_k() + d) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(out_v() + d) = make_uint4(0, 0, 0, 0);
+        }
+      };
       if (blk * BM >= len) {
-        if (exists)
-          for (int d = half * 8; d < sh.dim; d += 16) {
-            *reinterpret_cast<uint4*>(out_k() + d) = make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(out_v() + d) = make_uint4(0, 0, 0, 0);
-          }
+        if (exists) zeros();
         continue;
       }
       bool ok = true;
-      for (int c = 0; c < nch; ++c, ++cc) {
-        const int s = cc % kStages, u = kh * g.kv_units + c / per_unit, r0 = (c % per_unit) * BC;
-        const int rows = min(BC, g.rows - r0), c0 = half * 32;
-        const bool work = !idle && c0 < ((rows + 15) & ~15);
-        uint32_t word = 0xffffffffu;  // keep bits of four columns x eight keys, drawn by this lane for its eight
-        if (DROP && work) {
-          word = 0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = r0 + c0 + (lane & 7) * 4 + e;
-            const uint32_t bh = (uint32_t)(b * sh.heads + (u << g.gp_shift) + (r & gp_mask));
-            word |= keep_bits(rng((uint32_t)j >> 3, (uint32_t)(r >> g.gp_shift), bh), drop.limit) << (8 * e);
+      for (int u = kh * g.kv_units; u < (kh + 1) * g.kv_units && ok; ++u) {
+        for (int r0 = 0; r0 < g.rows; r0 += BC, ++cc, ch.next()) {
+          const int rows = min(BC, g.rows - r0);
+          // the statistics are read from the stage: wait for its TMA as well as for the products
+          if (!umma::mbar_wait(&ch_full[ch.s], ch.phase, 0xb8) || !umma::mbar_wait(sd_full, cc & 1, 0xb9)) {
+            ok = false;
+            break;
           }
-        }
-        if (!umma::mbar_wait(&ch_full[s], (cc / kStages) & 1, 0xb8) || !umma::mbar_wait(sd_full, cc & 1, 0xb9)) {
-          ok = false;
-          break;
-        }
-        umma::tc_fence_after();
-        uint32_t pp[16], pd[16];
-        if (work) {
-          const uint64_t sl22 = pk2(sl2, sl2), mult22 = pk2(mult, mult);
-          const float* ls = reinterpret_cast<const float*>(smem + Y::OFF_CH + s * Y::STAGE + Y::OFF_STAT) + c0;
+          umma::tc_fence_after();
+          if (!idle) {
+            const float* stats = reinterpret_cast<const float*>(smem + Y::OFF_CH + ch.s * Y::STAGE + Y::OFF_STAT);
+#pragma unroll 1
+            for (int c0 = 0; c0 < rows; c0 += 32) {
+              uint32_t su[32], du[32];
+              tmem_ld32_nowait(lanes + c0, su);
+              tmem_ld32_nowait(lanes + Y::kTmemDP + c0, du);
+              uint32_t word = 0;  // keep bits of four columns x eight keys, drawn by this lane for its eight
+              if (DROP) {
 #pragma unroll
-          for (int q8 = 0; q8 < 4; ++q8) {  // 8 columns at a time keep the registers under 96
-            uint32_t su[8], du[8];
-            tmem_ld8_nowait(tmem + lane_off + c0 + q8 * 8, su);
-            tmem_ld8_nowait(tmem + lane_off + Y::kTmemDP + c0 + q8 * 8, du);
-            tmem_wait8(su, du);
-#pragma unroll
-            for (int q4 = 0; q4 < 2; ++q4) {
-              uint32_t bits = 0;
-              if (DROP) bits = __shfl_sync(0xffffffffu, word, (lane & 24) + q8 * 2 + q4) >> (lane & 7);
-              const float4 l4 = *reinterpret_cast<const float4*>(ls + q8 * 8 + 4 * q4);
-              const float4 d4 = *reinterpret_cast<const float4*>(ls + BC + q8 * 8 + 4 * q4);
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int i = 4 * q4 + 2 * e;
-                // p = 2^(s - lse2), ds = p (dp - D); the statistics come negated
-                float p0, p1, d0 = __uint_as_float(du[i]), d1 = __uint_as_float(du[i + 1]);
-                unpk2(fma2(pk2(__uint_as_float(su[i]), __uint_as_float(su[i + 1])), sl22,
-                           e ? pk2(l4.z, l4.w) : pk2(l4.x, l4.y)), p0, p1);
-                p0 = ex2(p0);
-                p1 = ex2(p1);
-                const uint64_t nd = e ? pk2(d4.z, d4.w) : pk2(d4.x, d4.y);
-                uint64_t t;
-                float q0 = p0, q1 = p1;
-                if (DROP) {
-                  const bool k0 = bits & (1u << (16 * e)), k1 = bits & (1u << (16 * e + 8));
-                  d0 = k0 ? d0 : 0.f;
-                  d1 = k1 ? d1 : 0.f;
-                  q0 = k0 ? p0 : 0.f;
-                  q1 = k1 ? p1 : 0.f;
-                  t = fma2(pk2(d0, d1), mult22, nd);
-                } else {
-                  t = add2(pk2(d0, d1), nd);
+                for (int e = 0; e < 4; ++e) {
+                  const int r = r0 + c0 + (lane & 7) * 4 + e;
+                  const uint32_t bh = (uint32_t)(b * sh.heads + (u << g.gp_shift) + (r & gp_mask));
+                  word |= keep_bits(rng((uint32_t)j >> 3, (uint32_t)(r >> g.gp_shift), bh), drop.limit) << (8 * e);
                 }
-                unpk2(mul2(pk2(p0, p1), t), d0, d1);
-                pp[q8 * 4 + 2 * q4 + e] = pack2<T>(q0, q1);
-                pd[q8 * 4 + 2 * q4 + e] = pack2<T>(d0, d1);
               }
+              tmem_wait2(su, du);
+              uint32_t pp[16], pd[16];
+#pragma unroll
+              for (int q4 = 0; q4 < 8; ++q4) {
+                uint32_t bits = 0;
+                if (DROP) bits = __shfl_sync(0xffffffffu, word, (lane & 24) + q4) >> (lane & 7);
+                const float4 l4 = *reinterpret_cast<const float4*>(stats + c0 + 4 * q4);
+                const float4 d4 = *reinterpret_cast<const float4*>(stats + BC + c0 + 4 * q4);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int i = 4 * q4 + 2 * e;
+                  // p = 2^(s - lse2), ds = p (dp - D); the statistics come negated
+                  float p0, p1, d0 = __uint_as_float(du[i]), d1 = __uint_as_float(du[i + 1]);
+                  unpk2(fma2(pk2(__uint_as_float(su[i]), __uint_as_float(su[i + 1])), sl22,
+                             e ? pk2(l4.z, l4.w) : pk2(l4.x, l4.y)), p0, p1);
+                  p0 = ex2(p0);
+                  p1 = ex2(p1);
+                  const uint64_t nd = e ? pk2(d4.z, d4.w) : pk2(d4.x, d4.y);
+                  uint64_t x;
+                  float q0 = p0, q1 = p1;
+                  if (DROP) {
+                    const bool k0 = bits & (1u << (16 * e)), k1 = bits & (1u << (16 * e + 8));
+                    d0 = k0 ? d0 : 0.f;
+                    d1 = k1 ? d1 : 0.f;
+                    q0 = k0 ? p0 : 0.f;
+                    q1 = k1 ? p1 : 0.f;
+                    x = fma2(pk2(d0, d1), mult2, nd);
+                  } else {
+                    x = add2(pk2(d0, d1), nd);
+                  }
+                  unpk2(mul2(pk2(p0, p1), x), d0, d1);
+                  pp[2 * q4 + e] = pack2<T>(q0, q1);
+                  pd[2 * q4 + e] = pack2<T>(d0, d1);
+                }
+              }
+              if (c0 + 32 > rows) {  // queries behind the last: their statistics are someone else's, so zeros outright
+                zero_tail(pp, rows - c0);
+                zero_tail(pd, rows - c0);
+              }
+              umma::tmem_st16(lanes + c0 / 2, pp);  // over accumulators this warp has read
+              umma::tmem_st16(lanes + Y::kTmemDP + c0 / 2, pd);
             }
+            umma::tmem_wait_st();
           }
-          if (c0 + 32 > rows) {  // queries behind the last: their statistics are someone else's, so zeros outright
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (c0 + i >= rows) {
-                pp[i / 2] &= i & 1 ? 0x0000ffffu : 0u;
-                pd[i / 2] &= i & 1 ? 0x0000ffffu : 0u;
-              }
-          }
+          warp_arrive(ps_full, false);
         }
-        warp_arrive(s_free, false);
-        if (!umma::mbar_wait(ps_free, (cc & 1) ^ 1, 0xba)) {
-          ok = false;
-          break;
-        }
-        if (work) {
-#pragma unroll
-          for (int gr = 0; gr < 4; ++gr) {
-            const uint32_t at16 = sw128(row, half * 4 + gr);
-            *reinterpret_cast<uint4*>(smem + Y::OFF_PT + at16) =
-                make_uint4(pp[gr * 4], pp[gr * 4 + 1], pp[gr * 4 + 2], pp[gr * 4 + 3]);
-            *reinterpret_cast<uint4*>(smem + Y::OFF_DST + at16) =
-                make_uint4(pd[gr * 4], pd[gr * 4 + 1], pd[gr * 4 + 2], pd[gr * 4 + 3]);
-          }
-        }
-        warp_arrive(ps_full, true);
       }
       if (!ok || !umma::mbar_wait(acc_full, t & 1, 0xbb)) {
         abort_flag = 1;
         break;
       }
       umma::tc_fence_after();
-#pragma unroll
-      for (int dc = 0; dc < DC; ++dc) {
-        const int d0 = dc * 64 + half * 32;
-        if (d0 < sh.dim) {
-#pragma unroll
-          for (int which = 0; which < 2; ++which) {
-            uint32_t a[32];
-            if (!idle) {
-              tmem_ld32_nowait(tmem + lane_off + (which ? Y::kTmemDK : Y::kTmemDV) + d0, a);
-              wait_ld();
-              tie32(a);
-            }
-            const float* f = reinterpret_cast<const float*>(a);
-            const float by = which ? sh.scale : mult;
-            T* out = which ? out_k() : out_v();
-            if (exists) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                if (d0 + 8 * i >= sh.dim) continue;
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (live)
-                  w = make_uint4(pack2<T>(f[8 * i] * by, f[8 * i + 1] * by),
-                                 pack2<T>(f[8 * i + 2] * by, f[8 * i + 3] * by),
-                                 pack2<T>(f[8 * i + 4] * by, f[8 * i + 5] * by),
-                                 pack2<T>(f[8 * i + 6] * by, f[8 * i + 7] * by));
-                *reinterpret_cast<uint4*>(out + d0 + 8 * i) = w;
-              }
-            }
-          }
-        }
+#pragma unroll 1
+      for (int k = 0; k < 4 * DC; ++k) {
+        const int d0 = (k >> 1) * 32;
+        if (idle || d0 >= sh.dim) break;
+        uint32_t a[32];
+        tmem_ld32_nowait(lanes + ((k & 1) ? Y::kTmemDK : Y::kTmemDV) + d0, a);
+        wait_ld();
+        tie32(a);
+        if (live) store_row<T>((k & 1) ? out_k() : out_v(), d0, sh.dim, a, (k & 1) ? sh.scale : mult);
       }
+      if (exists && !live) zeros();
       warp_arrive(acc_empty, false);
       ++t;
     }
@@ -1382,13 +1298,13 @@ int forward_launch(const Shape& sh, const Forward& a, Geometry g, const char* na
 
 template <typename T, int DC, bool DROP>
 int backward_launch(const Shape& sh, const Backward& a, Geometry g, const char* name) {
-  CUtensorMap q128, do128, q64, do64, k64, v64, k128, v128;
+  CUtensorMap q128, do128, q64, do64, k96, v96, k128, v128;
   if (int st = query_map(q128, a.q, a.pq, sh, g, a.dtype, BM, name)) return st;
   if (int st = query_map(do128, a.go, a.pgo, sh, g, a.dtype, BM, name)) return st;
-  if (int st = query_map(q64, a.q, a.pq, sh, g, a.dtype, bw::BC, name)) return st;
-  if (int st = query_map(do64, a.go, a.pgo, sh, g, a.dtype, bw::BC, name)) return st;
-  if (int st = key_map(k64, a.k, a.pk, sh, a.dtype, bw::BC, name)) return st;
-  if (int st = key_map(v64, a.v, a.pv, sh, a.dtype, bw::BC, name)) return st;
+  if (int st = query_map(q64, a.q, a.pq, sh, g, a.dtype, bk::BC, name)) return st;
+  if (int st = query_map(do64, a.go, a.pgo, sh, g, a.dtype, bk::BC, name)) return st;
+  if (int st = key_map(k96, a.k, a.pk, sh, a.dtype, bq::BC, name)) return st;
+  if (int st = key_map(v96, a.v, a.pv, sh, a.dtype, bq::BC, name)) return st;
   if (int st = key_map(k128, a.k, a.pk, sh, a.dtype, BM, name)) return st;
   if (int st = key_map(v128, a.v, a.pv, sh, a.dtype, BM, name)) return st;
   float* delta = static_cast<float*>(a.workspace);
@@ -1398,7 +1314,7 @@ int backward_launch(const Shape& sh, const Backward& a, Geometry g, const char* 
     constexpr int smem = bq::L<DC>::SMEM;
     PMB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), name);
     kernel<<<persistent_grid(g.total, per_sm), bw::kThreads, smem, a.stream>>>(
-        q128, do128, k64, v64, static_cast<const T*>(a.o), a.lse, delta, static_cast<T*>(a.gq), a.po, a.pgq, sh, g,
+        q128, do128, k96, v96, static_cast<const T*>(a.o), a.lse, delta, static_cast<T*>(a.gq), a.po, a.pgq, sh, g,
         a.drop);
     PMB_CHECK_LAUNCH(name);
   }
