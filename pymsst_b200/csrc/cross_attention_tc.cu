@@ -64,28 +64,35 @@ struct Desc {
   static constexpr uint32_t MN = umma::idesc_f16(kBf16, false, true, BM, 64);  // B MN-major, 64 head elements
 };
 
+// Descriptor of a 128-byte-swizzled tile in shared memory; tiles and K steps
+// further on are 16-byte units added to it.
+__device__ __forceinline__ uint64_t tile_desc(const void* smem) {
+  return umma::smem_desc_sw128(umma::smem_u32(smem), 16, 1024);
+}
+
 // D (+)= A B^T, A and B K-major: DC sub-tiles of 64 elements, strides a_sub / b_sub bytes apart.
 template <int DC>
-__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t a_sub, uint32_t b, uint32_t b_sub,
+__device__ __forceinline__ void mma_scores(uint32_t d, uint64_t a, uint32_t a_sub, uint64_t b, uint32_t b_sub,
                                            uint32_t idesc) {
 #pragma unroll
   for (int dc = 0; dc < DC; ++dc)
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk)
-      umma::mma_f16(d, umma::smem_desc_sw128(a + dc * a_sub + kk * 32, 16, 1024),
-                    umma::smem_desc_sw128(b + dc * b_sub + kk * 32, 16, 1024), idesc, (dc || kk) ? 1u : 0u);
+      umma::mma_f16(d, a + (dc * a_sub + kk * 32) / 16, b + (dc * b_sub + kk * 32) / 16, idesc, (dc || kk) ? 1u : 0u);
 }
 
 // D (+)= A B with A in tensor memory, 16-bit pairs in 32-bit columns, and B MN-major: its rows are the K index, its
 // 64 head elements the N index, DC sub-tiles b_sub bytes apart into accumulators 64 columns apart.
 template <int DC>
-__device__ __forceinline__ void mma_rows_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t b_sub, uint32_t idesc,
+__device__ __forceinline__ void mma_rows_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t b_sub, uint32_t idesc,
                                             int ksteps, bool accumulate) {
-  for (int ks = 0; ks < ksteps; ++ks)
+#pragma unroll
+  for (int ks = 0; ks < 6; ++ks) {  // chunks hold 96 rows at most
+    if (ks >= ksteps) break;
 #pragma unroll
     for (int dc = 0; dc < DC; ++dc)
-      umma::mma_f16_ts(d + dc * 64, a + ks * 8, umma::smem_desc_sw128(b + dc * b_sub + ks * 2048, 16, 1024), idesc,
-                       (accumulate || ks) ? 1u : 0u);
+      umma::mma_f16_ts(d + dc * 64, a + ks * 8, b + (dc * b_sub + ks * 2048) / 16, idesc, (accumulate || ks) ? 1u : 0u);
+  }
 }
 
 // Elements [n, 32) of 16 packed pairs to zero.
@@ -262,7 +269,7 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
   uint64_t* o_empty = o_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
   __shared__ int abort_flag;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // uniform in a warp
   const int gp_mask = (1 << g.gp_shift) - 1;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -286,7 +293,7 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
   umma::tc_fence_before();
   __syncthreads();
   umma::tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp == 0) {
     if (lane == 0) {
@@ -326,7 +333,8 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
       if (!ok) abort_flag = 1;
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    {  // the whole warp, so that addresses and descriptors stay uniform; one lane issues
+      const bool leader = umma::elect_one();
       // O += P V of the chunk whose scores were issued last
       struct Pending {
         bool live, first;
@@ -340,10 +348,13 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
         if (!umma::mbar_wait(&p_full[c & 1], (c >> 1) & 1, 0x94) || !umma::mbar_wait(&v_full[vr.s], vr.phase, 0x95)) return false;
         if (prev.first && !umma::mbar_wait(o_empty, (prev.t & 1) ^ 1, 0x96)) return false;
         umma::tc_fence_after();
-        mma_rows_ts<DC>(tmem + Y::kTmemO, tmem + (c & 1) * kMaxW, umma::smem_u32(smem + Y::OFF_V + vr.s * DC * SUB), SUB,
-                        Desc<T>::MN, (prev.keys + 15) >> 4, !prev.first);
-        umma::mma_commit(&o_done[c & 1]);
-        umma::mma_commit(&v_empty[vr.s]);
+        if (leader) {
+          mma_rows_ts<DC>(tmem + Y::kTmemO, tmem + (c & 1) * kMaxW, tile_desc(smem + Y::OFF_V + vr.s * DC * SUB), SUB,
+                          Desc<T>::MN, (prev.keys + 15) >> 4, !prev.first);
+          umma::mma_commit(&o_done[c & 1]);
+          umma::mma_commit(&v_empty[vr.s]);
+        }
+        __syncwarp();
         vr.next();
         return true;
       };
@@ -366,12 +377,15 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
             break;
           }
           umma::tc_fence_after();
-          mma_scores<DC>(tmem + (cc & 1) * kMaxW, umma::smem_u32(smem + q.s * DC * TILE), TILE,
-                         umma::smem_u32(smem + Y::OFF_K + kr.s * DC * SUB), SUB, Desc<T>::kk((keys + 15) & ~15));
-          umma::mma_commit(&s_full[cc & 1]);
-          umma::mma_commit(&k_empty[kr.s]);
+          if (leader) {
+            mma_scores<DC>(tmem + (cc & 1) * kMaxW, tile_desc(smem + q.s * DC * TILE), TILE,
+                           tile_desc(smem + Y::OFF_K + kr.s * DC * SUB), SUB, Desc<T>::kk((keys + 15) & ~15));
+            umma::mma_commit(&s_full[cc & 1]);
+            umma::mma_commit(&k_empty[kr.s]);
+            if (c == c1 - 1) umma::mma_commit(&q_empty[q.s]);
+          }
+          __syncwarp();
           kr.next();
-          if (c == c1 - 1) umma::mma_commit(&q_empty[q.s]);
           if (prev.live && !issue_o(cc - 1)) {
             ok = false;
             break;
@@ -605,517 +619,645 @@ __global__ void __launch_bounds__(256)
   if (d == 0) lse[bu * g.ldr + R] = any ? -(mx + log2f(w)) : -INFINITY;
 }
 
-// ------------------------------------------------------------ backward: dQ
-// Item = 128 packed rows of a unit; keys in chunks of 96.  S = Q K^T, dP =
-// dO V^T; the row threads (one per row) write dS, as 16-bit pairs, over the
-// scores they have read, and dQ += dS K takes it from there.  S of the next
-// chunk waits for that product (it overwrites dS); two CTAs per SM fill the
-// gap.  D = rowsum(dO * O) is formed once per item and kept for the dK / dV
-// kernel.
+// ---------------------------------------------------------------- backward
+// One CTA per SM, its row warps two groups of four (one tensor memory lane
+// per thread), NB pairs of 64-column accumulators (S and dP, or their
+// transposes).  Chunk n of the CTA's stream uses pair n % NB and goes to group
+// n % 2.  The MMA lane forms chunk n's scores, then the products of chunk
+// n - (NB - 1), whose 16-bit operands its group has written over the scores
+// and dP it read.  With three pairs the scores a group takes next are ready
+// when it finishes a chunk, and the pair they went to was freed a step
+// earlier: neither side waits for a round trip.  (Time axis, 258 positions,
+// dropout, dK / dV + dQ: one pair per CTA and two CTAs per SM 321 + 219 us,
+// three groups with a pair each 355 + 290.)
+//
+// Barriers that groups wait on out of step have turns: item t uses barrier
+// t % NB.  A chunk's scores are complete only after the products of the chunk
+// NB before it, so when a group that has seen the scores of item t's last
+// chunk waits, the turn before (item t - NB, at least NB chunks back) is over.
+// What a group writes before it has seen the scores (dQ's row sums, written at
+// an item's first chunk) has 2 NB turns: certain then are the scores of its
+// previous chunk, two before, so that item t - 2 NB is over.
 namespace bw {
-constexpr int kThreads = 192;
+constexpr int BC = 64;                 // chunk rows
+constexpr int CT = BC * 128;           // bytes of a chunk's 64-element sub-tile
+constexpr int G = 2;                   // groups of row warps
+constexpr int kThreads = 64 + 128 * G;
 }  // namespace bw
 
+// ------------------------------------------------------------ backward: dQ
+// Item = 128 packed rows of a unit, chunks of 64 keys: S = Q K^T, dP = dO V^T,
+// dQ += dS K.  The group with an item's first chunk forms D = rowsum(dO * O),
+// leaves it for the other groups and keeps it for the dK / dV kernel; the
+// group with the last chunk writes dQ.
 namespace bq {
-constexpr int kStages = 3;
-constexpr int BC = 96;                 // keys per chunk
-constexpr int CT = BC * 128;           // bytes of a chunk's 64-element sub-tile
 template <int DC>
 struct L {
-  static constexpr int OFF_DO = DC * TILE;
-  static constexpr int OFF_KV = 2 * DC * TILE;             // stages of DC K sub-tiles, DC V sub-tiles
-  static constexpr int STAGE = 2 * DC * CT;
-  static constexpr int OFF_BAR = OFF_KV + (DC == 1 ? kStages : kStages - 1) * STAGE;
-  static constexpr int kN = DC == 1 ? kStages : kStages - 1;
-  static constexpr int SMEM = OFF_BAR + 256 + 1024;
-  static constexpr uint32_t kTmemDP = BC, kTmemDQ = 2 * BC, kCols = DC == 1 ? 256 : 512;
+  static constexpr int NB = 3;
+  static constexpr int kTiles = DC == 1 ? 2 : 1;            // Q, dO tiles
+  static constexpr int kN = DC == 1 ? 8 : 4;                // stages of DC K sub-tiles, DC V sub-tiles
+  static constexpr int TILES = 2 * DC * TILE;
+  static constexpr int STAGE = 2 * DC * bw::CT;
+  static constexpr int OFF_KV = kTiles * TILES;
+  static constexpr int OFF_D = OFF_KV + kN * STAGE;         // [2 NB][128] -D, then [2 NB][128] -lse2
+  static constexpr int OFF_BAR = OFF_D + 4 * NB * 512;
+  static constexpr int SMEM = OFF_BAR + 512 + 1024;
+  static constexpr uint32_t kTmemDQ = 128 * NB;
 };
-constexpr int kBars = 2 + 2 * kStages + 5;
 }  // namespace bq
 
+// One chunk of the stream of a CTA: items with keys, in order, chunk by chunk.
+struct QueryCursor {
+  int item, len, c, nch;
+  Item it;
+  uint32_t t, n;  // items and chunks before this one
+  bool live;
+
+  __device__ __forceinline__ void seek(const Shape& sh, const Geometry& g) {  // from `item` on
+    live = false;
+    for (; item < g.total; item += gridDim.x) {
+      it = forward_item(item, g);
+      len = sh.keys(it.b);
+      nch = (len + bw::BC - 1) / bw::BC;
+      c = 0;
+      if (nch > 0) {
+        live = true;
+        return;
+      }
+    }
+  }
+  __device__ __forceinline__ QueryCursor(const Shape& sh, const Geometry& g) : item(blockIdx.x), t(0), n(0) {
+    seek(sh, g);
+  }
+  __device__ __forceinline__ void next(const Shape& sh, const Geometry& g) {
+    ++n;
+    if (++c < nch) return;
+    ++t;
+    item += gridDim.x;
+    seek(sh, g);
+  }
+  __device__ __forceinline__ int keys() const { return min(bw::BC, len - c * bw::BC); }
+};
+
 template <typename T, int DC, bool DROP>
-__global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
+__global__ void __launch_bounds__(bw::kThreads, 1)
     xattn_bwd_dq(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
                  const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                  const T* __restrict__ o, const float* __restrict__ lse, float* __restrict__ delta, T* __restrict__ dq,
                  Plane po, Plane pdq, Shape sh, Geometry g, DropArgs drop) {
-  using namespace bq;
+  using namespace bw;
   using Y = bq::L<DC>;
+  constexpr int NB = Y::NB;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Y::OFF_BAR);
-  uint64_t* qd_full = bars;
-  uint64_t* qd_empty = bars + 1;
-  uint64_t* kv_full = bars + 2;
-  uint64_t* kv_empty = kv_full + kStages;
-  uint64_t* sd_full = kv_empty + kStages;
-  uint64_t* ds_full = sd_full + 1;
-  uint64_t* ds_done = ds_full + 1;
-  uint64_t* dq_full = ds_done + 1;
-  uint64_t* dq_empty = dq_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
+  uint64_t* qd_full = bars;                  // [kTiles]
+  uint64_t* qd_empty = qd_full + Y::kTiles;  // [kTiles]
+  uint64_t* kv_full = qd_empty + Y::kTiles;  // [kN]
+  uint64_t* kv_empty = kv_full + Y::kN;      // [kN]
+  uint64_t* sd_full = kv_empty + Y::kN;      // [NB]
+  uint64_t* ds_full = sd_full + NB;           // [NB]
+  uint64_t* ds_done = ds_full + NB;           // [NB]
+  uint64_t* d_full = ds_done + NB;            // [2 NB]
+  uint64_t* dq_full = d_full + 2 * NB;        // [NB]
+  uint64_t* dq_empty = dq_full + NB;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dq_empty + 1);
+  float* nd_s = reinterpret_cast<float*>(smem + Y::OFF_D);
+  float* nl_s = nd_s + 2 * NB * 128;
   __shared__ int abort_flag;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // uniform in a warp
   const int gp_mask = (1 << g.gp_shift) - 1;
   if (threadIdx.x == 0) {
-    umma::mbar_init(qd_full, 1);
-    umma::mbar_init(qd_empty, 1 + 4);  // the products' commit and the row warps' reads of dO
-    for (int s = 0; s < kStages; ++s) {
-      umma::mbar_init(&kv_full[s], 1);
-      umma::mbar_init(&kv_empty[s], 1);
+    for (int i = 0; i < Y::kTiles; ++i) {
+      umma::mbar_init(&qd_full[i], 1);
+      umma::mbar_init(&qd_empty[i], 1 + 4);  // the products' commit and the four warps that read dO
     }
-    umma::mbar_init(sd_full, 1);
-    umma::mbar_init(ds_full, 4);
-    umma::mbar_init(ds_done, 1);
-    umma::mbar_init(dq_full, 1);
+    for (int i = 0; i < Y::kN; ++i) {
+      umma::mbar_init(&kv_full[i], 1);
+      umma::mbar_init(&kv_empty[i], 1);
+    }
+    for (int i = 0; i < NB; ++i) {
+      umma::mbar_init(&sd_full[i], 1);
+      umma::mbar_init(&ds_full[i], 4);
+      umma::mbar_init(&ds_done[i], 1);
+      umma::mbar_init(&d_full[i], 4);
+      umma::mbar_init(&d_full[NB + i], 4);
+      umma::mbar_init(&dq_full[i], 1);
+    }
     umma::mbar_init(dq_empty, 4);
     abort_flag = 0;
     umma::fence_barrier_init();
   }
-  if (warp == 0) umma::tmem_alloc(tmem_slot, Y::kCols);
+  if (warp == 0) umma::tmem_alloc(tmem_slot, 512);
   umma::tc_fence_before();
   __syncthreads();
   umma::tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp == 0) {
-    if (lane == 0) {  // tiles of an item, then its chunks
+    if (lane == 0) {  // tiles of an item before its first chunk
       umma::tma_prefetch(&tmQ);
       umma::tma_prefetch(&tmDO);
       umma::tma_prefetch(&tmK);
       umma::tma_prefetch(&tmV);
-      uint32_t t = 0;
+      Ring<Y::kTiles> qd;
       Ring<Y::kN> kv;
-      bool ok = true;
-      for (int item = blockIdx.x; item < g.total && ok && !abort_flag; item += gridDim.x) {
-        const Item it = forward_item(item, g);
-        const int nch = (sh.keys(it.b) + BC - 1) / BC;
-        if (nch == 0) continue;
-        if (!umma::mbar_wait(qd_empty, (t & 1) ^ 1, 0xa1)) {
-          ok = false;
-          break;
-        }
-        umma::mbar_arrive_expect_tx(qd_full, 2 * DC * TILE);
-#pragma unroll
-        for (int dc = 0; dc < DC; ++dc) {
-          const int pos = (it.blk * BM) >> g.gp_shift;
-          umma::tma_load_5d(smem + dc * TILE, &tmQ, qd_full, dc * 64, 0, pos, it.u, it.b);
-          umma::tma_load_5d(smem + Y::OFF_DO + dc * TILE, &tmDO, qd_full, dc * 64, 0, pos, it.u, it.b);
-        }
-        for (int c = 0; c < nch; ++c, kv.next()) {
-          if (!umma::mbar_wait(&kv_empty[kv.s], kv.phase ^ 1, 0xa2)) {
-            ok = false;
+      for (QueryCursor cu(sh, g); cu.live && !abort_flag; cu.next(sh, g), kv.next()) {
+        if (cu.c == 0) {
+          if (!umma::mbar_wait(&qd_empty[qd.s], qd.phase ^ 1, 0xa1)) {
+            abort_flag = 1;
             break;
           }
-          uint8_t* dst = smem + Y::OFF_KV + kv.s * Y::STAGE;
-          umma::mbar_arrive_expect_tx(&kv_full[kv.s], Y::STAGE);
+          uint8_t* dst = smem + qd.s * Y::TILES;
+          umma::mbar_arrive_expect_tx(&qd_full[qd.s], Y::TILES);
+          const int pos = (cu.it.blk * BM) >> g.gp_shift;
 #pragma unroll
           for (int dc = 0; dc < DC; ++dc) {
-            umma::tma_load_4d(dst + dc * CT, &tmK, &kv_full[kv.s], dc * 64, c * BC, it.u / g.kv_units, it.b);
-            umma::tma_load_4d(dst + (DC + dc) * CT, &tmV, &kv_full[kv.s], dc * 64, c * BC, it.u / g.kv_units, it.b);
+            umma::tma_load_5d(dst + dc * TILE, &tmQ, &qd_full[qd.s], dc * 64, 0, pos, cu.it.u, cu.it.b);
+            umma::tma_load_5d(dst + (DC + dc) * TILE, &tmDO, &qd_full[qd.s], dc * 64, 0, pos, cu.it.u, cu.it.b);
           }
+          qd.next();
         }
-        ++t;
-      }
-      if (!ok) abort_flag = 1;
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      uint32_t cc = 0, t = 0;
-      Ring<Y::kN> kv;
-      bool ok = true;
-      for (int item = blockIdx.x; item < g.total && ok && !abort_flag; item += gridDim.x) {
-        const Item it = forward_item(item, g);
-        const int len = sh.keys(it.b), nch = (len + BC - 1) / BC;
-        if (nch == 0) continue;
-        if (!umma::mbar_wait(qd_full, t & 1, 0xa3)) {
-          ok = false;
+        if (!umma::mbar_wait(&kv_empty[kv.s], kv.phase ^ 1, 0xa2)) {
+          abort_flag = 1;
           break;
         }
-        for (int c = 0; c < nch; ++c, ++cc, kv.next()) {
-          const int keys = min(BC, len - c * BC), ksteps = (keys + 15) >> 4;
-          if (!umma::mbar_wait(&kv_full[kv.s], kv.phase, 0xa4) ||
-              (cc > 0 && !umma::mbar_wait(ds_done, (cc - 1) & 1, 0xa5))) {
-            ok = false;
-            break;
-          }
-          umma::tc_fence_after();
-          const uint32_t k = umma::smem_u32(smem + Y::OFF_KV + kv.s * Y::STAGE), idesc = Desc<T>::kk(ksteps * 16);
-          mma_scores<DC>(tmem, umma::smem_u32(smem), TILE, k, CT, idesc);
-          mma_scores<DC>(tmem + Y::kTmemDP, umma::smem_u32(smem + Y::OFF_DO), TILE, k + DC * CT, CT, idesc);
-          umma::mma_commit(sd_full);
-          if (c == nch - 1) umma::mma_commit(qd_empty);
-          if (!umma::mbar_wait(ds_full, cc & 1, 0xa6) ||
-              (c == 0 && !umma::mbar_wait(dq_empty, (t & 1) ^ 1, 0xa7))) {
-            ok = false;
-            break;
-          }
-          umma::tc_fence_after();
-          mma_rows_ts<DC>(tmem + Y::kTmemDQ, tmem, k, CT, Desc<T>::MN, ksteps, c > 0);
-          umma::mma_commit(ds_done);
-          umma::mma_commit(&kv_empty[kv.s]);
-          if (c == nch - 1) umma::mma_commit(dq_full);
+        uint8_t* dst = smem + Y::OFF_KV + kv.s * Y::STAGE;
+        umma::mbar_arrive_expect_tx(&kv_full[kv.s], Y::STAGE);
+#pragma unroll
+        for (int dc = 0; dc < DC; ++dc) {
+          umma::tma_load_4d(dst + dc * CT, &tmK, &kv_full[kv.s], dc * 64, cu.c * BC, cu.it.u / g.kv_units, cu.it.b);
+          umma::tma_load_4d(dst + (DC + dc) * CT, &tmV, &kv_full[kv.s], dc * 64, cu.c * BC, cu.it.u / g.kv_units,
+                            cu.it.b);
         }
-        ++t;
       }
-      if (!ok) abort_flag = 1;
     }
-  } else {
-    const int quarter = warp & 3, row = quarter * 32 + lane;
-    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-    const float sl2 = sh.scale * kLog2e, mult = DROP ? drop.scale : 1.f;
-    const Philox rng(DROP ? drop : DropArgs{});
-    uint32_t cc = 0, t = 0;
-    Ring<Y::kN> kv;
-    for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
-      const Item it = forward_item(item, g);
-      const int len = sh.keys(it.b), nch = (len + BC - 1) / BC;
-      const int R = it.blk * BM + row, pos = R >> g.gp_shift, head = (it.u << g.gp_shift) + (R & gp_mask);
-      const bool valid = R < g.rows, idle = it.blk * BM + quarter * 32 >= g.rows;
-      const int64_t stat = (int64_t)(it.b * g.units + it.u) * g.ldr + R;
-      auto dst = [&] { return dq + it.b * pdq.s_b + pos * pdq.s_n + head * pdq.s_h; };
-      if (nch == 0) {
-        if (valid) {
-          for (int d = 0; d < sh.dim; d += 8) *reinterpret_cast<uint4*>(dst() + d) = make_uint4(0, 0, 0, 0);
-          delta[stat] = 0.f;
+  } else if (warp == 1) {
+    {  // the whole warp, so that addresses and descriptors stay uniform; one lane issues
+      const bool leader = umma::elect_one();
+      QueryCursor cu(sh, g), done = cu;  // scores, and products NB - 1 chunks behind
+      Ring<Y::kTiles> qd;
+      Ring<Y::kN> kv, kvd;
+      Ring<NB> gr, grd;
+      auto products = [&]() -> bool {
+        if (!umma::mbar_wait(&ds_full[grd.s], grd.phase, 0xa6) ||
+            (done.c == 0 && !umma::mbar_wait(dq_empty, (done.t & 1) ^ 1, 0xa7)))
+          return false;
+        umma::tc_fence_after();
+        if (leader) {
+          mma_rows_ts<DC>(tmem + Y::kTmemDQ, tmem + grd.s * 128, tile_desc(smem + Y::OFF_KV + kvd.s * Y::STAGE), CT,
+                          Desc<T>::MN, (done.keys() + 15) >> 4, done.c > 0);
+          umma::mma_commit(&ds_done[grd.s]);
+          umma::mma_commit(&kv_empty[kvd.s]);
+          if (done.c == done.nch - 1) umma::mma_commit(&dq_full[done.t % NB]);
         }
-        continue;
-      }
-      // this row of O and its statistics, fetched while the tiles are in flight
-      uint4 orow[8 * DC];
-      float nlse = 0.f;
-      const T* osrc = o + it.b * po.s_b + pos * po.s_n + head * po.s_h;
-#pragma unroll
-      for (int i = 0; i < 8 * DC; ++i)
-        orow[i] = valid && i * 8 < sh.dim ? *reinterpret_cast<const uint4*>(osrc + i * 8) : make_uint4(0, 0, 0, 0);
-      if (valid) nlse = lse[stat];
-      if (!umma::mbar_wait(qd_full, t & 1, 0xa8)) {
-        abort_flag = 1;
-        break;
-      }
-      float ndsum = 0.f;  // -D
-#pragma unroll
-      for (int i = 0; i < 8 * DC; ++i) {
-        const uint4 d4 = *reinterpret_cast<const uint4*>(smem + Y::OFF_DO + (i >> 3) * TILE + sw128(row, i & 7));
-        const T* oe = reinterpret_cast<const T*>(&orow[i]);
-        const T* de = reinterpret_cast<const T*>(&d4);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ndsum = fmaf(-Elem<T>::to_f(oe[e]), Elem<T>::to_f(de[e]), ndsum);
-      }
-      if (valid) delta[stat] = ndsum;
-      warp_arrive(qd_empty, false);
-      const uint32_t bh = (uint32_t)(it.b * sh.heads + head);
-      const uint64_t sl22 = pk2(sl2, sl2), nlse2 = pk2(nlse, nlse), nd2 = pk2(ndsum, ndsum), mult2 = pk2(mult, mult);
+        __syncwarp();
+        done.next(sh, g);
+        grd.next();
+        kvd.next();
+        return true;
+      };
       bool ok = true;
-      for (int c = 0; c < nch; ++c, ++cc, kv.next()) {
-        const int kc = c * BC, keys = min(BC, len - kc);
-        if (!umma::mbar_wait(sd_full, cc & 1, 0xaa)) {
+      for (; cu.live && !abort_flag; cu.next(sh, g), kv.next(), gr.next()) {
+        if ((cu.c == 0 && !umma::mbar_wait(&qd_full[qd.s], qd.phase, 0xa3)) ||
+            !umma::mbar_wait(&kv_full[kv.s], kv.phase, 0xa4) || !umma::mbar_wait(&ds_done[gr.s], gr.phase ^ 1, 0xa5)) {
           ok = false;
           break;
         }
         umma::tc_fence_after();
+        const uint64_t k = tile_desc(smem + Y::OFF_KV + kv.s * Y::STAGE), q = tile_desc(smem + qd.s * Y::TILES);
+        const uint32_t idesc = Desc<T>::kk((cu.keys() + 15) & ~15), acc = tmem + gr.s * 128;
+        if (leader) {
+          mma_scores<DC>(acc, q, TILE, k, CT, idesc);
+          mma_scores<DC>(acc + 64, q + DC * TILE / 16, TILE, k + DC * CT / 16, CT, idesc);
+          umma::mma_commit(&sd_full[gr.s]);
+          if (cu.c == cu.nch - 1) umma::mma_commit(&qd_empty[qd.s]);
+        }
+        __syncwarp();
+        if (cu.c == cu.nch - 1) qd.next();
+        if (cu.n >= NB - 1 && !products()) {
+          ok = false;
+          break;
+        }
+      }
+      while (ok && done.live && done.n < cu.n) ok = products();
+      if (!ok) abort_flag = 1;
+    }
+  } else {
+    const int grp = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const float sl2 = sh.scale * kLog2e, mult = DROP ? drop.scale : 1.f;
+    const uint64_t sl22 = pk2(sl2, sl2), mult2 = pk2(mult, mult);
+    const Philox rng(DROP ? drop : DropArgs{});
+    // rows of items without keys: zeros
+    if (grp == 0 && sh.lengths != nullptr)
+      for (int item = blockIdx.x; item < g.total; item += gridDim.x) {
+        const Item it = forward_item(item, g);
+        const int R = it.blk * BM + row;
+        if (sh.keys(it.b) > 0 || R >= g.rows) continue;
+        T* dst = dq + it.b * pdq.s_b + (R >> g.gp_shift) * pdq.s_n + ((it.u << g.gp_shift) + (R & gp_mask)) * pdq.s_h;
+        for (int d = 0; d < sh.dim; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
+        delta[(int64_t)(it.b * g.units + it.u) * g.ldr + R] = 0.f;
+      }
+    Ring<Y::kTiles> qd;
+    Ring<Y::kN> kv;
+    Ring<NB> gr;     // accumulators of the cursor's chunk
+    Ring<NB> turn;   // of the items
+    Ring<2 * NB> dturn;
+    for (QueryCursor cu(sh, g); cu.live && !abort_flag; cu.next(sh, g), kv.next(), gr.next()) {
+      const bool last = cu.c == cu.nch - 1;
+      if ((int)(cu.n % G) == grp) {
+        const uint32_t acc = tmem + lane_off + gr.s * 128;
+        const Item& it = cu.it;
+        const int R = it.blk * BM + row, pos = R >> g.gp_shift, head = (it.u << g.gp_shift) + (R & gp_mask);
+        const bool valid = R < g.rows, idle = it.blk * BM + quarter * 32 >= g.rows;
+        if (cu.c == 0) {  // D and the statistics of this item, for all groups
+          float nlse = 0.f, nd = 0.f;
+          uint4 orow[8 * DC];
+          const T* osrc = o + it.b * po.s_b + pos * po.s_n + head * po.s_h;
+#pragma unroll
+          for (int i = 0; i < 8 * DC; ++i)
+            orow[i] = valid && i * 8 < sh.dim ? *reinterpret_cast<const uint4*>(osrc + i * 8) : make_uint4(0, 0, 0, 0);
+          const int64_t stat = (int64_t)(it.b * g.units + it.u) * g.ldr + R;
+          if (valid) nlse = lse[stat];
+          if (!umma::mbar_wait(&qd_full[qd.s], qd.phase, 0xa8)) {
+            abort_flag = 1;
+            break;
+          }
+          const uint8_t* go = smem + qd.s * Y::TILES + DC * TILE;
+#pragma unroll
+          for (int i = 0; i < 8 * DC; ++i) {
+            const uint4 d4 = *reinterpret_cast<const uint4*>(go + (i >> 3) * TILE + sw128(row, i & 7));
+            const T* oe = reinterpret_cast<const T*>(&orow[i]);
+            const T* de = reinterpret_cast<const T*>(&d4);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) nd = fmaf(-Elem<T>::to_f(oe[e]), Elem<T>::to_f(de[e]), nd);
+          }
+          if (valid) delta[stat] = nd;
+          nd_s[dturn.s * 128 + row] = nd;
+          nl_s[dturn.s * 128 + row] = nlse;
+          warp_arrive(&qd_empty[qd.s], false);
+          __syncwarp();
+          if (lane == 0) umma::mbar_arrive(&d_full[dturn.s]);
+        }
+        if (!umma::mbar_wait(&sd_full[gr.s], gr.phase, 0xaa) || !umma::mbar_wait(&d_full[dturn.s], dturn.phase, 0xa9)) {
+          abort_flag = 1;
+          break;
+        }
+        umma::tc_fence_after();
+        const int keys = cu.keys();
         if (!idle) {
+          const float nd = nd_s[dturn.s * 128 + row], nlse = nl_s[dturn.s * 128 + row];
+          const uint64_t nd2 = pk2(nd, nd), nlse2 = pk2(nlse, nlse);
+          const uint32_t bh = (uint32_t)(it.b * sh.heads + head);
 #pragma unroll 1
           for (int first = 0; first < keys; first += 32) {
             uint32_t su[32], du[32];
-            tmem_ld32_nowait(lanes + first, su);
-            tmem_ld32_nowait(lanes + Y::kTmemDP + first, du);
-            uint32_t w[16];
-            if (DROP) {
-#pragma unroll
-              for (int gr = 0; gr < 4; ++gr) {  // drawn while the products come
-                const uint4 r = rng((uint32_t)(kc + first) / 8 + gr, (uint32_t)pos, bh);
-                w[gr * 4] = r.x;
-                w[gr * 4 + 1] = r.y;
-                w[gr * 4 + 2] = r.z;
-                w[gr * 4 + 3] = r.w;
-              }
-            }
+            tmem_ld32_nowait(acc + first, su);
+            tmem_ld32_nowait(acc + 64 + first, du);
             tmem_wait2(su, du);
             uint32_t p2[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float d0 = __uint_as_float(du[2 * i]), d1 = __uint_as_float(du[2 * i + 1]), p0, p1;
-              unpk2(fma2(pk2(__uint_as_float(su[2 * i]), __uint_as_float(su[2 * i + 1])), sl22, nlse2), p0, p1);
-              uint64_t x;
-              if (DROP) {
-                d0 = kept(w[i], 0, drop.high) ? d0 : 0.f;
-                d1 = kept(w[i], 1, drop.high) ? d1 : 0.f;
-                x = fma2(pk2(d0, d1), mult2, nd2);
-              } else {
-                x = add2(pk2(d0, d1), nd2);
+            for (int q8 = 0; q8 < 4; ++q8) {
+              uint4 r = make_uint4(0, 0, 0, 0);
+              if (DROP) r = rng((uint32_t)(cu.c * BC + first) / 8 + q8, (uint32_t)pos, bh);
+              const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int i = q8 * 4 + e;
+                float d0 = __uint_as_float(du[2 * i]), d1 = __uint_as_float(du[2 * i + 1]), p0, p1;
+                unpk2(fma2(pk2(__uint_as_float(su[2 * i]), __uint_as_float(su[2 * i + 1])), sl22, nlse2), p0, p1);
+                uint64_t x;
+                if (DROP) {
+                  d0 = kept(w[e], 0, drop.high) ? d0 : 0.f;
+                  d1 = kept(w[e], 1, drop.high) ? d1 : 0.f;
+                  x = fma2(pk2(d0, d1), mult2, nd2);
+                } else {
+                  x = add2(pk2(d0, d1), nd2);
+                }
+                unpk2(mul2(pk2(ex2(p0), ex2(p1)), x), p0, p1);
+                p2[i] = pack2<T>(p0, p1);
               }
-              unpk2(mul2(pk2(ex2(p0), ex2(p1)), x), p0, p1);
-              p2[i] = pack2<T>(p0, p1);
             }
             if (first + 32 > keys) zero_tail(p2, keys - first);
-            umma::tmem_st16(lanes + first / 2, p2);  // over scores this warp has read
+            umma::tmem_st16(acc + first / 2, p2);  // over scores this warp has read
           }
           umma::tmem_wait_st();
         }
         const bool pad = keys < BC && sh.lengths != nullptr;
         if (pad)  // S of this chunk is formed: its keys behind the length become zeros
-          zero_rows<DC>(smem + Y::OFF_KV + kv.s * Y::STAGE, CT, keys, (keys + 15) & ~15, threadIdx.x - 64);
-        warp_arrive(ds_full, pad);
-      }
-      if (!ok || !umma::mbar_wait(dq_full, t & 1, 0xac)) {
-        abort_flag = 1;
-        break;
-      }
-      umma::tc_fence_after();
+          zero_rows<DC>(smem + Y::OFF_KV + kv.s * Y::STAGE, CT, keys, (keys + 15) & ~15, row);
+        warp_arrive(&ds_full[gr.s], pad);
+        if (last) {
+          if (!umma::mbar_wait(&dq_full[turn.s], turn.phase, 0xac)) {
+            abort_flag = 1;
+            break;
+          }
+          umma::tc_fence_after();
+          T* dst = dq + it.b * pdq.s_b + pos * pdq.s_n + head * pdq.s_h;
 #pragma unroll 1
-      for (int k = 0; k < 2 * DC; ++k) {
-        if (idle || k * 32 >= sh.dim) break;
-        uint32_t a[32];
-        tmem_ld32_nowait(lanes + Y::kTmemDQ + k * 32, a);
-        wait_ld();
-        tie32(a);
-        if (valid) store_row<T>(dst(), k * 32, sh.dim, a, sh.scale);
+          for (int k = 0; k < 2 * DC; ++k) {
+            if (idle || k * 32 >= sh.dim) break;
+            uint32_t a[32];
+            tmem_ld32_nowait(tmem + lane_off + Y::kTmemDQ + k * 32, a);
+            wait_ld();
+            tie32(a);
+            if (valid) store_row<T>(dst, k * 32, sh.dim, a, sh.scale);
+          }
+          warp_arrive(dq_empty, false);
+        }
       }
-      warp_arrive(dq_empty, false);
-      ++t;
+      if (last) {
+        qd.next();
+        turn.next();
+        dturn.next();
+      }
     }
   }
   umma::tc_fence_before();
   __syncthreads();
   if (warp == 0) {
     umma::tc_fence_after();
-    umma::tmem_dealloc(tmem, Y::kCols);
+    umma::tmem_dealloc(tmem, 512);
   }
 }
 
 // -------------------------------------------------------- backward: dK, dV
 // Item = 128 keys of a key / value head; the packed rows of all its units
 // come in chunks of 64 with their lse2 and D.  S^T = K Q^T and dP^T = V dO^T
-// put a key in each tensor memory lane; the row threads write P^T and dS^T,
-// as 16-bit pairs, over the accumulators they have read, where dV += P^T dO
-// and dK += dS^T Q take them.  The dropout bits come in groups of eight keys
-// of one query, that is of eight lanes: each lane draws the groups of four of
-// 32 columns and the eight exchange the keep bits by shuffles, so a group is
-// still drawn once.
+// put a key in each tensor memory lane; dV += P^T dO, dK += dS^T Q.  The
+// dropout bits come in groups of eight keys of one query, that is of eight
+// lanes: each lane draws the groups of four of 32 columns and the eight
+// exchange the keep bits by shuffles, so a group is still drawn once.
 namespace bk {
-constexpr int kStages = 4;
-constexpr int BC = 64;                 // packed rows per chunk
-constexpr int CT = BC * 128;
 template <int DC>
 struct L {
-  static constexpr int OFF_V = DC * TILE;
-  static constexpr int OFF_CH = 2 * DC * TILE;
-  static constexpr int OFF_STAT = 2 * DC * CT;              // within a stage: -lse2[64], -D[64]
+  static constexpr int NB = DC == 1 ? 3 : 2;                // 512 columns: 128 NB + dV + dK
+  static constexpr int kTiles = DC == 1 ? 2 : 1;            // K, V tiles
+  static constexpr int kN = DC == 1 ? 8 : 4;
+  static constexpr int TILES = 2 * DC * TILE;
+  static constexpr int OFF_STAT = 2 * DC * bw::CT;          // within a stage: -lse2[64], -D[64]
   static constexpr int STAGE = OFF_STAT + 1024;
-  static constexpr int kN = DC == 1 ? kStages : kStages - 1;
+  static constexpr int OFF_CH = kTiles * TILES;
   static constexpr int OFF_BAR = OFF_CH + kN * STAGE;
-  static constexpr int SMEM = OFF_BAR + 256 + 1024;
-  static constexpr uint32_t kTmemDP = 64, kTmemDV = 128, kTmemDK = 128 + 64 * DC;
-  static constexpr uint32_t kCols = DC == 1 ? 256 : 512;
+  static constexpr int SMEM = OFF_BAR + 512 + 1024;
+  static constexpr uint32_t kTmemDV = 128 * NB, kTmemDK = 128 * NB + 64 * DC;
 };
-constexpr int kBars = 2 + 2 * kStages + 5;
 }  // namespace bk
 
-template <typename T, int DC, bool DROP>
-__global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
-    xattn_bwd_dkdv(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                   const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
-                   const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk,
-                   T* __restrict__ dv, Plane pdk, Plane pdv, Shape sh, Geometry g, int kblk, DropArgs drop) {
-  using namespace bk;
-  using Y = bk::L<DC>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = align1024(smem_raw);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Y::OFF_BAR);
-  uint64_t* kv_full = bars;
-  uint64_t* kv_empty = bars + 1;
-  uint64_t* ch_full = bars + 2;
-  uint64_t* ch_empty = ch_full + kStages;
-  uint64_t* sd_full = ch_empty + kStages;
-  uint64_t* ps_full = sd_full + 1;
-  uint64_t* ps_done = ps_full + 1;
-  uint64_t* acc_full = ps_done + 1;
-  uint64_t* acc_empty = acc_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
-  __shared__ int abort_flag;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int gp_mask = (1 << g.gp_shift) - 1;
-  const int per_unit = (g.rows + BC - 1) / BC;
-  if (threadIdx.x == 0) {
-    umma::mbar_init(kv_full, 1);
-    umma::mbar_init(kv_empty, 1);
-    for (int s = 0; s < kStages; ++s) {
-      umma::mbar_init(&ch_full[s], 1);
-      umma::mbar_init(&ch_empty[s], 1);
-    }
-    umma::mbar_init(sd_full, 1);
-    umma::mbar_init(ps_full, 4);
-    umma::mbar_init(ps_done, 1);
-    umma::mbar_init(acc_full, 1);
-    umma::mbar_init(acc_empty, 4);
-    abort_flag = 0;
-    umma::fence_barrier_init();
-  }
-  if (warp == 0) umma::tmem_alloc(tmem_slot, Y::kCols);
-  umma::tc_fence_before();
-  __syncthreads();
-  umma::tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+// One chunk of the stream of a CTA: key blocks with keys, in order, unit by unit, chunk by chunk.
+struct KeyCursor {
+  int item, blk, kh, b, len, u, r0;
+  uint32_t t, n;  // items and chunks before this one
+  bool live;
 
-  // item -> key block, key / value head, batch item
-  auto at = [&](int item, int& blk, int& kh, int& b) {
+  __device__ __forceinline__ void at(const Shape& sh, int kblk) {
     blk = item % kblk;
     const int r = item / kblk;
     kh = r % sh.kv_heads;
     b = r / sh.kv_heads;
-  };
+    len = sh.keys(b);
+  }
+  __device__ __forceinline__ void seek(const Shape& sh, const Geometry& g, int kblk) {
+    live = false;
+    for (; item < g.total; item += gridDim.x) {
+      at(sh, kblk);
+      u = kh * g.kv_units;
+      r0 = 0;
+      if (blk * BM < len) {
+        live = true;
+        return;
+      }
+    }
+  }
+  __device__ __forceinline__ KeyCursor(const Shape& sh, const Geometry& g, int kblk) : item(blockIdx.x), t(0), n(0) {
+    seek(sh, g, kblk);
+  }
+  __device__ __forceinline__ bool first(const Geometry& g) const { return r0 == 0 && u == kh * g.kv_units; }
+  __device__ __forceinline__ bool last(const Geometry& g) const {
+    return r0 + bw::BC >= g.rows && u + 1 == (kh + 1) * g.kv_units;
+  }
+  __device__ __forceinline__ void next(const Shape& sh, const Geometry& g, int kblk) {
+    ++n;
+    r0 += bw::BC;
+    if (r0 < g.rows) return;
+    r0 = 0;
+    if (++u < (kh + 1) * g.kv_units) return;
+    ++t;
+    item += gridDim.x;
+    seek(sh, g, kblk);
+  }
+};
+
+template <typename T, int DC, bool DROP>
+__global__ void __launch_bounds__(bw::kThreads, 1)
+    xattn_bwd_dkdv(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                   const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
+                   const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk,
+                   T* __restrict__ dv, Plane pdk, Plane pdv, Shape sh, Geometry g, int kblk, DropArgs drop) {
+  using namespace bw;
+  using Y = bk::L<DC>;
+  constexpr int NB = Y::NB;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Y::OFF_BAR);
+  uint64_t* kv_full = bars;                  // [kTiles]
+  uint64_t* kv_empty = kv_full + Y::kTiles;  // [kTiles]
+  uint64_t* ch_full = kv_empty + Y::kTiles;  // [kN]
+  uint64_t* ch_empty = ch_full + Y::kN;      // [kN]
+  uint64_t* sd_full = ch_empty + Y::kN;      // [NB]
+  uint64_t* ps_full = sd_full + NB;           // [NB]
+  uint64_t* ps_done = ps_full + NB;           // [NB]
+  uint64_t* acc_full = ps_done + NB;          // [NB]
+  uint64_t* acc_empty = acc_full + NB;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 1);
+  __shared__ int abort_flag;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // uniform in a warp
+  const int gp_mask = (1 << g.gp_shift) - 1;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < Y::kTiles; ++i) {
+      umma::mbar_init(&kv_full[i], 1);
+      umma::mbar_init(&kv_empty[i], 1);
+    }
+    for (int i = 0; i < Y::kN; ++i) {
+      umma::mbar_init(&ch_full[i], 1);
+      umma::mbar_init(&ch_empty[i], 1);
+    }
+    for (int i = 0; i < NB; ++i) {
+      umma::mbar_init(&sd_full[i], 1);
+      umma::mbar_init(&ps_full[i], 4);
+      umma::mbar_init(&ps_done[i], 1);
+      umma::mbar_init(&acc_full[i], 1);
+    }
+    umma::mbar_init(acc_empty, 4);
+    abort_flag = 0;
+    umma::fence_barrier_init();
+  }
+  if (warp == 0) umma::tmem_alloc(tmem_slot, 512);
+  umma::tc_fence_before();
+  __syncthreads();
+  umma::tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp == 0) {
-    if (lane == 0) {  // K and V tiles of an item, then the query chunks
+    if (lane == 0) {  // tiles of an item before its first chunk
       umma::tma_prefetch(&tmK);
       umma::tma_prefetch(&tmV);
       umma::tma_prefetch(&tmQ);
       umma::tma_prefetch(&tmDO);
-      uint32_t t = 0;
+      Ring<Y::kTiles> kv;
       Ring<Y::kN> ch;
-      bool ok = true;
-      for (int item = blockIdx.x; item < g.total && ok && !abort_flag; item += gridDim.x) {
-        int blk, kh, b;
-        at(item, blk, kh, b);
-        if (blk * BM >= sh.keys(b)) continue;
-        if (!umma::mbar_wait(kv_empty, (t & 1) ^ 1, 0xb1)) {
-          ok = false;
+      for (KeyCursor cu(sh, g, kblk); cu.live && !abort_flag; cu.next(sh, g, kblk), ch.next()) {
+        if (cu.first(g)) {
+          if (!umma::mbar_wait(&kv_empty[kv.s], kv.phase ^ 1, 0xb1)) {
+            abort_flag = 1;
+            break;
+          }
+          uint8_t* dst = smem + kv.s * Y::TILES;
+          umma::mbar_arrive_expect_tx(&kv_full[kv.s], Y::TILES);
+#pragma unroll
+          for (int dc = 0; dc < DC; ++dc) {
+            umma::tma_load_4d(dst + dc * TILE, &tmK, &kv_full[kv.s], dc * 64, cu.blk * BM, cu.kh, cu.b);
+            umma::tma_load_4d(dst + (DC + dc) * TILE, &tmV, &kv_full[kv.s], dc * 64, cu.blk * BM, cu.kh, cu.b);
+          }
+          kv.next();
+        }
+        if (!umma::mbar_wait(&ch_empty[ch.s], ch.phase ^ 1, 0xb2)) {
+          abort_flag = 1;
           break;
         }
-        umma::mbar_arrive_expect_tx(kv_full, 2 * DC * TILE);
+        uint8_t* dst = smem + Y::OFF_CH + ch.s * Y::STAGE;
+        umma::mbar_arrive_expect_tx(&ch_full[ch.s], 2 * DC * CT + 2 * BC * 4);
 #pragma unroll
         for (int dc = 0; dc < DC; ++dc) {
-          umma::tma_load_4d(smem + dc * TILE, &tmK, kv_full, dc * 64, blk * BM, kh, b);
-          umma::tma_load_4d(smem + Y::OFF_V + dc * TILE, &tmV, kv_full, dc * 64, blk * BM, kh, b);
+          umma::tma_load_5d(dst + dc * CT, &tmQ, &ch_full[ch.s], dc * 64, 0, cu.r0 >> g.gp_shift, cu.u, cu.b);
+          umma::tma_load_5d(dst + (DC + dc) * CT, &tmDO, &ch_full[ch.s], dc * 64, 0, cu.r0 >> g.gp_shift, cu.u, cu.b);
         }
-        for (int u = kh * g.kv_units; u < (kh + 1) * g.kv_units && ok; ++u) {
-          for (int r0 = 0; r0 < g.rows; r0 += BC, ch.next()) {
-            if (!umma::mbar_wait(&ch_empty[ch.s], ch.phase ^ 1, 0xb2)) {
-              ok = false;
-              break;
-            }
-            uint8_t* dst = smem + Y::OFF_CH + ch.s * Y::STAGE;
-            umma::mbar_arrive_expect_tx(&ch_full[ch.s], 2 * DC * CT + 2 * BC * 4);
-#pragma unroll
-            for (int dc = 0; dc < DC; ++dc) {
-              umma::tma_load_5d(dst + dc * CT, &tmQ, &ch_full[ch.s], dc * 64, 0, r0 >> g.gp_shift, u, b);
-              umma::tma_load_5d(dst + (DC + dc) * CT, &tmDO, &ch_full[ch.s], dc * 64, 0, r0 >> g.gp_shift, u, b);
-            }
-            const int64_t stat = (int64_t)(b * g.units + u) * g.ldr + r0;  // both end 64 values behind the last row
-            umma::bulk_load(dst + Y::OFF_STAT, lse + stat, BC * 4, &ch_full[ch.s]);
-            umma::bulk_load(dst + Y::OFF_STAT + BC * 4, delta + stat, BC * 4, &ch_full[ch.s]);
-          }
-        }
-        ++t;
+        const int64_t stat = (int64_t)(cu.b * g.units + cu.u) * g.ldr + cu.r0;  // both end 64 values behind the last row
+        umma::bulk_load(dst + Y::OFF_STAT, lse + stat, BC * 4, &ch_full[ch.s]);
+        umma::bulk_load(dst + Y::OFF_STAT + BC * 4, delta + stat, BC * 4, &ch_full[ch.s]);
       }
-      if (!ok) abort_flag = 1;
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      uint32_t cc = 0, t = 0;
-      Ring<Y::kN> ch;
-      const int nch = per_unit * g.kv_units;
+    {  // the whole warp, so that addresses and descriptors stay uniform; one lane issues
+      const bool leader = umma::elect_one();
+      KeyCursor cu(sh, g, kblk), done = cu;  // scores, and products NB - 1 chunks behind
+      Ring<Y::kTiles> kv;
+      Ring<Y::kN> ch, chd;
+      Ring<NB> gr, grd;
+      auto products = [&]() -> bool {
+        const bool first = done.first(g);
+        if (!umma::mbar_wait(&ps_full[grd.s], grd.phase, 0xb6) ||
+            (first && !umma::mbar_wait(acc_empty, (done.t & 1) ^ 1, 0xb7)))
+          return false;
+        umma::tc_fence_after();
+        const uint64_t q = tile_desc(smem + Y::OFF_CH + chd.s * Y::STAGE);
+        const uint32_t acc = tmem + grd.s * 128;
+        const int ksteps = (min(BC, g.rows - done.r0) + 15) >> 4;
+        if (leader) {
+          mma_rows_ts<DC>(tmem + Y::kTmemDV, acc, q + DC * CT / 16, CT, Desc<T>::MN, ksteps, !first);
+          mma_rows_ts<DC>(tmem + Y::kTmemDK, acc + 64, q, CT, Desc<T>::MN, ksteps, !first);
+          umma::mma_commit(&ps_done[grd.s]);
+          umma::mma_commit(&ch_empty[chd.s]);
+          if (done.last(g)) umma::mma_commit(&acc_full[done.t % NB]);
+        }
+        __syncwarp();
+        done.next(sh, g, kblk);
+        grd.next();
+        chd.next();
+        return true;
+      };
       bool ok = true;
-      for (int item = blockIdx.x; item < g.total && ok && !abort_flag; item += gridDim.x) {
-        int blk, kh, b;
-        at(item, blk, kh, b);
-        if (blk * BM >= sh.keys(b)) continue;
-        if (!umma::mbar_wait(kv_full, t & 1, 0xb3)) {
+      for (; cu.live && !abort_flag; cu.next(sh, g, kblk), ch.next(), gr.next()) {
+        if ((cu.first(g) && !umma::mbar_wait(&kv_full[kv.s], kv.phase, 0xb3)) ||
+            !umma::mbar_wait(&ch_full[ch.s], ch.phase, 0xb4) || !umma::mbar_wait(&ps_done[gr.s], gr.phase ^ 1, 0xb5)) {
           ok = false;
           break;
         }
-        int r0 = 0;  // first row of the chunk in its unit
-        for (int c = 0; c < nch; ++c, ++cc, ch.next()) {
-          const int ksteps = (min(BC, g.rows - r0) + 15) >> 4;
-          if (!umma::mbar_wait(&ch_full[ch.s], ch.phase, 0xb4) ||
-              (cc > 0 && !umma::mbar_wait(ps_done, (cc - 1) & 1, 0xb5))) {
-            ok = false;
-            break;
-          }
-          umma::tc_fence_after();
-          const uint32_t q = umma::smem_u32(smem + Y::OFF_CH + ch.s * Y::STAGE), idesc = Desc<T>::kk(ksteps * 16);
-          mma_scores<DC>(tmem, umma::smem_u32(smem), TILE, q, CT, idesc);
-          mma_scores<DC>(tmem + Y::kTmemDP, umma::smem_u32(smem + Y::OFF_V), TILE, q + DC * CT, CT, idesc);
-          umma::mma_commit(sd_full);
-          if (c == nch - 1) umma::mma_commit(kv_empty);
-          if (!umma::mbar_wait(ps_full, cc & 1, 0xb6) ||
-              (c == 0 && !umma::mbar_wait(acc_empty, (t & 1) ^ 1, 0xb7))) {
-            ok = false;
-            break;
-          }
-          umma::tc_fence_after();
-          mma_rows_ts<DC>(tmem + Y::kTmemDV, tmem, q + DC * CT, CT, Desc<T>::MN, ksteps, c > 0);
-          mma_rows_ts<DC>(tmem + Y::kTmemDK, tmem + Y::kTmemDP, q, CT, Desc<T>::MN, ksteps, c > 0);
-          umma::mma_commit(ps_done);
-          umma::mma_commit(&ch_empty[ch.s]);
-          if (c == nch - 1) umma::mma_commit(acc_full);
-          r0 += BC;
-          if (r0 >= g.rows) r0 = 0;
+        umma::tc_fence_after();
+        const uint64_t q = tile_desc(smem + Y::OFF_CH + ch.s * Y::STAGE), k = tile_desc(smem + kv.s * Y::TILES);
+        const uint32_t idesc = Desc<T>::kk((min(BC, g.rows - cu.r0) + 15) & ~15), acc = tmem + gr.s * 128;
+        const bool last = cu.last(g);
+        if (leader) {
+          mma_scores<DC>(acc, k, TILE, q, CT, idesc);
+          mma_scores<DC>(acc + 64, k + DC * TILE / 16, TILE, q + DC * CT / 16, CT, idesc);
+          umma::mma_commit(&sd_full[gr.s]);
+          if (last) umma::mma_commit(&kv_empty[kv.s]);
         }
-        ++t;
+        __syncwarp();
+        if (last) kv.next();
+        if (cu.n >= NB - 1 && !products()) {
+          ok = false;
+          break;
+        }
       }
+      while (ok && done.live && done.n < cu.n) ok = products();
       if (!ok) abort_flag = 1;
     }
   } else {
-    const int quarter = warp & 3, row = quarter * 32 + lane;
-    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    const int grp = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const float sl2 = sh.scale * kLog2e, mult = DROP ? drop.scale : 1.f;
     const uint64_t sl22 = pk2(sl2, sl2), mult2 = pk2(mult, mult);
     const Philox rng(DROP ? drop : DropArgs{});
-    uint32_t cc = 0, t = 0;
-    Ring<Y::kN> ch;
-    for (int item = blockIdx.x; item < g.total && !abort_flag; item += gridDim.x) {
-      int blk, kh, b;
-      at(item, blk, kh, b);
-      const int len = sh.keys(b), j = blk * BM + row;
-      const bool exists = j < sh.nk, live = j < len, idle = blk * BM + quarter * 32 >= len;
-      auto out_k = [&] { return dk + b * pdk.s_b + j * pdk.s_n + kh * pdk.s_h; };
-      auto out_v = [&] { return dv + b * pdv.s_b + j * pdv.s_n + kh * pdv.s_h; };
-      auto zeros = [&] {
-        for (int d = 0; d < sh.dim; d += 8) {
-          *reinterpret_cast<uint4*>(out_k() + d) = make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(out_v() + d) = make_uint4(0, 0, 0, 0);
-        }
-      };
-      if (blk * BM >= len) {
-        if (exists) zeros();
-        continue;
+    auto zeros = [&](const KeyCursor& c) {
+      const int j = c.blk * BM + row;
+      T* ok_ = dk + c.b * pdk.s_b + j * pdk.s_n + c.kh * pdk.s_h;
+      T* ov = dv + c.b * pdv.s_b + j * pdv.s_n + c.kh * pdv.s_h;
+      for (int d = 0; d < sh.dim; d += 8) {
+        *reinterpret_cast<uint4*>(ok_ + d) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(ov + d) = make_uint4(0, 0, 0, 0);
       }
-      bool ok = true;
-      for (int u = kh * g.kv_units; u < (kh + 1) * g.kv_units && ok; ++u) {
-        for (int r0 = 0; r0 < g.rows; r0 += BC, ++cc, ch.next()) {
-          const int rows = min(BC, g.rows - r0);
-          // the statistics are read from the stage: wait for its TMA as well as for the products
-          if (!umma::mbar_wait(&ch_full[ch.s], ch.phase, 0xb8) || !umma::mbar_wait(sd_full, cc & 1, 0xb9)) {
-            ok = false;
-            break;
-          }
-          umma::tc_fence_after();
-          if (!idle) {
-            const float* stats = reinterpret_cast<const float*>(smem + Y::OFF_CH + ch.s * Y::STAGE + Y::OFF_STAT);
+    };
+    // keys at or behind the length: zeros
+    if (grp == 0 && sh.lengths != nullptr) {
+      KeyCursor c(sh, g, kblk);
+      for (c.item = blockIdx.x; c.item < g.total; c.item += gridDim.x) {
+        c.at(sh, kblk);
+        if (c.blk * BM + row >= c.len && c.blk * BM + row < sh.nk) zeros(c);
+      }
+    }
+    Ring<Y::kN> ch;
+    Ring<NB> gr;     // accumulators of the cursor's chunk
+    Ring<NB> turn;   // of the items
+    for (KeyCursor cu(sh, g, kblk); cu.live && !abort_flag; cu.next(sh, g, kblk), ch.next(), gr.next()) {
+      const bool last = cu.last(g);
+      if ((int)(cu.n % G) == grp) {
+        const uint32_t acc = tmem + lane_off + gr.s * 128;
+        const int j = cu.blk * BM + row, rows = min(BC, g.rows - cu.r0);
+        const bool live = j < cu.len, idle = cu.blk * BM + quarter * 32 >= cu.len;
+        // the statistics are read from the stage: wait for its TMA as well as for the products
+        if (!umma::mbar_wait(&ch_full[ch.s], ch.phase, 0xb8) || !umma::mbar_wait(&sd_full[gr.s], gr.phase, 0xb9)) {
+          abort_flag = 1;
+          break;
+        }
+        umma::tc_fence_after();
+        if (!idle) {
+          const float* stats = reinterpret_cast<const float*>(smem + Y::OFF_CH + ch.s * Y::STAGE + Y::OFF_STAT);
 #pragma unroll 1
-            for (int c0 = 0; c0 < rows; c0 += 32) {
-              uint32_t su[32], du[32];
-              tmem_ld32_nowait(lanes + c0, su);
-              tmem_ld32_nowait(lanes + Y::kTmemDP + c0, du);
-              uint32_t word = 0;  // keep bits of four columns x eight keys, drawn by this lane for its eight
-              if (DROP) {
+          for (int c0 = 0; c0 < rows; c0 += 32) {
+            uint32_t word = 0;  // keep bits of four columns x eight keys, drawn by this lane for its eight
+            if (DROP) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const int r = r0 + c0 + (lane & 7) * 4 + e;
-                  const uint32_t bh = (uint32_t)(b * sh.heads + (u << g.gp_shift) + (r & gp_mask));
-                  word |= keep_bits(rng((uint32_t)j >> 3, (uint32_t)(r >> g.gp_shift), bh), drop.limit) << (8 * e);
-                }
+              for (int e = 0; e < 4; ++e) {
+                const int r = cu.r0 + c0 + (lane & 7) * 4 + e;
+                const uint32_t bh = (uint32_t)(cu.b * sh.heads + (cu.u << g.gp_shift) + (r & gp_mask));
+                word |= keep_bits(rng((uint32_t)j >> 3, (uint32_t)(r >> g.gp_shift), bh), drop.limit) << (8 * e);
               }
-              tmem_wait2(su, du);
-              uint32_t pp[16], pd[16];
+            }
+            uint32_t pp[16], pd[16];
 #pragma unroll
-              for (int q4 = 0; q4 < 8; ++q4) {
+            for (int h = 0; h < 2; ++h) {
+              uint32_t su[16], du[16];
+              tmem_ld16_nowait(acc + c0 + h * 16, su);
+              tmem_ld16_nowait(acc + 64 + c0 + h * 16, du);
+              tmem_wait16(su, du);
+#pragma unroll
+              for (int q4 = 0; q4 < 4; ++q4) {
                 uint32_t bits = 0;
-                if (DROP) bits = __shfl_sync(0xffffffffu, word, (lane & 24) + q4) >> (lane & 7);
-                const float4 l4 = *reinterpret_cast<const float4*>(stats + c0 + 4 * q4);
-                const float4 d4 = *reinterpret_cast<const float4*>(stats + BC + c0 + 4 * q4);
+                if (DROP) bits = __shfl_sync(0xffffffffu, word, (lane & 24) + h * 4 + q4) >> (lane & 7);
+                const float4 l4 = *reinterpret_cast<const float4*>(stats + c0 + h * 16 + 4 * q4);
+                const float4 d4 = *reinterpret_cast<const float4*>(stats + BC + c0 + h * 16 + 4 * q4);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                   const int i = 4 * q4 + 2 * e;
@@ -1139,47 +1281,50 @@ __global__ void __launch_bounds__(bw::kThreads, DC == 1 ? 2 : 1)
                     x = add2(pk2(d0, d1), nd);
                   }
                   unpk2(mul2(pk2(p0, p1), x), d0, d1);
-                  pp[2 * q4 + e] = pack2<T>(q0, q1);
-                  pd[2 * q4 + e] = pack2<T>(d0, d1);
+                  pp[h * 8 + 2 * q4 + e] = pack2<T>(q0, q1);
+                  pd[h * 8 + 2 * q4 + e] = pack2<T>(d0, d1);
                 }
               }
-              if (c0 + 32 > rows) {  // queries behind the last: their statistics are someone else's, so zeros outright
-                zero_tail(pp, rows - c0);
-                zero_tail(pd, rows - c0);
-              }
-              umma::tmem_st16(lanes + c0 / 2, pp);  // over accumulators this warp has read
-              umma::tmem_st16(lanes + Y::kTmemDP + c0 / 2, pd);
             }
-            umma::tmem_wait_st();
+            if (c0 + 32 > rows) {  // queries behind the last: their statistics are someone else's, so zeros outright
+              zero_tail(pp, rows - c0);
+              zero_tail(pd, rows - c0);
+            }
+            umma::tmem_st16(acc + c0 / 2, pp);  // over accumulators this warp has read
+            umma::tmem_st16(acc + 64 + c0 / 2, pd);
           }
-          warp_arrive(ps_full, false);
+          umma::tmem_wait_st();
+        }
+        warp_arrive(&ps_full[gr.s], false);
+        if (last) {
+          if (!umma::mbar_wait(&acc_full[turn.s], turn.phase, 0xbb)) {
+            abort_flag = 1;
+            break;
+          }
+          umma::tc_fence_after();
+          T* out_k = dk + cu.b * pdk.s_b + j * pdk.s_n + cu.kh * pdk.s_h;
+          T* out_v = dv + cu.b * pdv.s_b + j * pdv.s_n + cu.kh * pdv.s_h;
+#pragma unroll 1
+          for (int k = 0; k < 4 * DC; ++k) {
+            const int d0 = (k >> 1) * 32;
+            if (idle || d0 >= sh.dim) break;
+            uint32_t a[32];
+            tmem_ld32_nowait(tmem + lane_off + ((k & 1) ? Y::kTmemDK : Y::kTmemDV) + d0, a);
+            wait_ld();
+            tie32(a);
+            if (live) store_row<T>((k & 1) ? out_k : out_v, d0, sh.dim, a, (k & 1) ? sh.scale : mult);
+          }
+          warp_arrive(acc_empty, false);
         }
       }
-      if (!ok || !umma::mbar_wait(acc_full, t & 1, 0xbb)) {
-        abort_flag = 1;
-        break;
-      }
-      umma::tc_fence_after();
-#pragma unroll 1
-      for (int k = 0; k < 4 * DC; ++k) {
-        const int d0 = (k >> 1) * 32;
-        if (idle || d0 >= sh.dim) break;
-        uint32_t a[32];
-        tmem_ld32_nowait(lanes + ((k & 1) ? Y::kTmemDK : Y::kTmemDV) + d0, a);
-        wait_ld();
-        tie32(a);
-        if (live) store_row<T>((k & 1) ? out_k() : out_v(), d0, sh.dim, a, (k & 1) ? sh.scale : mult);
-      }
-      if (exists && !live) zeros();
-      warp_arrive(acc_empty, false);
-      ++t;
+      if (last) turn.next();
     }
   }
   umma::tc_fence_before();
   __syncthreads();
   if (warp == 0) {
     umma::tc_fence_after();
-    umma::tmem_dealloc(tmem, Y::kCols);
+    umma::tmem_dealloc(tmem, 512);
   }
 }
 
@@ -1298,23 +1443,22 @@ int forward_launch(const Shape& sh, const Forward& a, Geometry g, const char* na
 
 template <typename T, int DC, bool DROP>
 int backward_launch(const Shape& sh, const Backward& a, Geometry g, const char* name) {
-  CUtensorMap q128, do128, q64, do64, k96, v96, k128, v128;
+  CUtensorMap q128, do128, q64, do64, k64, v64, k128, v128;
   if (int st = query_map(q128, a.q, a.pq, sh, g, a.dtype, BM, name)) return st;
   if (int st = query_map(do128, a.go, a.pgo, sh, g, a.dtype, BM, name)) return st;
-  if (int st = query_map(q64, a.q, a.pq, sh, g, a.dtype, bk::BC, name)) return st;
-  if (int st = query_map(do64, a.go, a.pgo, sh, g, a.dtype, bk::BC, name)) return st;
-  if (int st = key_map(k96, a.k, a.pk, sh, a.dtype, bq::BC, name)) return st;
-  if (int st = key_map(v96, a.v, a.pv, sh, a.dtype, bq::BC, name)) return st;
+  if (int st = query_map(q64, a.q, a.pq, sh, g, a.dtype, bw::BC, name)) return st;
+  if (int st = query_map(do64, a.go, a.pgo, sh, g, a.dtype, bw::BC, name)) return st;
+  if (int st = key_map(k64, a.k, a.pk, sh, a.dtype, bw::BC, name)) return st;
+  if (int st = key_map(v64, a.v, a.pv, sh, a.dtype, bw::BC, name)) return st;
   if (int st = key_map(k128, a.k, a.pk, sh, a.dtype, BM, name)) return st;
   if (int st = key_map(v128, a.v, a.pv, sh, a.dtype, BM, name)) return st;
   float* delta = static_cast<float*>(a.workspace);
-  constexpr int per_sm = DC == 1 ? 2 : 1;
   {
     auto kernel = xattn_bwd_dq<T, DC, DROP>;
     constexpr int smem = bq::L<DC>::SMEM;
     PMB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), name);
-    kernel<<<persistent_grid(g.total, per_sm), bw::kThreads, smem, a.stream>>>(
-        q128, do128, k96, v96, static_cast<const T*>(a.o), a.lse, delta, static_cast<T*>(a.gq), a.po, a.pgq, sh, g,
+    kernel<<<persistent_grid(g.total, 1), bw::kThreads, smem, a.stream>>>(
+        q128, do128, k64, v64, static_cast<const T*>(a.o), a.lse, delta, static_cast<T*>(a.gq), a.po, a.pgq, sh, g,
         a.drop);
     PMB_CHECK_LAUNCH(name);
   }
@@ -1325,7 +1469,7 @@ int backward_launch(const Shape& sh, const Backward& a, Geometry g, const char* 
   auto kernel = xattn_bwd_dkdv<T, DC, DROP>;
   constexpr int smem = bk::L<DC>::SMEM;
   PMB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), name);
-  kernel<<<persistent_grid(items, per_sm), bw::kThreads, smem, a.stream>>>(
+  kernel<<<persistent_grid(items, 1), bw::kThreads, smem, a.stream>>>(
       k128, v128, q64, do64, a.lse, delta, static_cast<T*>(a.gk), static_cast<T*>(a.gv), a.pgk, a.pgv, sh, g, kblk,
       a.drop);
   PMB_CHECK_LAUNCH(name);
