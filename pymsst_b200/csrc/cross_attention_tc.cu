@@ -623,13 +623,14 @@ __global__ void __launch_bounds__(256)
 // One CTA per SM, its row warps two groups of four (one tensor memory lane
 // per thread), NB pairs of 64-column accumulators (S and dP, or their
 // transposes).  Chunk n of the CTA's stream uses pair n % NB and goes to group
-// n % 2.  The MMA lane forms chunk n's scores, then the products of chunk
-// n - (NB - 1), whose 16-bit operands its group has written over the scores
-// and dP it read.  With three pairs the scores a group takes next are ready
-// when it finishes a chunk, and the pair they went to was freed a step
-// earlier: neither side waits for a round trip.  (Time axis, 258 positions,
-// dropout, dK / dV + dQ: one pair per CTA and two CTAs per SM 321 + 219 us,
-// three groups with a pair each 355 + 290.)
+// n % 2.  One warp issues the score products, another the products of the
+// 16-bit operands that a group has written over the scores and dP it read: a
+// wait that is already over still costs a warp about 115 cycles and eight
+// tcgen05.mma about 500, so one warp for both was the bound (1825 cycles per
+// chunk).  With three pairs the scores a group takes next are ready when it
+// finishes a chunk.  (Time axis, 258 positions, dropout, dK / dV + dQ: one
+// pair per CTA and two CTAs per SM 321 + 219 us, three groups with a pair each
+// 355 + 290, this 310 + 247 with one issuing warp.)
 //
 // Barriers that groups wait on out of step have turns: item t uses barrier
 // t % NB.  A chunk's scores are complete only after the products of the chunk
@@ -642,7 +643,7 @@ namespace bw {
 constexpr int BC = 64;                 // chunk rows
 constexpr int CT = BC * 128;           // bytes of a chunk's 64-element sub-tile
 constexpr int G = 2;                   // groups of row warps
-constexpr int kThreads = 64 + 128 * G;
+constexpr int kThreads = 96 + 128 * G;
 }  // namespace bw
 
 // ------------------------------------------------------------ backward: dQ
@@ -670,7 +671,7 @@ struct L {
 struct QueryCursor {
   int item, len, c, nch;
   Item it;
-  uint32_t t, n;  // items and chunks before this one
+  uint32_t n;  // chunks before this one
   bool live;
 
   __device__ __forceinline__ void seek(const Shape& sh, const Geometry& g) {  // from `item` on
@@ -686,16 +687,17 @@ struct QueryCursor {
       }
     }
   }
-  __device__ __forceinline__ QueryCursor(const Shape& sh, const Geometry& g) : item(blockIdx.x), t(0), n(0) {
-    seek(sh, g);
-  }
-  __device__ __forceinline__ void next(const Shape& sh, const Geometry& g) {
+  __device__ __forceinline__ QueryCursor(const Shape& sh, const Geometry& g) : item(blockIdx.x), n(0) { seek(sh, g); }
+  // to the next chunk; true when that begins another item (or ends the stream)
+  __device__ __forceinline__ bool next(const Shape& sh, const Geometry& g) {
     ++n;
-    if (++c < nch) return;
-    ++t;
+    if (++c < nch) return false;
     item += gridDim.x;
     seek(sh, g);
+    return true;
   }
+  __device__ __forceinline__ bool first() const { return c == 0; }
+  __device__ __forceinline__ bool last() const { return c == nch - 1; }
   __device__ __forceinline__ int keys() const { return min(bw::BC, len - c * bw::BC); }
 };
 
@@ -763,7 +765,7 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
       Ring<Y::kTiles> qd;
       Ring<Y::kN> kv;
       for (QueryCursor cu(sh, g); cu.live && !abort_flag; cu.next(sh, g), kv.next()) {
-        if (cu.c == 0) {
+        if (cu.first()) {
           if (!umma::mbar_wait(&qd_empty[qd.s], qd.phase ^ 1, 0xa1)) {
             abort_flag = 1;
             break;
@@ -792,59 +794,60 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
         }
       }
     }
-  } else if (warp == 1) {
-    {  // the whole warp, so that addresses and descriptors stay uniform; one lane issues
-      const bool leader = umma::elect_one();
-      QueryCursor cu(sh, g), done = cu;  // scores, and products NB - 1 chunks behind
-      Ring<Y::kTiles> qd;
-      Ring<Y::kN> kv, kvd;
-      Ring<NB> gr, grd;
-      auto products = [&]() -> bool {
-        if (!umma::mbar_wait(&ds_full[grd.s], grd.phase, 0xa6) ||
-            (done.c == 0 && !umma::mbar_wait(dq_empty, (done.t & 1) ^ 1, 0xa7)))
-          return false;
-        umma::tc_fence_after();
-        if (leader) {
-          mma_rows_ts<DC>(tmem + Y::kTmemDQ, tmem + grd.s * 128, tile_desc(smem + Y::OFF_KV + kvd.s * Y::STAGE), CT,
-                          Desc<T>::MN, (done.keys() + 15) >> 4, done.c > 0);
-          umma::mma_commit(&ds_done[grd.s]);
-          umma::mma_commit(&kv_empty[kvd.s]);
-          if (done.c == done.nch - 1) umma::mma_commit(&dq_full[done.t % NB]);
-        }
-        __syncwarp();
-        done.next(sh, g);
-        grd.next();
-        kvd.next();
-        return true;
-      };
-      bool ok = true;
-      for (; cu.live && !abort_flag; cu.next(sh, g), kv.next(), gr.next()) {
-        if ((cu.c == 0 && !umma::mbar_wait(&qd_full[qd.s], qd.phase, 0xa3)) ||
-            !umma::mbar_wait(&kv_full[kv.s], kv.phase, 0xa4) || !umma::mbar_wait(&ds_done[gr.s], gr.phase ^ 1, 0xa5)) {
-          ok = false;
-          break;
-        }
-        umma::tc_fence_after();
-        const uint64_t k = tile_desc(smem + Y::OFF_KV + kv.s * Y::STAGE), q = tile_desc(smem + qd.s * Y::TILES);
-        const uint32_t idesc = Desc<T>::kk((cu.keys() + 15) & ~15), acc = tmem + gr.s * 128;
-        if (leader) {
-          mma_scores<DC>(acc, q, TILE, k, CT, idesc);
-          mma_scores<DC>(acc + 64, q + DC * TILE / 16, TILE, k + DC * CT / 16, CT, idesc);
-          umma::mma_commit(&sd_full[gr.s]);
-          if (cu.c == cu.nch - 1) umma::mma_commit(&qd_empty[qd.s]);
-        }
-        __syncwarp();
-        if (cu.c == cu.nch - 1) qd.next();
-        if (cu.n >= NB - 1 && !products()) {
-          ok = false;
-          break;
-        }
+  } else if (warp == 1) {  // scores; the whole warp runs along, so that addresses and descriptors stay uniform
+    const bool leader = umma::elect_one();
+    Ring<Y::kTiles> qd;
+    Ring<Y::kN> kv;
+    Ring<NB> gr;
+    for (QueryCursor cu(sh, g); cu.live && !abort_flag;) {
+      if ((cu.first() && !umma::mbar_wait(&qd_full[qd.s], qd.phase, 0xa3)) ||
+          !umma::mbar_wait(&kv_full[kv.s], kv.phase, 0xa4) || !umma::mbar_wait(&ds_done[gr.s], gr.phase ^ 1, 0xa5)) {
+        abort_flag = 1;
+        break;
       }
-      while (ok && done.live && done.n < cu.n) ok = products();
-      if (!ok) abort_flag = 1;
+      umma::tc_fence_after();
+      const uint64_t k = tile_desc(smem + Y::OFF_KV + kv.s * Y::STAGE), q = tile_desc(smem + qd.s * Y::TILES);
+      const uint32_t idesc = Desc<T>::kk((cu.keys() + 15) & ~15), acc = tmem + gr.s * 128;
+      if (leader) {
+        mma_scores<DC>(acc, q, TILE, k, CT, idesc);
+        mma_scores<DC>(acc + 64, q + DC * TILE / 16, TILE, k + DC * CT / 16, CT, idesc);
+        umma::mma_commit(&sd_full[gr.s]);
+        if (cu.last()) umma::mma_commit(&qd_empty[qd.s]);
+      }
+      __syncwarp();
+      kv.next();
+      gr.next();
+      if (cu.next(sh, g)) qd.next();
+    }
+  } else if (warp == 2) {  // products
+    const bool leader = umma::elect_one();
+    Ring<Y::kN> kv;
+    Ring<NB> gr, turn;
+    uint32_t odd = 0;  // items so far, modulo 2
+    for (QueryCursor cu(sh, g); cu.live && !abort_flag;) {
+      const bool first = cu.first();
+      if (!umma::mbar_wait(&ds_full[gr.s], gr.phase, 0xa6) || (first && !umma::mbar_wait(dq_empty, odd ^ 1, 0xa7))) {
+        abort_flag = 1;
+        break;
+      }
+      umma::tc_fence_after();
+      if (leader) {
+        mma_rows_ts<DC>(tmem + Y::kTmemDQ, tmem + gr.s * 128, tile_desc(smem + Y::OFF_KV + kv.s * Y::STAGE), CT,
+                        Desc<T>::MN, (cu.keys() + 15) >> 4, !first);
+        if (cu.last()) umma::mma_commit(&dq_full[turn.s]);  // before the pair is free: see the turns above
+        umma::mma_commit(&ds_done[gr.s]);
+        umma::mma_commit(&kv_empty[kv.s]);
+      }
+      __syncwarp();
+      kv.next();
+      gr.next();
+      if (cu.next(sh, g)) {
+        turn.next();
+        odd ^= 1;
+      }
     }
   } else {
-    const int grp = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const int grp = (warp - 3) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const float sl2 = sh.scale * kLog2e, mult = DROP ? drop.scale : 1.f;
     const uint64_t sl22 = pk2(sl2, sl2), mult2 = pk2(mult, mult);
@@ -864,14 +867,14 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
     Ring<NB> gr;     // accumulators of the cursor's chunk
     Ring<NB> turn;   // of the items
     Ring<2 * NB> dturn;
-    for (QueryCursor cu(sh, g); cu.live && !abort_flag; cu.next(sh, g), kv.next(), gr.next()) {
-      const bool last = cu.c == cu.nch - 1;
+    for (QueryCursor cu(sh, g); cu.live && !abort_flag;) {
       if ((int)(cu.n % G) == grp) {
+        const bool last = cu.last();
         const uint32_t acc = tmem + lane_off + gr.s * 128;
         const Item& it = cu.it;
         const int R = it.blk * BM + row, pos = R >> g.gp_shift, head = (it.u << g.gp_shift) + (R & gp_mask);
         const bool valid = R < g.rows, idle = it.blk * BM + quarter * 32 >= g.rows;
-        if (cu.c == 0) {  // D and the statistics of this item, for all groups
+        if (cu.first()) {  // D and the statistics of this item, for all groups
           float nlse = 0.f, nd = 0.f;
           uint4 orow[8 * DC];
           const T* osrc = o + it.b * po.s_b + pos * po.s_n + head * po.s_h;
@@ -967,7 +970,9 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
           warp_arrive(dq_empty, false);
         }
       }
-      if (last) {
+      kv.next();
+      gr.next();
+      if (cu.next(sh, g)) {
         qd.next();
         turn.next();
         dturn.next();
@@ -1007,9 +1012,9 @@ struct L {
 
 // One chunk of the stream of a CTA: key blocks with keys, in order, unit by unit, chunk by chunk.
 struct KeyCursor {
-  int item, blk, kh, b, len, u, r0;
-  uint32_t t, n;  // items and chunks before this one
-  bool live;
+  int item, blk, kh, b, len, u, u_end, r0;
+  uint32_t n;  // chunks before this one
+  bool live, begins;
 
   __device__ __forceinline__ void at(const Shape& sh, int kblk) {
     blk = item % kblk;
@@ -1018,35 +1023,37 @@ struct KeyCursor {
     b = r / sh.kv_heads;
     len = sh.keys(b);
   }
-  __device__ __forceinline__ void seek(const Shape& sh, const Geometry& g, int kblk) {
+  __device__ __forceinline__ void seek(const Shape& sh, const Geometry& g, int kblk) {  // from `item` on
     live = false;
     for (; item < g.total; item += gridDim.x) {
       at(sh, kblk);
       u = kh * g.kv_units;
+      u_end = u + g.kv_units;
       r0 = 0;
+      begins = true;
       if (blk * BM < len) {
         live = true;
         return;
       }
     }
   }
-  __device__ __forceinline__ KeyCursor(const Shape& sh, const Geometry& g, int kblk) : item(blockIdx.x), t(0), n(0) {
+  __device__ __forceinline__ KeyCursor(const Shape& sh, const Geometry& g, int kblk) : item(blockIdx.x), n(0) {
     seek(sh, g, kblk);
   }
-  __device__ __forceinline__ bool first(const Geometry& g) const { return r0 == 0 && u == kh * g.kv_units; }
-  __device__ __forceinline__ bool last(const Geometry& g) const {
-    return r0 + bw::BC >= g.rows && u + 1 == (kh + 1) * g.kv_units;
-  }
-  __device__ __forceinline__ void next(const Shape& sh, const Geometry& g, int kblk) {
+  // to the next chunk; true when that begins another item (or ends the stream)
+  __device__ __forceinline__ bool next(const Shape& sh, const Geometry& g, int kblk) {
     ++n;
+    begins = false;
     r0 += bw::BC;
-    if (r0 < g.rows) return;
+    if (r0 < g.rows) return false;
     r0 = 0;
-    if (++u < (kh + 1) * g.kv_units) return;
-    ++t;
+    if (++u < u_end) return false;
     item += gridDim.x;
     seek(sh, g, kblk);
+    return true;
   }
+  __device__ __forceinline__ bool first() const { return begins; }
+  __device__ __forceinline__ bool last(const Geometry& g) const { return r0 + bw::BC >= g.rows && u + 1 == u_end; }
 };
 
 template <typename T, int DC, bool DROP>
@@ -1108,7 +1115,7 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
       Ring<Y::kTiles> kv;
       Ring<Y::kN> ch;
       for (KeyCursor cu(sh, g, kblk); cu.live && !abort_flag; cu.next(sh, g, kblk), ch.next()) {
-        if (cu.first(g)) {
+        if (cu.first()) {
           if (!umma::mbar_wait(&kv_empty[kv.s], kv.phase ^ 1, 0xb1)) {
             abort_flag = 1;
             break;
@@ -1138,64 +1145,63 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
         umma::bulk_load(dst + Y::OFF_STAT + BC * 4, delta + stat, BC * 4, &ch_full[ch.s]);
       }
     }
-  } else if (warp == 1) {
-    {  // the whole warp, so that addresses and descriptors stay uniform; one lane issues
-      const bool leader = umma::elect_one();
-      KeyCursor cu(sh, g, kblk), done = cu;  // scores, and products NB - 1 chunks behind
-      Ring<Y::kTiles> kv;
-      Ring<Y::kN> ch, chd;
-      Ring<NB> gr, grd;
-      auto products = [&]() -> bool {
-        const bool first = done.first(g);
-        if (!umma::mbar_wait(&ps_full[grd.s], grd.phase, 0xb6) ||
-            (first && !umma::mbar_wait(acc_empty, (done.t & 1) ^ 1, 0xb7)))
-          return false;
-        umma::tc_fence_after();
-        const uint64_t q = tile_desc(smem + Y::OFF_CH + chd.s * Y::STAGE);
-        const uint32_t acc = tmem + grd.s * 128;
-        const int ksteps = (min(BC, g.rows - done.r0) + 15) >> 4;
-        if (leader) {
-          mma_rows_ts<DC>(tmem + Y::kTmemDV, acc, q + DC * CT / 16, CT, Desc<T>::MN, ksteps, !first);
-          mma_rows_ts<DC>(tmem + Y::kTmemDK, acc + 64, q, CT, Desc<T>::MN, ksteps, !first);
-          umma::mma_commit(&ps_done[grd.s]);
-          umma::mma_commit(&ch_empty[chd.s]);
-          if (done.last(g)) umma::mma_commit(&acc_full[done.t % NB]);
-        }
-        __syncwarp();
-        done.next(sh, g, kblk);
-        grd.next();
-        chd.next();
-        return true;
-      };
-      bool ok = true;
-      for (; cu.live && !abort_flag; cu.next(sh, g, kblk), ch.next(), gr.next()) {
-        if ((cu.first(g) && !umma::mbar_wait(&kv_full[kv.s], kv.phase, 0xb3)) ||
-            !umma::mbar_wait(&ch_full[ch.s], ch.phase, 0xb4) || !umma::mbar_wait(&ps_done[gr.s], gr.phase ^ 1, 0xb5)) {
-          ok = false;
-          break;
-        }
-        umma::tc_fence_after();
-        const uint64_t q = tile_desc(smem + Y::OFF_CH + ch.s * Y::STAGE), k = tile_desc(smem + kv.s * Y::TILES);
-        const uint32_t idesc = Desc<T>::kk((min(BC, g.rows - cu.r0) + 15) & ~15), acc = tmem + gr.s * 128;
-        const bool last = cu.last(g);
-        if (leader) {
-          mma_scores<DC>(acc, k, TILE, q, CT, idesc);
-          mma_scores<DC>(acc + 64, k + DC * TILE / 16, TILE, q + DC * CT / 16, CT, idesc);
-          umma::mma_commit(&sd_full[gr.s]);
-          if (last) umma::mma_commit(&kv_empty[kv.s]);
-        }
-        __syncwarp();
-        if (last) kv.next();
-        if (cu.n >= NB - 1 && !products()) {
-          ok = false;
-          break;
-        }
+  } else if (warp == 1) {  // scores
+    const bool leader = umma::elect_one();
+    Ring<Y::kTiles> kv;
+    Ring<Y::kN> ch;
+    Ring<NB> gr;
+    for (KeyCursor cu(sh, g, kblk); cu.live && !abort_flag;) {
+      if ((cu.first() && !umma::mbar_wait(&kv_full[kv.s], kv.phase, 0xb3)) ||
+          !umma::mbar_wait(&ch_full[ch.s], ch.phase, 0xb4) || !umma::mbar_wait(&ps_done[gr.s], gr.phase ^ 1, 0xb5)) {
+        abort_flag = 1;
+        break;
       }
-      while (ok && done.live && done.n < cu.n) ok = products();
-      if (!ok) abort_flag = 1;
+      umma::tc_fence_after();
+      const uint64_t q = tile_desc(smem + Y::OFF_CH + ch.s * Y::STAGE), k = tile_desc(smem + kv.s * Y::TILES);
+      const uint32_t idesc = Desc<T>::kk((min(BC, g.rows - cu.r0) + 15) & ~15), acc = tmem + gr.s * 128;
+      if (leader) {
+        mma_scores<DC>(acc, k, TILE, q, CT, idesc);
+        mma_scores<DC>(acc + 64, k + DC * TILE / 16, TILE, q + DC * CT / 16, CT, idesc);
+        umma::mma_commit(&sd_full[gr.s]);
+        if (cu.last(g)) umma::mma_commit(&kv_empty[kv.s]);
+      }
+      __syncwarp();
+      ch.next();
+      gr.next();
+      if (cu.next(sh, g, kblk)) kv.next();
+    }
+  } else if (warp == 2) {  // products
+    const bool leader = umma::elect_one();
+    Ring<Y::kN> ch;
+    Ring<NB> gr, turn;
+    uint32_t odd = 0;  // items so far, modulo 2
+    for (KeyCursor cu(sh, g, kblk); cu.live && !abort_flag;) {
+      const bool first = cu.first();
+      if (!umma::mbar_wait(&ps_full[gr.s], gr.phase, 0xb6) || (first && !umma::mbar_wait(acc_empty, odd ^ 1, 0xb7))) {
+        abort_flag = 1;
+        break;
+      }
+      umma::tc_fence_after();
+      const uint64_t q = tile_desc(smem + Y::OFF_CH + ch.s * Y::STAGE);
+      const uint32_t acc = tmem + gr.s * 128;
+      const int ksteps = (min(BC, g.rows - cu.r0) + 15) >> 4;
+      if (leader) {
+        mma_rows_ts<DC>(tmem + Y::kTmemDV, acc, q + DC * CT / 16, CT, Desc<T>::MN, ksteps, !first);
+        mma_rows_ts<DC>(tmem + Y::kTmemDK, acc + 64, q, CT, Desc<T>::MN, ksteps, !first);
+        if (cu.last(g)) umma::mma_commit(&acc_full[turn.s]);
+        umma::mma_commit(&ps_done[gr.s]);
+        umma::mma_commit(&ch_empty[ch.s]);
+      }
+      __syncwarp();
+      ch.next();
+      gr.next();
+      if (cu.next(sh, g, kblk)) {
+        turn.next();
+        odd ^= 1;
+      }
     }
   } else {
-    const int grp = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const int grp = (warp - 3) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const float sl2 = sh.scale * kLog2e, mult = DROP ? drop.scale : 1.f;
     const uint64_t sl22 = pk2(sl2, sl2), mult2 = pk2(mult, mult);
@@ -1220,9 +1226,9 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
     Ring<Y::kN> ch;
     Ring<NB> gr;     // accumulators of the cursor's chunk
     Ring<NB> turn;   // of the items
-    for (KeyCursor cu(sh, g, kblk); cu.live && !abort_flag; cu.next(sh, g, kblk), ch.next(), gr.next()) {
-      const bool last = cu.last(g);
+    for (KeyCursor cu(sh, g, kblk); cu.live && !abort_flag;) {
       if ((int)(cu.n % G) == grp) {
+        const bool last = cu.last(g);
         const uint32_t acc = tmem + lane_off + gr.s * 128;
         const int j = cu.blk * BM + row, rows = min(BC, g.rows - cu.r0);
         const bool live = j < cu.len, idle = cu.blk * BM + quarter * 32 >= cu.len;
@@ -1317,7 +1323,9 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
           warp_arrive(acc_empty, false);
         }
       }
-      if (last) turn.next();
+      ch.next();
+      gr.next();
+      if (cu.next(sh, g, kblk)) turn.next();
     }
   }
   umma::tc_fence_before();
