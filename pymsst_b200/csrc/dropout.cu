@@ -19,7 +19,7 @@ namespace pmb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;
+constexpr int kUnroll = 2;
 
 enum Mode { kPlain = 0, kResidual = 1, kGelu = 2, kGeluGrad = 3 };
 
@@ -28,12 +28,39 @@ struct alignas(16) Pack8 {
   T v[8];
 };
 
+// Results of two neighbouring elements before the drop: a = x, b = residual or gy.
 template <typename T, int MODE>
-__device__ __forceinline__ float value(float a, float b, bool keep, float c) {
-  if (MODE == kPlain) return keep ? a * c : 0.f;
-  if (MODE == kResidual) return keep ? fmaf(a, c, b) : b;
-  if (MODE == kGelu) return keep ? gelu_of<T>(a) * c : 0.f;
-  return keep ? b * gelu_grad_of<T>(a) * c : 0.f;  // a = x, b = gy
+__device__ __forceinline__ void value2(float a0, float a1, float b0, float b1, float c, bool k0, bool k1, float& y0,
+                                       float& y1) {
+  if (MODE == kPlain || MODE == kResidual) {
+    y0 = k0 ? a0 : 0.f;
+    y1 = k1 ? a1 : 0.f;
+    const uint64_t r = fma2(pk2(y0, y1), pk2(c, c), MODE == kResidual ? pk2(b0, b1) : pk2(0.f, 0.f));
+    unpk2(r, y0, y1);
+    return;
+  }
+  if constexpr (MODE == kGelu) {
+    if constexpr (sizeof(T) == 2) {
+      float p0, p1;
+      uint64_t t;
+      phi_cdf_fast2(a0, a1, p0, p1, t);
+      unpk2(mul2(mul2(pk2(a0, a1), pk2(p0, p1)), pk2(c, c)), y0, y1);
+    } else {
+      y0 = gelu_of<T>(a0) * c;
+      y1 = gelu_of<T>(a1) * c;
+    }
+  } else if constexpr (MODE == kGeluGrad) {
+    float d0, d1;
+    if constexpr (sizeof(T) == 2) {
+      gelu_grad_fast2(a0, a1, d0, d1);
+    } else {
+      d0 = gelu_grad_of<T>(a0);
+      d1 = gelu_grad_of<T>(a1);
+    }
+    unpk2(mul2(mul2(pk2(d0, d1), pk2(b0, b1)), pk2(c, c)), y0, y1);
+  }
+  y0 = k0 ? y0 : 0.f;
+  y1 = k1 ? y1 : 0.f;
 }
 
 template <typename T, int MODE, bool DROP, bool VEC>
@@ -69,9 +96,18 @@ __global__ void __launch_bounds__(kThreads)
       const uint32_t w[4] = {r.x, r.y, r.z, r.w};
       Pack8<T> out;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        out.v[e] = Elem<T>::from_f(value<T, MODE>(Elem<T>::to_f(pa[u].v[e]), kTwo ? Elem<T>::to_f(pb[u].v[e]) : 0.f,
-                                                  !DROP || kept(w[e / 2], e & 1, drop.high), DROP ? drop.scale : 1.f));
+      for (int e = 0; e < 8; e += 2) {
+        float y0, y1;
+        value2<T, MODE>(Elem<T>::to_f(pa[u].v[e]), Elem<T>::to_f(pa[u].v[e + 1]), kTwo ? Elem<T>::to_f(pb[u].v[e]) : 0.f,
+                        kTwo ? Elem<T>::to_f(pb[u].v[e + 1]) : 0.f, DROP ? drop.scale : 1.f,
+                        !DROP || kept(w[e / 2], 0, drop.high), !DROP || kept(w[e / 2], 1, drop.high), y0, y1);
+        if constexpr (sizeof(T) == 2) {
+          reinterpret_cast<uint32_t*>(out.v)[e / 2] = Elem<T>::pack2(y0, y1);
+        } else {
+          out.v[e] = y0;
+          out.v[e + 1] = y1;
+        }
+      }
       if (g < full) {
         reinterpret_cast<Pack8<T>*>(y)[g] = out;
       } else {
@@ -88,9 +124,11 @@ int launch(const void* a, const void* b, void* y, int64_t n, int threshold, cons
            const char* name) {
   const bool vec = ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) |
                      reinterpret_cast<uintptr_t>(y)) & 15) == 0;
-  int64_t grid = ((n + 7) / 8 + kThreads - 1) / kThreads;
-  const int64_t cap = (int64_t)num_sms() * 8;
-  if (grid > cap) grid = cap;
+  // small sizes: one group per thread, spread over the SMs; large ones: kUnroll groups per thread, and no more than
+  // 2^30 CTAs
+  const int64_t groups = (n + 7) / 8, per = groups > (int64_t)num_sms() * 4 * kThreads ? kUnroll : 1;
+  int64_t grid = (groups + kThreads * per - 1) / (kThreads * per);
+  if (grid > (1 << 30)) grid = 1 << 30;
   auto kernel = threshold > 0 ? (vec ? dropout_kernel<T, MODE, true, true> : dropout_kernel<T, MODE, true, false>)
                               : (vec ? dropout_kernel<T, MODE, false, true> : dropout_kernel<T, MODE, false, false>);
   kernel<<<(unsigned)grid, kThreads, 0, s>>>(static_cast<const T*>(a), static_cast<const T*>(b), static_cast<T*>(y), n,

@@ -38,63 +38,99 @@ struct alignas(sizeof(T) * 2 * P < 16 ? sizeof(T) * 2 * P : 16) Pairs {
   T v[2 * P];
 };
 
-// One CTA per (batch, token tile), `tiles` of them per batch; tile * rotated pairs <= kAngles.
+// Position of a vector in a tile, moved on by a fixed step without divisions.
+struct Place {
+  int t, h, c;  // token, head, vector of the head
+};
+
+// One CTA per (batch, token tile), `tiles` of them per batch; tile * pitch <= kAngles (pitch: rotated pairs, made even
+// so that a token's angles start on 16 bytes).
 template <typename T, typename PosT, int P>
 __global__ void __launch_bounds__(kThreads)
     rotary_axes_kernel(const T* __restrict__ x, const PosT* __restrict__ pos, const float* __restrict__ freqs,
-                       T* __restrict__ y, int tokens, int heads, int pairs, int tile, int tiles, View vx, View vy,
-                       int64_t pos_b, Axes axes, float sign) {
-  __shared__ float2 cs[kAngles];
+                       T* __restrict__ y, int tokens, int heads, int pairs, int tile, int tiles, int pitch, View vx,
+                       View vy, int64_t pos_b, Axes axes, float sign) {
+  __shared__ __align__(16) float2 cs[kAngles];
   const int rot = axes.end[axes.count - 1];
   const int64_t b = blockIdx.x / tiles;
   const int t0 = (int)(blockIdx.x - b * tiles) * tile, nt = tokens - t0 < tile ? tokens - t0 : tile;
-  const int per_head = pairs / P, per_token = heads * per_head, total = nt * per_token;
+  const int per_head = pairs / P, per_token = heads * per_head;
   x += b * vx.s_b + (int64_t)t0 * vx.s_n;
   y += b * vy.s_b + (int64_t)t0 * vy.s_n;
 
-  Pairs<T, P> buf[kUnroll];
-  auto load = [&](int base) {
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int i = base + u * kThreads;
-      if (i < total) {
-        const int t = i / per_token, r = i - t * per_token, h = r / per_head, c = r - h * per_head;
-        buf[u] = *reinterpret_cast<const Pairs<T, P>*>(x + t * vx.s_n + h * vx.s_h + c * 2 * P);
-      }
+  auto place = [&](int i) {
+    Place p;
+    p.t = i / per_token;
+    const int r = i - p.t * per_token;
+    p.h = r / per_head;
+    p.c = r - p.h * per_head;
+    return p;
+  };
+  const Place step = place(kThreads);
+  auto advance = [&](Place& p) {
+    p.c += step.c;
+    p.h += step.h;
+    p.t += step.t;
+    if (p.c >= per_head) {
+      p.c -= per_head;
+      ++p.h;
+    }
+    if (p.h >= heads) {
+      p.h -= heads;
+      ++p.t;
     }
   };
-  load(threadIdx.x);
+  Pairs<T, P> buf[kUnroll];
+  auto load = [&](Place p) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (p.t < nt) buf[u] = *reinterpret_cast<const Pairs<T, P>*>(x + p.t * vx.s_n + p.h * vx.s_h + p.c * 2 * P);
+      advance(p);
+    }
+  };
+  Place at = place(threadIdx.x);
+  load(at);
   for (int i = threadIdx.x; i < nt * rot; i += kThreads) {
     const int t = i / rot, p = i - t * rot;
     int a = 0;
-    while (p >= axes.end[a]) ++a;
+#pragma unroll
+    for (int k = 0; k + 1 < kMaxAxes; ++k) a += p >= axes.end[k] ? 1 : 0;
     const double where = (double)pos[b * pos_b + (int64_t)(t0 + t) * axes.count + a];
     double turns = where * (double)freqs[p] * 0.15915494309189533577;
     turns -= rint(turns);
     float s, c;
     sincospif(2.f * (float)turns, &s, &c);
-    cs[i] = make_float2(c, s * sign);
+    cs[t * pitch + p] = make_float2(c, s * sign);
   }
   __syncthreads();
-  for (int base = threadIdx.x; base < total; base += kThreads * kUnroll) {
-    if (base != threadIdx.x) load(base);
+  for (bool more = false; at.t < nt; more = true) {
+    if (more) load(at);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int i = base + u * kThreads;
-      if (i >= total) break;
-      const int t = i / per_token, r = i - t * per_token, h = r / per_head, c = r - h * per_head;
-      Pairs<T, P> out = buf[u];
+      if (at.t < nt) {
+        Pairs<T, P> out = buf[u];
+        const float2* w = cs + at.t * pitch + at.c * P;
+        const int live = rot - at.c * P;  // rotated pairs from this vector on
+        float2 cv[P];
+        if (P > 1 && live >= P) {
 #pragma unroll
-      for (int j = 0; j < P; ++j) {
-        const int p = c * P + j;
-        if (p < rot) {
-          const float2 w = cs[t * rot + p];
-          const float e = Elem<T>::to_f(buf[u].v[2 * j]), o = Elem<T>::to_f(buf[u].v[2 * j + 1]);
-          out.v[2 * j] = Elem<T>::from_f(e * w.x - o * w.y);
-          out.v[2 * j + 1] = Elem<T>::from_f(o * w.x + e * w.y);
+          for (int j = 0; j < P; j += 2) *reinterpret_cast<float4*>(cv + j) = *reinterpret_cast<const float4*>(w + j);
+        } else {
+#pragma unroll
+          for (int j = 0; j < P; ++j)
+            if (j < live) cv[j] = w[j];
         }
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          if (j < live) {
+            const float e = Elem<T>::to_f(buf[u].v[2 * j]), o = Elem<T>::to_f(buf[u].v[2 * j + 1]);
+            out.v[2 * j] = Elem<T>::from_f(e * cv[j].x - o * cv[j].y);
+            out.v[2 * j + 1] = Elem<T>::from_f(o * cv[j].x + e * cv[j].y);
+          }
+        }
+        *reinterpret_cast<Pairs<T, P>*>(y + at.t * vy.s_n + at.h * vy.s_h + at.c * 2 * P) = out;
       }
-      *reinterpret_cast<Pairs<T, P>*>(y + t * vy.s_n + h * vy.s_h + c * 2 * P) = out;
+      advance(at);
     }
   }
 }
@@ -113,7 +149,8 @@ int launch(const void* x, const void* pos, const float* freqs, void* y, int64_t 
   // tokens per CTA: kUnroll vectors per thread, as many as the angle slots allow
   const int64_t per_token = (int64_t)heads * (vec ? pairs / P : pairs);
   int64_t tile = (int64_t)kThreads * kUnroll / per_token;
-  if (tile > kAngles / rot) tile = kAngles / rot;
+  const int pitch = (rot + 1) / 2 * 2;
+  if (tile > kAngles / pitch) tile = kAngles / pitch;
   if (tile < 1) tile = 1;
   if (tile > tokens) tile = tokens;
   const int64_t tiles = (tokens + tile - 1) / tile;
@@ -122,11 +159,11 @@ int launch(const void* x, const void* pos, const float* freqs, void* y, int64_t 
   if (vec)
     rotary_axes_kernel<T, PosT, P><<<grid, kThreads, 0, s>>>(
         static_cast<const T*>(x), static_cast<const PosT*>(pos), freqs, static_cast<T*>(y), tokens, heads, pairs,
-        (int)tile, (int)tiles, vx, vy, pos_b, axes, sign);
+        (int)tile, (int)tiles, pitch, vx, vy, pos_b, axes, sign);
   else
     rotary_axes_kernel<T, PosT, 1><<<grid, kThreads, 0, s>>>(
         static_cast<const T*>(x), static_cast<const PosT*>(pos), freqs, static_cast<T*>(y), tokens, heads, pairs,
-        (int)tile, (int)tiles, vx, vy, pos_b, axes, sign);
+        (int)tile, (int)tiles, pitch, vx, vy, pos_b, axes, sign);
   PMB_CHECK_LAUNCH(name);
   return PMB_OK;
 }
