@@ -38,14 +38,48 @@ struct alignas(sizeof(T) * 2 * P < 16 ? sizeof(T) * 2 * P : 16) Pairs {
   T v[2 * P];
 };
 
-// Position of a vector in a tile, moved on by a fixed step without divisions.
-struct Place {
-  int t, h, c;  // token, head, vector of the head
-};
+// Rotated vector: P pairs, `live` of them (or all) by the angles at w.
+template <typename T, int P>
+__device__ __forceinline__ Pairs<T, P> rotated(const Pairs<T, P>& in, const float2* w, int live) {
+  Pairs<T, P> out = in;
+  if (live >= P) {
+    float2 cv[P];
+    if constexpr (P > 1) {
+#pragma unroll
+      for (int j = 0; j < P; j += 2) *reinterpret_cast<float4*>(cv + j) = *reinterpret_cast<const float4*>(w + j);
+    } else {
+      cv[0] = w[0];
+    }
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      const float e = Elem<T>::to_f(in.v[2 * j]), o = Elem<T>::to_f(in.v[2 * j + 1]);
+      const float ye = e * cv[j].x - o * cv[j].y, yo = o * cv[j].x + e * cv[j].y;
+      if constexpr (sizeof(T) == 2) {
+        reinterpret_cast<uint32_t*>(out.v)[j] = Elem<T>::pack2(ye, yo);
+      } else {
+        out.v[2 * j] = ye;
+        out.v[2 * j + 1] = yo;
+      }
+    }
+  } else if (live > 0) {
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      if (j < live) {
+        const float2 c = w[j];
+        const float e = Elem<T>::to_f(in.v[2 * j]), o = Elem<T>::to_f(in.v[2 * j + 1]);
+        out.v[2 * j] = Elem<T>::from_f(e * c.x - o * c.y);
+        out.v[2 * j + 1] = Elem<T>::from_f(o * c.x + e * c.y);
+      }
+    }
+  }
+  return out;
+}
 
 // One CTA per (batch, token tile), `tiles` of them per batch; tile * pitch <= kAngles (pitch: rotated pairs, made even
-// so that a token's angles start on 16 bytes).
-template <typename T, typename PosT, int P>
+// so that a token's angles start on 16 bytes).  ROWS: the CTA's threads are a multiple of the vectors of a token, so a
+// thread keeps its head and its place in the head and steps over tokens; otherwise (tokens of more than kThreads
+// vectors) each vector's place is divided out.
+template <typename T, typename PosT, int P, bool ROWS>
 __global__ void __launch_bounds__(kThreads)
     rotary_axes_kernel(const T* __restrict__ x, const PosT* __restrict__ pos, const float* __restrict__ freqs,
                        T* __restrict__ y, int tokens, int heads, int pairs, int tile, int tiles, int pitch, View vx,
@@ -54,43 +88,31 @@ __global__ void __launch_bounds__(kThreads)
   const int rot = axes.end[axes.count - 1];
   const int64_t b = blockIdx.x / tiles;
   const int t0 = (int)(blockIdx.x - b * tiles) * tile, nt = tokens - t0 < tile ? tokens - t0 : tile;
-  const int per_head = pairs / P, per_token = heads * per_head;
+  const int per_head = pairs / P, per_token = heads * per_head, total = nt * per_token;
   x += b * vx.s_b + (int64_t)t0 * vx.s_n;
   y += b * vy.s_b + (int64_t)t0 * vy.s_n;
+  // this thread's first vector: token, head, place in the head
+  const int tt = threadIdx.x / per_token, rr = threadIdx.x - tt * per_token, hh = rr / per_head, cc = rr - hh * per_head;
+  const int step = ROWS ? (int)blockDim.x / per_token : 0;
 
-  auto place = [&](int i) {
-    Place p;
-    p.t = i / per_token;
-    const int r = i - p.t * per_token;
-    p.h = r / per_head;
-    p.c = r - p.h * per_head;
-    return p;
-  };
-  const Place step = place(kThreads);
-  auto advance = [&](Place& p) {
-    p.c += step.c;
-    p.h += step.h;
-    p.t += step.t;
-    if (p.c >= per_head) {
-      p.c -= per_head;
-      ++p.h;
-    }
-    if (p.h >= heads) {
-      p.h -= heads;
-      ++p.t;
-    }
-  };
   Pairs<T, P> buf[kUnroll];
-  auto load = [&](Place p) {
+  auto load = [&](int first) {  // ROWS: a token, else a vector of the tile
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      if (p.t < nt) buf[u] = *reinterpret_cast<const Pairs<T, P>*>(x + p.t * vx.s_n + p.h * vx.s_h + p.c * 2 * P);
-      advance(p);
+      if constexpr (ROWS) {
+        const int t = first + u * step;
+        if (t < nt) buf[u] = *reinterpret_cast<const Pairs<T, P>*>(x + t * vx.s_n + hh * vx.s_h + cc * 2 * P);
+      } else {
+        const int i = first + u * kThreads;
+        if (i < total) {
+          const int t = i / per_token, r = i - t * per_token, h = r / per_head, c = r - h * per_head;
+          buf[u] = *reinterpret_cast<const Pairs<T, P>*>(x + t * vx.s_n + h * vx.s_h + c * 2 * P);
+        }
+      }
     }
   };
-  Place at = place(threadIdx.x);
-  load(at);
-  for (int i = threadIdx.x; i < nt * rot; i += kThreads) {
+  load(ROWS ? tt : (int)threadIdx.x);
+  for (int i = threadIdx.x; i < nt * rot; i += blockDim.x) {
     const int t = i / rot, p = i - t * rot;
     int a = 0;
 #pragma unroll
@@ -103,34 +125,30 @@ __global__ void __launch_bounds__(kThreads)
     cs[t * pitch + p] = make_float2(c, s * sign);
   }
   __syncthreads();
-  for (bool more = false; at.t < nt; more = true) {
-    if (more) load(at);
+  if constexpr (ROWS) {
+    const int live = rot - cc * P;
+    const float2* w = cs + cc * P;
+    T* dst = y + hh * vy.s_h + cc * 2 * P;
+    for (int first = tt; first < nt; first += kUnroll * step) {
+      if (first != tt) load(first);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (at.t < nt) {
-        Pairs<T, P> out = buf[u];
-        const float2* w = cs + at.t * pitch + at.c * P;
-        const int live = rot - at.c * P;  // rotated pairs from this vector on
-        float2 cv[P];
-        if (P > 1 && live >= P) {
-#pragma unroll
-          for (int j = 0; j < P; j += 2) *reinterpret_cast<float4*>(cv + j) = *reinterpret_cast<const float4*>(w + j);
-        } else {
-#pragma unroll
-          for (int j = 0; j < P; ++j)
-            if (j < live) cv[j] = w[j];
-        }
-#pragma unroll
-        for (int j = 0; j < P; ++j) {
-          if (j < live) {
-            const float e = Elem<T>::to_f(buf[u].v[2 * j]), o = Elem<T>::to_f(buf[u].v[2 * j + 1]);
-            out.v[2 * j] = Elem<T>::from_f(e * cv[j].x - o * cv[j].y);
-            out.v[2 * j + 1] = Elem<T>::from_f(o * cv[j].x + e * cv[j].y);
-          }
-        }
-        *reinterpret_cast<Pairs<T, P>*>(y + at.t * vy.s_n + at.h * vy.s_h + at.c * 2 * P) = out;
+      for (int u = 0; u < kUnroll; ++u) {
+        const int t = first + u * step;
+        if (t < nt) *reinterpret_cast<Pairs<T, P>*>(dst + t * vy.s_n) = rotated<T, P>(buf[u], w + t * pitch, live);
       }
-      advance(at);
+    }
+  } else {
+    for (int first = threadIdx.x; first < total; first += kThreads * kUnroll) {
+      if (first != (int)threadIdx.x) load(first);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int i = first + u * kThreads;
+        if (i < total) {
+          const int t = i / per_token, r = i - t * per_token, h = r / per_head, c = r - h * per_head;
+          *reinterpret_cast<Pairs<T, P>*>(y + t * vy.s_n + h * vy.s_h + c * 2 * P) =
+              rotated<T, P>(buf[u], cs + t * pitch + c * P, rot - c * P);
+        }
+      }
     }
   }
 }
@@ -148,7 +166,9 @@ int launch(const void* x, const void* pos, const float* freqs, void* y, int64_t 
   const int rot = axes.end[axes.count - 1];
   // tokens per CTA: kUnroll vectors per thread, as many as the angle slots allow
   const int64_t per_token = (int64_t)heads * (vec ? pairs / P : pairs);
-  int64_t tile = (int64_t)kThreads * kUnroll / per_token;
+  const bool rows = per_token <= kThreads;
+  const int block = rows ? (int)(kThreads / per_token * per_token) : kThreads;
+  int64_t tile = (int64_t)block * kUnroll / per_token;
   const int pitch = (rot + 1) / 2 * 2;
   if (tile > kAngles / pitch) tile = kAngles / pitch;
   if (tile < 1) tile = 1;
@@ -156,14 +176,10 @@ int launch(const void* x, const void* pos, const float* freqs, void* y, int64_t 
   const int64_t tiles = (tokens + tile - 1) / tile;
   PMB_REQUIRE(tiles * batch < ((int64_t)1 << 31), "%s: too many tokens", name);
   const unsigned grid = (unsigned)(tiles * batch);
-  if (vec)
-    rotary_axes_kernel<T, PosT, P><<<grid, kThreads, 0, s>>>(
-        static_cast<const T*>(x), static_cast<const PosT*>(pos), freqs, static_cast<T*>(y), tokens, heads, pairs,
-        (int)tile, (int)tiles, pitch, vx, vy, pos_b, axes, sign);
-  else
-    rotary_axes_kernel<T, PosT, 1><<<grid, kThreads, 0, s>>>(
-        static_cast<const T*>(x), static_cast<const PosT*>(pos), freqs, static_cast<T*>(y), tokens, heads, pairs,
-        (int)tile, (int)tiles, pitch, vx, vy, pos_b, axes, sign);
+  auto kernel = vec ? (rows ? rotary_axes_kernel<T, PosT, P, true> : rotary_axes_kernel<T, PosT, P, false>)
+                    : (rows ? rotary_axes_kernel<T, PosT, 1, true> : rotary_axes_kernel<T, PosT, 1, false>);
+  kernel<<<grid, block, 0, s>>>(static_cast<const T*>(x), static_cast<const PosT*>(pos), freqs, static_cast<T*>(y),
+                                tokens, heads, pairs, (int)tile, (int)tiles, pitch, vx, vy, pos_b, axes, sign);
   PMB_CHECK_LAUNCH(name);
   return PMB_OK;
 }
