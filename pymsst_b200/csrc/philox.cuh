@@ -46,6 +46,25 @@ inline DropArgs drop_args(const int64_t* key, uint32_t site, int threshold) {
 }
 
 #ifdef __CUDACC__
+// One call by itself.
+__device__ __forceinline__ uint4 philox(const DropArgs& d, uint32_t c0, uint32_t c1, uint32_t c2) {
+  const uint64_t seed = (uint64_t)__ldg(reinterpret_cast<const long long*>(d.key));
+  uint32_t a = (uint32_t)seed, b = (uint32_t)(seed >> 32) ^ d.site;
+  uint32_t c3 = (uint32_t)__ldg(reinterpret_cast<const long long*>(d.key) + 1);
+#pragma unroll
+  for (int r = 0; r < 7; ++r) {
+    const uint64_t p0 = (uint64_t)c0 * 0xD2511F53u, p1 = (uint64_t)c2 * 0xCD9E8D57u;
+    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ a;
+    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ b;
+    c1 = (uint32_t)p1;
+    c3 = (uint32_t)p0;
+    a += 0x9E3779B9u;
+    b += 0xBB67AE85u;
+  }
+  return make_uint4(c0, c1, c2, c3);
+}
+
+// Many calls under one key.
 struct Philox {
   uint32_t ka[7], kb[7], step;  // the rounds' keys, held in registers: 14 additions per call less
 

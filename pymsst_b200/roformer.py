@@ -44,6 +44,8 @@ import torch.nn.functional as F
 from torch import nn
 
 from . import bands as band_tables
+from .cross_attention import cross_attention
+from .dropout import DropoutGenerator, dropout, gelu_dropout
 from .fused import (
     AttentionFn,
     AttentionGateFn,
@@ -194,6 +196,13 @@ def _attention(q, k, v, dropout_p, backend="auto"):
     return F.scaled_dot_product_attention(q, k, v, dropout_p=dropout_p)
 
 
+def _dropout_sum(x, p, key, site, residual):
+    """residual + dropout(x): one pass when both have one type."""
+    if residual is None or residual.dtype == x.dtype:
+        return dropout(x, p, key, site, residual=residual)
+    return dropout(x, p, key, site) + residual
+
+
 class Attention(nn.Module):
     def __init__(self, dim, heads=8, dim_head=64, dropout=0.0, rotary_embed=None, flash=True):
         super().__init__()
@@ -207,6 +216,7 @@ class Attention(nn.Module):
         self.to_gates = nn.Linear(dim, heads)
         self.to_out = nn.Sequential(nn.Linear(inner, dim, bias=False), nn.Dropout(dropout))
         self.attention_backend = "auto"
+        self.dropout_site = 0  # of the probabilities; the output's dropout has the next one
 
     def set_cuda_attention_backend(self, backend: str) -> None:
         """Attention kernel choice, the hook the reference's training module calls on every module
@@ -216,10 +226,13 @@ class Attention(nn.Module):
             raise ValueError(f"unknown cuda attention backend {backend!r}; expected one of {ATTENTION_BACKENDS}")
         self.attention_backend = name
 
-    def forward(self, x, seq_len=None, inner=1, residual=None):
+    def forward(self, x, seq_len=None, inner=1, residual=None, dropout_key=None):
         """x [b, n, d]; or any [..., d] whose rows are ordered (outer, position, inner) with sequences of
         ``seq_len`` positions (sequence = outer * inner + inner index).  With ``residual`` (same shape as x)
-        the block returns residual + attention(x), the addition done by the output projection GEMM."""
+        the block returns residual + attention(x), the addition done by the output projection GEMM.
+
+        ``dropout_key`` (a key of DropoutGenerator): live dropout takes its masks from the key, on the probabilities
+        inside the attention kernels and after the output projection together with the residual sum."""
         d = x.shape[-1]
         n = x.shape[-2] if seq_len is None else seq_len
         rows = x.numel() // d
@@ -250,7 +263,10 @@ class Attention(nn.Module):
             else:
                 q, k, v, xg = QKVRotaryFn.apply(xn.reshape(b, n, d), self.to_qkv.weight, cos, sin, cos_t, sin_t,
                                                 self.heads, inner, True)
-                attn = _attention(q, k, v, dropout_p, self.attention_backend)
+                if dropout_key is not None and dropout_p > 0.0:
+                    attn = cross_attention(q, k, v, dropout_p=dropout_p, key=dropout_key, site=self.dropout_site)
+                else:
+                    attn = _attention(q, k, v, dropout_p, self.attention_backend)
             gated = AttentionGateFn.apply(attn, xg.reshape(rows, d), self.to_gates.weight, self.to_gates.bias,
                                           inner)
         drop = self.to_out[1]
@@ -258,7 +274,10 @@ class Attention(nn.Module):
             # residual + gated W^T in one GEMM (C = residual, beta = 1)
             res = residual.reshape(rows, d).to(gated.dtype)
             return OutProjFn.apply(res, gated, self.to_out[0].weight).reshape(x.shape)
-        out = drop(F.linear(gated, self.to_out[0].weight.to(gated.dtype))).reshape(x.shape)
+        out = F.linear(gated, self.to_out[0].weight.to(gated.dtype)).reshape(x.shape)
+        if dropout_key is not None and self.training and drop.p > 0.0:
+            return _dropout_sum(out, drop.p, dropout_key, self.dropout_site + 1, residual)
+        out = drop(out)
         return out if residual is None else out + residual
 
 
@@ -269,14 +288,20 @@ class FeedForward(nn.Module):
         self.net = nn.Sequential(
             RMSNorm(dim), nn.Linear(dim, inner), nn.GELU(), nn.Dropout(dropout), nn.Linear(inner, dim), nn.Dropout(dropout)
         )
+        self.dropout_site = 0  # of the activation; the output's dropout has the next one
 
-    def forward(self, x, add_residual=False):
+    def forward(self, x, add_residual=False, dropout_key=None):
         """ff(x), or ff(x) + x with ``add_residual`` (the residual branch's gradient of x then joins the norm's
-        backward pass)."""
-        if add_residual:
-            h, res = self.net[0].with_residual(x)
-            return self._ff(h) + res
-        return self._ff(self.net[0](x))
+        backward pass).  ``dropout_key`` as in Attention.forward: GELU with its dropout is then one pass, the output's
+        dropout and the residual sum another."""
+        h, res = self.net[0].with_residual(x) if add_residual else (self.net[0](x), None)
+        if dropout_key is not None and self.training and (self.net[3].p > 0 or self.net[5].p > 0):
+            dt, site = h.dtype, self.dropout_site
+            h = F.linear(h, self.net[1].weight.to(dt), self.net[1].bias.to(dt))
+            h = gelu_dropout(h, self.net[3].p, dropout_key, site)
+            h = F.linear(h, self.net[4].weight.to(dt), self.net[4].bias.to(dt))
+            return _dropout_sum(h, self.net[5].p, dropout_key, site + 1, res)
+        return self._ff(h) + res if add_residual else self._ff(h)
 
     def _ff(self, h):
         dt = h.dtype
@@ -312,11 +337,11 @@ class Transformer(nn.Module):
         )
         self.norm = RMSNorm(dim) if norm_output else nn.Identity()
 
-    def forward(self, x, seq_len=None, inner=1):
+    def forward(self, x, seq_len=None, inner=1, dropout_key=None):
         """x [b, n, d], or rows in (outer, position, inner) order (see Attention.forward)."""
         for attn, ff in self.layers:
-            x = attn(x, seq_len, inner, residual=x)
-            x = ff(x, add_residual=True)
+            x = attn(x, seq_len, inner, residual=x, dropout_key=dropout_key)
+            x = ff(x, add_residual=True, dropout_key=dropout_key)
         return self.norm(x)
 
 
@@ -422,6 +447,27 @@ class _Roformer(nn.Module):
         self.multi_stft_kwargs = dict(hop_length=multi_stft_hop_size, normalized=multi_stft_normalized)
         self._device_tables: dict = {}
         self._windows: dict = {}
+        self.dropout_generator: DropoutGenerator | None = None
+
+    def set_dropout_generator(self, generator: DropoutGenerator | None) -> None:
+        """Take live dropout (attn_dropout / ff_dropout in training) from ``generator``, or, with None, from torch's
+        as before.  Every dropout of the model gets a site of its own and each forward one key, so a recomputed
+        transformer (use_torch_checkpoint) draws the same masks, in a captured step too, where every replay draws new
+        ones.  Data-parallel ranks need generators of different seeds.  CUDA only."""
+        site = 0
+        for module in self.modules():
+            if isinstance(module, (Attention, FeedForward)):
+                module.dropout_site = site
+                site += 2
+        self.dropout_generator = generator
+
+    def _dropout_key(self):
+        """The key of this forward, or None where no dropout draws from the generator."""
+        if self.dropout_generator is None or not self.training:
+            return None
+        live = any(isinstance(m, nn.Dropout) and m.p > 0 for m in self.modules()) or any(
+            isinstance(m, Attention) and m.dropout > 0 for m in self.modules())
+        return self.dropout_generator.next_key() if live else None
 
     # ------------------------------------------------------------ helpers
     def _window(self, n: int, device: torch.device) -> torch.Tensor:
@@ -459,6 +505,7 @@ class _Roformer(nn.Module):
 
     def _axial(self, x):
         store = []
+        key = self._dropout_key()
         for time_t, freq_t in self.layers:
             if self.skip_connection:
                 for prev in store:
@@ -466,8 +513,8 @@ class _Roformer(nn.Module):
             b, t, f, d = x.shape
             # rows stay in (b, t, f) order for both axes: the time transformer's sequences are (b, f) pairs
             # over t (inner = f), the frequency transformer's are (b, t) pairs over f
-            x = self._run_transformer(time_t, x, seq_len=t, inner=f)
-            x = self._run_transformer(freq_t, x.reshape(b * t, f, d)).reshape(b, t, f, d)
+            x = self._run_transformer(time_t, x, seq_len=t, inner=f, dropout_key=key)
+            x = self._run_transformer(freq_t, x.reshape(b * t, f, d), dropout_key=key).reshape(b, t, f, d)
             if self.skip_connection:
                 store.append(x)
         return self.final_norm(x)
@@ -476,14 +523,15 @@ class _Roformer(nn.Module):
         """One axial transformer; with ``use_torch_checkpoint`` (training, gradients on) its activations are
         recomputed in the backward instead of kept (torch.utils.checkpoint, non-reentrant), as pymss-core
         does per transformer.  Dropout masks are replayed exactly only when dropout is live (the RNG state is
-        then saved, which a captured CUDA graph does not allow)."""
+        then saved, which a captured CUDA graph does not allow, unless the masks come from a dropout key)."""
         if not (self.use_torch_checkpoint and self.training and torch.is_grad_enabled()):
             return transformer(x, **kwargs)
         from torch.utils.checkpoint import checkpoint
 
         dropout_live = any(isinstance(m, nn.Dropout) and m.p > 0 for m in transformer.modules()) or any(
             getattr(m, "dropout", 0.0) > 0 for m in transformer.modules() if isinstance(m, Attention))
-        return checkpoint(transformer, x, use_reentrant=False, preserve_rng_state=dropout_live, **kwargs)
+        keep_rng = dropout_live and kwargs.get("dropout_key") is None
+        return checkpoint(transformer, x, use_reentrant=False, preserve_rng_state=keep_rng, **kwargs)
 
     def _istft(self, spec, window, length):  # spec fp32 [b, n, s, f, t, 2]
         b, n, s, f, t, _ = spec.shape

@@ -56,6 +56,24 @@ def work(name: str, a: tuple) -> tuple[float, float]:
         rows, h, dh, dim, dt, pt = a[9], a[10], a[11], a[12], a[17], a[18]
         return rows * (3 * h * dh + 2 * dim + h) * ES[dt] + 8 * rows * h + 2 * h * (dim + 1) * ES[pt], \
             4.0 * rows * h * (dim + dh)
+    if name == "pmb_dropout":  # x (and the residual) read, y written
+        n, dt = a[3], a[7]
+        return n * ES[dt] * (2 + (a[1] is not None)), 2.0 * n
+    if name == "pmb_gelu_dropout_forward":
+        n, dt = a[2], a[6]
+        return 2.0 * n * ES[dt], 10.0 * n
+    if name == "pmb_gelu_dropout_backward":
+        n, dt = a[3], a[7]
+        return 3.0 * n * ES[dt], 10.0 * n
+    if name == "pmb_cross_attention_forward":  # key lengths live on the device: every key counted
+        b, hq, hk, nq, nk, d, dt = a[6], a[7], a[8], a[9], a[10], a[11], a[17]
+        return 2.0 * b * d * (nq * hq + nk * hk) * ES[dt] + 4 * b * hq * nq, 4.0 * b * hq * nq * nk * d
+    if name == "pmb_cross_attention_backward":
+        b, hq, hk, nq, nk, d, dt = a[10], a[11], a[12], a[13], a[14], a[15], a[21]
+        return 4.0 * b * d * (nq * hq + nk * hk) * ES[dt] + 4 * b * hq * nq, 10.0 * b * hq * nq * nk * d
+    if name == "pmb_rotary_axes":
+        b, n, h, d, axes, dt = a[4], a[5], a[6], a[7], a[11], a[14]
+        return 2.0 * b * n * h * d * ES[dt] + b * n * axes * 4, 3.0 * b * n * h * d
     if name == "pmb_band_gather_forward":
         b, s, f, t, j, xd = a[2], a[3], a[4], a[5], a[6], a[9]
         return b * t * j * 2 * (4 + ES[xd]) + 4 * j, 0.0

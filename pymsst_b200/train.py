@@ -376,6 +376,8 @@ class Trainer:
         from . import _native as nat
 
         static_mix, static_tgt = mixture.clone(), target.clone()
+        generator = getattr(self.model, "dropout_generator", None)
+        steps = None if generator is None else generator.state.clone()
         side = torch.cuda.Stream(self.device)
         side.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(side):
@@ -399,6 +401,8 @@ class Trainer:
         torch.cuda.current_stream(self.device).wait_stream(side)
         self._zero_grads()
         self.check_kernels()
+        if steps is not None:  # the untimed passes drew keys: the captured run draws those an uncaptured one does
+            generator.state.copy_(steps)
         graph = torch.cuda.CUDAGraph()
         before = nat.library().pmb_launch_count()
         with torch.cuda.graph(graph):
