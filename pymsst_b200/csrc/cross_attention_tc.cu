@@ -39,12 +39,26 @@ constexpr int BM = 128;                // rows of a tile
 constexpr int TILE = BM * 128;         // bytes of 128 rows x 64 16-bit elements
 constexpr int kMaxSplits = 64;
 
+// Division of numbers below 2^31 by a divisor known at launch: floor(n m / 2^(31 + s)) with s = ceil(log2 d) and m =
+// ceil(2^(31 + s) / d) (Granlund and Montgomery, PLDI 1994).  Item decoding divides a few times per item and warp.
+struct Divisor {
+  uint32_t mul, shift, d;
+
+  __device__ __forceinline__ int div(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
+  __device__ __forceinline__ int split(int n, int& rest) const {  // quotient, and the remainder in rest
+    const int q = div(n);
+    rest = n - q * (int)d;
+    return q;
+  }
+};
+
 // What a kernel needs to find its tiles.
 struct Geometry {
   int units, gp_shift, kv_units;       // units per batch item, log2 gp, units per key / value head
   int rows, ldr, nblk;                 // packed rows per unit, their pitch in lse, row tiles per unit
   int width, splits;                   // forward: keys per chunk, key ranges per row tile
   int total;                           // work items
+  Divisor by_nblk, by_splits, by_units, by_width, by_kv_units, by_kblk, by_kv_heads;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -182,9 +196,10 @@ template <int N>
 struct Ring {
   int s = 0;
   uint32_t phase = 0;
-  __device__ __forceinline__ void next() {
-    if (++s == N) {
-      s = 0;
+  __device__ __forceinline__ void next(int k = 1) {  // k <= N
+    s += k;
+    if (s >= N) {
+      s -= N;
       phase ^= 1;
     }
   }
@@ -226,23 +241,18 @@ struct Item {
 
 __device__ __forceinline__ Item forward_item(int item, const Geometry& g) {
   Item it;
-  it.blk = item % g.nblk;
-  int r = item / g.nblk;
-  it.split = r % g.splits;
-  r /= g.splits;
-  it.u = r % g.units;
-  it.b = r / g.units;
+  it.b = g.by_units.split(g.by_splits.split(g.by_nblk.split(item, it.blk), it.split), it.u);
   return it;
 }
 
 // Chunks [c0, c1) of an item.
 __device__ __forceinline__ void chunk_range(int len, const Item& it, const Geometry& g, int& c0, int& c1) {
-  const int n = (len + g.width - 1) / g.width;
+  const int n = g.by_width.div(len + g.width - 1);
   c0 = 0;
   c1 = n;
-  if (g.splits > 1) {  // n < 2^30 / 16 and splits <= 64 fit 32 bits
-    c0 = (int)((unsigned)n * (unsigned)it.split / (unsigned)g.splits);
-    c1 = (int)((unsigned)n * (unsigned)(it.split + 1) / (unsigned)g.splits);
+  if (g.splits > 1) {  // n splits < 2^31: the host sees to it
+    c0 = g.by_splits.div(n * it.split);
+    c1 = g.by_splits.div(n * (it.split + 1));
   }
 }
 
@@ -309,7 +319,7 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
 #pragma unroll
         for (int dc = 0; dc < DC; ++dc)
           umma::tma_load_4d(smem + off + (kv.s * DC + dc) * SUB, map, &full[kv.s], dc * 64, c * g.width,
-                            it.u / g.kv_units, it.b);
+                            g.by_kv_units.div(it.u), it.b);
         return true;
       };
       for (int item = blockIdx.x; item < g.total && ok && !abort_flag; item += gridDim.x) {
@@ -636,28 +646,29 @@ __global__ void __launch_bounds__(256)
 // t % NB.  A chunk's scores are complete only after the products of the chunk
 // NB before it, so when a group that has seen the scores of item t's last
 // chunk waits, the turn before (item t - NB, at least NB chunks back) is over.
-// What a group writes before it has seen the scores (dQ's row sums, written at
-// an item's first chunk) has 2 NB turns: certain then are the scores of its
-// previous chunk, two before, so that item t - 2 NB is over.
+// D has 2 NB turns: it is formed when an item's tiles are there, so while the
+// scores of item t - 2 (two tiles) are complete, of which the last NB - 1
+// chunks may still be worked on: item t - 2 NB is over.
 namespace bw {
 constexpr int BC = 64;                 // chunk rows
 constexpr int CT = BC * 128;           // bytes of a chunk's 64-element sub-tile
 constexpr int G = 2;                   // groups of row warps
-constexpr int kThreads = 96 + 128 * G;
 }  // namespace bw
 
 // ------------------------------------------------------------ backward: dQ
 // Item = 128 packed rows of a unit, chunks of 64 keys: S = Q K^T, dP = dO V^T,
-// dQ += dS K.  The group with an item's first chunk forms D = rowsum(dO * O),
-// leaves it for the other groups and keeps it for the dK / dV kernel; the
-// group with the last chunk writes dQ.
+// dQ += dS K.  A warp of its own forms D = rowsum(dO * O) of the items ahead
+// of the groups, from tiles (O's rows read from global memory took a group
+// 3000 cycles per item), and keeps it for the dK / dV kernel; the group with
+// an item's last chunk writes dQ.
 namespace bq {
+constexpr int kThreads = 128 + 128 * bw::G;  // one more control warp, for D
 template <int DC>
 struct L {
   static constexpr int NB = 3;
-  static constexpr int kTiles = DC == 1 ? 2 : 1;            // Q, dO tiles
-  static constexpr int kN = DC == 1 ? 8 : 4;                // stages of DC K sub-tiles, DC V sub-tiles
-  static constexpr int TILES = 2 * DC * TILE;
+  static constexpr int kTiles = DC == 1 ? 2 : 1;            // Q, dO, O tiles
+  static constexpr int kN = DC == 1 ? 6 : 3;                // stages of DC K sub-tiles, DC V sub-tiles
+  static constexpr int TILES = 3 * DC * TILE;
   static constexpr int STAGE = 2 * DC * bw::CT;
   static constexpr int OFF_KV = kTiles * TILES;
   static constexpr int OFF_D = OFF_KV + kN * STAGE;         // [2 NB][128] -D, then [2 NB][128] -lse2
@@ -671,7 +682,6 @@ struct L {
 struct QueryCursor {
   int item, len, c, nch;
   Item it;
-  uint32_t n;  // chunks before this one
   bool live;
 
   __device__ __forceinline__ void seek(const Shape& sh, const Geometry& g) {  // from `item` on
@@ -680,21 +690,24 @@ struct QueryCursor {
       it = forward_item(item, g);
       len = sh.keys(it.b);
       nch = (len + bw::BC - 1) / bw::BC;
-      c = 0;
       if (nch > 0) {
         live = true;
         return;
       }
     }
   }
-  __device__ __forceinline__ QueryCursor(const Shape& sh, const Geometry& g) : item(blockIdx.x), n(0) { seek(sh, g); }
-  // to the next chunk; true when that begins another item (or ends the stream)
-  __device__ __forceinline__ bool next(const Shape& sh, const Geometry& g) {
-    ++n;
-    if (++c < nch) return false;
-    item += gridDim.x;
-    seek(sh, g);
-    return true;
+  __device__ __forceinline__ QueryCursor(const Shape& sh, const Geometry& g) : item(blockIdx.x), c(0) { seek(sh, g); }
+  // k chunks on; the number of items left behind
+  __device__ __forceinline__ int next(const Shape& sh, const Geometry& g, int k = 1) {
+    int items = 0;
+    c += k;
+    while (c >= nch && live) {
+      c -= nch;
+      item += gridDim.x;
+      seek(sh, g);
+      ++items;
+    }
+    return items;
   }
   __device__ __forceinline__ bool first() const { return c == 0; }
   __device__ __forceinline__ bool last() const { return c == nch - 1; }
@@ -702,11 +715,11 @@ struct QueryCursor {
 };
 
 template <typename T, int DC, bool DROP>
-__global__ void __launch_bounds__(bw::kThreads, 1)
+__global__ void __launch_bounds__(bq::kThreads, 1)
     xattn_bwd_dq(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
-                 const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                 const T* __restrict__ o, const float* __restrict__ lse, float* __restrict__ delta, T* __restrict__ dq,
-                 Plane po, Plane pdq, Shape sh, Geometry g, DropArgs drop) {
+                 const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmK,
+                 const __grid_constant__ CUtensorMap tmV, const float* __restrict__ lse, float* __restrict__ delta,
+                 T* __restrict__ dq, Plane pdq, Shape sh, Geometry g, DropArgs drop) {
   using namespace bw;
   using Y = bq::L<DC>;
   constexpr int NB = Y::NB;
@@ -732,7 +745,7 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < Y::kTiles; ++i) {
       umma::mbar_init(&qd_full[i], 1);
-      umma::mbar_init(&qd_empty[i], 1 + 4);  // the products' commit and the four warps that read dO
+      umma::mbar_init(&qd_empty[i], 2);  // the scores' commit and the warp that forms D
     }
     for (int i = 0; i < Y::kN; ++i) {
       umma::mbar_init(&kv_full[i], 1);
@@ -742,8 +755,8 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
       umma::mbar_init(&sd_full[i], 1);
       umma::mbar_init(&ds_full[i], 4);
       umma::mbar_init(&ds_done[i], 1);
-      umma::mbar_init(&d_full[i], 4);
-      umma::mbar_init(&d_full[NB + i], 4);
+      umma::mbar_init(&d_full[i], 1);
+      umma::mbar_init(&d_full[NB + i], 1);
       umma::mbar_init(&dq_full[i], 1);
     }
     umma::mbar_init(dq_empty, 4);
@@ -760,6 +773,7 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
     if (lane == 0) {  // tiles of an item before its first chunk
       umma::tma_prefetch(&tmQ);
       umma::tma_prefetch(&tmDO);
+      umma::tma_prefetch(&tmO);
       umma::tma_prefetch(&tmK);
       umma::tma_prefetch(&tmV);
       Ring<Y::kTiles> qd;
@@ -777,6 +791,7 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
           for (int dc = 0; dc < DC; ++dc) {
             umma::tma_load_5d(dst + dc * TILE, &tmQ, &qd_full[qd.s], dc * 64, 0, pos, cu.it.u, cu.it.b);
             umma::tma_load_5d(dst + (DC + dc) * TILE, &tmDO, &qd_full[qd.s], dc * 64, 0, pos, cu.it.u, cu.it.b);
+            umma::tma_load_5d(dst + (2 * DC + dc) * TILE, &tmO, &qd_full[qd.s], dc * 64, 0, pos, cu.it.u, cu.it.b);
           }
           qd.next();
         }
@@ -788,8 +803,8 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
         umma::mbar_arrive_expect_tx(&kv_full[kv.s], Y::STAGE);
 #pragma unroll
         for (int dc = 0; dc < DC; ++dc) {
-          umma::tma_load_4d(dst + dc * CT, &tmK, &kv_full[kv.s], dc * 64, cu.c * BC, cu.it.u / g.kv_units, cu.it.b);
-          umma::tma_load_4d(dst + (DC + dc) * CT, &tmV, &kv_full[kv.s], dc * 64, cu.c * BC, cu.it.u / g.kv_units,
+          umma::tma_load_4d(dst + dc * CT, &tmK, &kv_full[kv.s], dc * 64, cu.c * BC, g.by_kv_units.div(cu.it.u), cu.it.b);
+          umma::tma_load_4d(dst + (DC + dc) * CT, &tmV, &kv_full[kv.s], dc * 64, cu.c * BC, g.by_kv_units.div(cu.it.u),
                             cu.it.b);
         }
       }
@@ -846,8 +861,52 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
         odd ^= 1;
       }
     }
+  } else if (warp == 3) {  // D and the statistics of the items
+    Ring<Y::kTiles> qd;
+    Ring<2 * NB> turn;
+    for (QueryCursor cu(sh, g); cu.live && !abort_flag; cu.next(sh, g, cu.nch), qd.next(), turn.next()) {
+      const int rows = min(BM, g.rows - cu.it.blk * BM);
+      const int64_t stat = (int64_t)(cu.it.b * g.units + cu.it.u) * g.ldr + cu.it.blk * BM + lane;
+      float nlse[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) nlse[i] = lane + 32 * i < rows ? lse[stat + 32 * i] : 0.f;
+      if (!umma::mbar_wait(&qd_full[qd.s], qd.phase, 0xa8)) {
+        abort_flag = 1;
+        break;
+      }
+      const uint8_t* go = smem + qd.s * Y::TILES + DC * TILE;
+      float nd[4] = {0.f, 0.f, 0.f, 0.f};  // four rows at a time hide one another's latencies
+#pragma unroll 2
+      for (int c = 0; c < 8 * DC; ++c) {
+        uint4 o4[4], d4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t at = (c >> 3) * TILE + sw128(lane + 32 * i, c & 7);
+          d4[i] = *reinterpret_cast<const uint4*>(go + at);
+          o4[i] = *reinterpret_cast<const uint4*>(go + DC * TILE + at);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const T* oe = reinterpret_cast<const T*>(&o4[i]);
+          const T* de = reinterpret_cast<const T*>(&d4[i]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) nd[i] = fmaf(-Elem<T>::to_f(oe[e]), Elem<T>::to_f(de[e]), nd[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (lane + 32 * i < rows) delta[stat + 32 * i] = nd[i];
+        nd_s[turn.s * 128 + lane + 32 * i] = nd[i];
+        nl_s[turn.s * 128 + lane + 32 * i] = nlse[i];
+      }
+      __syncwarp();
+      if (lane == 0) {
+        umma::mbar_arrive(&d_full[turn.s]);
+        umma::mbar_arrive(&qd_empty[qd.s]);
+      }
+    }
   } else {
-    const int grp = (warp - 3) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const int grp = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const float sl2 = sh.scale * kLog2e, mult = DROP ? drop.scale : 1.f;
     const uint64_t sl22 = pk2(sl2, sl2), mult2 = pk2(mult, mult);
@@ -862,56 +921,46 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
         for (int d = 0; d < sh.dim; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
         delta[(int64_t)(it.b * g.units + it.u) * g.ldr + R] = 0.f;
       }
-    Ring<Y::kTiles> qd;
+    QueryCursor cu(sh, g);
     Ring<Y::kN> kv;
     Ring<NB> gr;     // accumulators of the cursor's chunk
     Ring<NB> turn;   // of the items
     Ring<2 * NB> dturn;
-    for (QueryCursor cu(sh, g); cu.live && !abort_flag;) {
-      if ((int)(cu.n % G) == grp) {
+    auto advance = [&](int k) {
+      kv.next(k);
+      gr.next(k);
+      for (int i = cu.next(sh, g, k); i > 0; --i) {
+        turn.next();
+        dturn.next();
+      }
+    };
+    if (grp == 1) advance(1);
+    int known = -1;  // item whose statistics these are
+    uint64_t nd2 = 0, nlse2 = 0;
+    for (; cu.live && !abort_flag; advance(G)) {
+      {
         const bool last = cu.last();
         const uint32_t acc = tmem + lane_off + gr.s * 128;
         const Item& it = cu.it;
         const int R = it.blk * BM + row, pos = R >> g.gp_shift, head = (it.u << g.gp_shift) + (R & gp_mask);
         const bool valid = R < g.rows, idle = it.blk * BM + quarter * 32 >= g.rows;
-        if (cu.first()) {  // D and the statistics of this item, for all groups
-          float nlse = 0.f, nd = 0.f;
-          uint4 orow[8 * DC];
-          const T* osrc = o + it.b * po.s_b + pos * po.s_n + head * po.s_h;
-#pragma unroll
-          for (int i = 0; i < 8 * DC; ++i)
-            orow[i] = valid && i * 8 < sh.dim ? *reinterpret_cast<const uint4*>(osrc + i * 8) : make_uint4(0, 0, 0, 0);
-          const int64_t stat = (int64_t)(it.b * g.units + it.u) * g.ldr + R;
-          if (valid) nlse = lse[stat];
-          if (!umma::mbar_wait(&qd_full[qd.s], qd.phase, 0xa8)) {
+        if (!umma::mbar_wait(&sd_full[gr.s], gr.phase, 0xaa)) {
+          abort_flag = 1;
+          break;
+        }
+        if (cu.item != known) {
+          if (!umma::mbar_wait(&d_full[dturn.s], dturn.phase, 0xa9)) {
             abort_flag = 1;
             break;
           }
-          const uint8_t* go = smem + qd.s * Y::TILES + DC * TILE;
-#pragma unroll
-          for (int i = 0; i < 8 * DC; ++i) {
-            const uint4 d4 = *reinterpret_cast<const uint4*>(go + (i >> 3) * TILE + sw128(row, i & 7));
-            const T* oe = reinterpret_cast<const T*>(&orow[i]);
-            const T* de = reinterpret_cast<const T*>(&d4);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) nd = fmaf(-Elem<T>::to_f(oe[e]), Elem<T>::to_f(de[e]), nd);
-          }
-          if (valid) delta[stat] = nd;
-          nd_s[dturn.s * 128 + row] = nd;
-          nl_s[dturn.s * 128 + row] = nlse;
-          warp_arrive(&qd_empty[qd.s], false);
-          __syncwarp();
-          if (lane == 0) umma::mbar_arrive(&d_full[dturn.s]);
-        }
-        if (!umma::mbar_wait(&sd_full[gr.s], gr.phase, 0xaa) || !umma::mbar_wait(&d_full[dturn.s], dturn.phase, 0xa9)) {
-          abort_flag = 1;
-          break;
+          known = cu.item;
+          const float nd = nd_s[dturn.s * 128 + row], nlse = nl_s[dturn.s * 128 + row];
+          nd2 = pk2(nd, nd);
+          nlse2 = pk2(nlse, nlse);
         }
         umma::tc_fence_after();
         const int keys = cu.keys();
         if (!idle) {
-          const float nd = nd_s[dturn.s * 128 + row], nlse = nl_s[dturn.s * 128 + row];
-          const uint64_t nd2 = pk2(nd, nd), nlse2 = pk2(nlse, nlse);
           const uint32_t bh = (uint32_t)(it.b * sh.heads + head);
 #pragma unroll 1
           for (int first = 0; first < keys; first += 32) {
@@ -970,13 +1019,6 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
           warp_arrive(dq_empty, false);
         }
       }
-      kv.next();
-      gr.next();
-      if (cu.next(sh, g)) {
-        qd.next();
-        turn.next();
-        dturn.next();
-      }
     }
   }
   umma::tc_fence_before();
@@ -995,6 +1037,7 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
 // lanes: each lane draws the groups of four of 32 columns and the eight
 // exchange the keep bits by shuffles, so a group is still drawn once.
 namespace bk {
+constexpr int kThreads = 96 + 128 * bw::G;
 template <int DC>
 struct L {
   static constexpr int NB = DC == 1 ? 3 : 2;                // 512 columns: 128 NB + dV + dK
@@ -1012,56 +1055,53 @@ struct L {
 
 // One chunk of the stream of a CTA: key blocks with keys, in order, unit by unit, chunk by chunk.
 struct KeyCursor {
-  int item, blk, kh, b, len, u, u_end, r0;
-  uint32_t n;  // chunks before this one
-  bool live, begins;
+  int item, blk, kh, b, len, u, u0, u_end, r0, span;  // span: the chunks' rows of a unit
+  bool live;
 
-  __device__ __forceinline__ void at(const Shape& sh, int kblk) {
-    blk = item % kblk;
-    const int r = item / kblk;
-    kh = r % sh.kv_heads;
-    b = r / sh.kv_heads;
+  __device__ __forceinline__ void at(const Shape& sh, const Geometry& g) {
+    b = g.by_kv_heads.split(g.by_kblk.split(item, blk), kh);
     len = sh.keys(b);
   }
-  __device__ __forceinline__ void seek(const Shape& sh, const Geometry& g, int kblk) {  // from `item` on
+  __device__ __forceinline__ void seek(const Shape& sh, const Geometry& g) {  // from `item` on
     live = false;
     for (; item < g.total; item += gridDim.x) {
-      at(sh, kblk);
-      u = kh * g.kv_units;
+      at(sh, g);
+      u = u0 = kh * g.kv_units;
       u_end = u + g.kv_units;
-      r0 = 0;
-      begins = true;
       if (blk * BM < len) {
         live = true;
         return;
       }
     }
   }
-  __device__ __forceinline__ KeyCursor(const Shape& sh, const Geometry& g, int kblk) : item(blockIdx.x), n(0) {
-    seek(sh, g, kblk);
+  __device__ __forceinline__ KeyCursor(const Shape& sh, const Geometry& g)
+      : item(blockIdx.x), r0(0), span((g.rows + bw::BC - 1) / bw::BC * bw::BC) {
+    seek(sh, g);
   }
-  // to the next chunk; true when that begins another item (or ends the stream)
-  __device__ __forceinline__ bool next(const Shape& sh, const Geometry& g, int kblk) {
-    ++n;
-    begins = false;
-    r0 += bw::BC;
-    if (r0 < g.rows) return false;
-    r0 = 0;
-    if (++u < u_end) return false;
-    item += gridDim.x;
-    seek(sh, g, kblk);
-    return true;
+  // k chunks on; the number of items left behind
+  __device__ __forceinline__ int next(const Shape& sh, const Geometry& g, int k = 1) {
+    int items = 0;
+    r0 += k * bw::BC;
+    while (r0 >= span && live) {
+      r0 -= span;
+      if (++u == u_end) {
+        item += gridDim.x;
+        seek(sh, g);
+        ++items;
+      }
+    }
+    return items;
   }
-  __device__ __forceinline__ bool first() const { return begins; }
-  __device__ __forceinline__ bool last(const Geometry& g) const { return r0 + bw::BC >= g.rows && u + 1 == u_end; }
+  __device__ __forceinline__ bool first() const { return r0 == 0 && u == u0; }
+  __device__ __forceinline__ bool last() const { return r0 + bw::BC == span && u + 1 == u_end; }
 };
 
 template <typename T, int DC, bool DROP>
-__global__ void __launch_bounds__(bw::kThreads, 1)
+__global__ void __launch_bounds__(bk::kThreads, 1)
     xattn_bwd_dkdv(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
                    const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk,
-                   T* __restrict__ dv, Plane pdk, Plane pdv, Shape sh, Geometry g, int kblk, DropArgs drop) {
+                   T* __restrict__ dv, Plane pdk, Plane pdv, Shape sh, Geometry g, DropArgs drop) {
   using namespace bw;
   using Y = bk::L<DC>;
   constexpr int NB = Y::NB;
@@ -1114,7 +1154,7 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
       umma::tma_prefetch(&tmDO);
       Ring<Y::kTiles> kv;
       Ring<Y::kN> ch;
-      for (KeyCursor cu(sh, g, kblk); cu.live && !abort_flag; cu.next(sh, g, kblk), ch.next()) {
+      for (KeyCursor cu(sh, g); cu.live && !abort_flag; cu.next(sh, g), ch.next()) {
         if (cu.first()) {
           if (!umma::mbar_wait(&kv_empty[kv.s], kv.phase ^ 1, 0xb1)) {
             abort_flag = 1;
@@ -1150,7 +1190,7 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
     Ring<Y::kTiles> kv;
     Ring<Y::kN> ch;
     Ring<NB> gr;
-    for (KeyCursor cu(sh, g, kblk); cu.live && !abort_flag;) {
+    for (KeyCursor cu(sh, g); cu.live && !abort_flag;) {
       if ((cu.first() && !umma::mbar_wait(&kv_full[kv.s], kv.phase, 0xb3)) ||
           !umma::mbar_wait(&ch_full[ch.s], ch.phase, 0xb4) || !umma::mbar_wait(&ps_done[gr.s], gr.phase ^ 1, 0xb5)) {
         abort_flag = 1;
@@ -1163,19 +1203,19 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
         mma_scores<DC>(acc, k, TILE, q, CT, idesc);
         mma_scores<DC>(acc + 64, k + DC * TILE / 16, TILE, q + DC * CT / 16, CT, idesc);
         umma::mma_commit(&sd_full[gr.s]);
-        if (cu.last(g)) umma::mma_commit(&kv_empty[kv.s]);
+        if (cu.last()) umma::mma_commit(&kv_empty[kv.s]);
       }
       __syncwarp();
       ch.next();
       gr.next();
-      if (cu.next(sh, g, kblk)) kv.next();
+      if (cu.next(sh, g)) kv.next();
     }
   } else if (warp == 2) {  // products
     const bool leader = umma::elect_one();
     Ring<Y::kN> ch;
     Ring<NB> gr, turn;
     uint32_t odd = 0;  // items so far, modulo 2
-    for (KeyCursor cu(sh, g, kblk); cu.live && !abort_flag;) {
+    for (KeyCursor cu(sh, g); cu.live && !abort_flag;) {
       const bool first = cu.first();
       if (!umma::mbar_wait(&ps_full[gr.s], gr.phase, 0xb6) || (first && !umma::mbar_wait(acc_empty, odd ^ 1, 0xb7))) {
         abort_flag = 1;
@@ -1188,14 +1228,14 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
       if (leader) {
         mma_rows_ts<DC>(tmem + Y::kTmemDV, acc, q + DC * CT / 16, CT, Desc<T>::MN, ksteps, !first);
         mma_rows_ts<DC>(tmem + Y::kTmemDK, acc + 64, q, CT, Desc<T>::MN, ksteps, !first);
-        if (cu.last(g)) umma::mma_commit(&acc_full[turn.s]);
+        if (cu.last()) umma::mma_commit(&acc_full[turn.s]);
         umma::mma_commit(&ps_done[gr.s]);
         umma::mma_commit(&ch_empty[ch.s]);
       }
       __syncwarp();
       ch.next();
       gr.next();
-      if (cu.next(sh, g, kblk)) {
+      if (cu.next(sh, g)) {
         turn.next();
         odd ^= 1;
       }
@@ -1217,18 +1257,25 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
     };
     // keys at or behind the length: zeros
     if (grp == 0 && sh.lengths != nullptr) {
-      KeyCursor c(sh, g, kblk);
+      KeyCursor c(sh, g);
       for (c.item = blockIdx.x; c.item < g.total; c.item += gridDim.x) {
-        c.at(sh, kblk);
+        c.at(sh, g);
         if (c.blk * BM + row >= c.len && c.blk * BM + row < sh.nk) zeros(c);
       }
     }
+    KeyCursor cu(sh, g);
     Ring<Y::kN> ch;
     Ring<NB> gr;     // accumulators of the cursor's chunk
     Ring<NB> turn;   // of the items
-    for (KeyCursor cu(sh, g, kblk); cu.live && !abort_flag;) {
-      if ((int)(cu.n % G) == grp) {
-        const bool last = cu.last(g);
+    auto advance = [&](int k) {
+      ch.next(k);
+      gr.next(k);
+      for (int i = cu.next(sh, g, k); i > 0; --i) turn.next();
+    };
+    if (grp == 1) advance(1);
+    for (; cu.live && !abort_flag; advance(G)) {
+      {
+        const bool last = cu.last();
         const uint32_t acc = tmem + lane_off + gr.s * 128;
         const int j = cu.blk * BM + row, rows = min(BC, g.rows - cu.r0);
         const bool live = j < cu.len, idle = cu.blk * BM + quarter * 32 >= cu.len;
@@ -1323,9 +1370,6 @@ __global__ void __launch_bounds__(bw::kThreads, 1)
           warp_arrive(acc_empty, false);
         }
       }
-      ch.next();
-      gr.next();
-      if (cu.next(sh, g, kblk)) turn.next();
     }
   }
   umma::tc_fence_before();
@@ -1361,6 +1405,12 @@ int split_count(int64_t items, int nch, int64_t elements) {
   return best;
 }
 
+Divisor divisor(int64_t d) {
+  uint32_t s = 0;
+  while (((int64_t)1 << s) < d) ++s;
+  return Divisor{(uint32_t)((((uint64_t)1 << (31 + s)) + (uint64_t)d - 1) / (uint64_t)d), 31 + s, (uint32_t)d};
+}
+
 // Rows and tiles of a shape; `splits` from the tile count alone, so that the
 // workspace size, the forward and its join agree.
 Geometry geometry(const Shape& sh) {
@@ -1376,7 +1426,15 @@ Geometry geometry(const Shape& sh) {
   const int nch = (sh.nk + fw::kMaxW - 1) / fw::kMaxW;
   g.width = (int)round_up((sh.nk + nch - 1) / nch, 16);
   g.splits = split_count((int64_t)sh.batch * g.units * g.nblk, nch, (int64_t)sh.batch * g.units * g.rows * sh.dim);
+  while ((int64_t)nch * g.splits >= ((int64_t)1 << 30)) --g.splits;
   g.total = 0;
+  g.by_nblk = divisor(g.nblk);
+  g.by_splits = divisor(g.splits);
+  g.by_units = divisor(g.units);
+  g.by_width = divisor(g.width);
+  g.by_kv_units = divisor(g.kv_units);
+  g.by_kblk = divisor((sh.nk + BM - 1) / BM);
+  g.by_kv_heads = divisor(sh.kv_heads);
   return g;
 }
 
@@ -1451,9 +1509,10 @@ int forward_launch(const Shape& sh, const Forward& a, Geometry g, const char* na
 
 template <typename T, int DC, bool DROP>
 int backward_launch(const Shape& sh, const Backward& a, Geometry g, const char* name) {
-  CUtensorMap q128, do128, q64, do64, k64, v64, k128, v128;
+  CUtensorMap q128, do128, o128, q64, do64, k64, v64, k128, v128;
   if (int st = query_map(q128, a.q, a.pq, sh, g, a.dtype, BM, name)) return st;
   if (int st = query_map(do128, a.go, a.pgo, sh, g, a.dtype, BM, name)) return st;
+  if (int st = query_map(o128, a.o, a.po, sh, g, a.dtype, BM, name)) return st;
   if (int st = query_map(q64, a.q, a.pq, sh, g, a.dtype, bw::BC, name)) return st;
   if (int st = query_map(do64, a.go, a.pgo, sh, g, a.dtype, bw::BC, name)) return st;
   if (int st = key_map(k64, a.k, a.pk, sh, a.dtype, bw::BC, name)) return st;
@@ -1465,9 +1524,8 @@ int backward_launch(const Shape& sh, const Backward& a, Geometry g, const char* 
     auto kernel = xattn_bwd_dq<T, DC, DROP>;
     constexpr int smem = bq::L<DC>::SMEM;
     PMB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), name);
-    kernel<<<persistent_grid(g.total, 1), bw::kThreads, smem, a.stream>>>(
-        q128, do128, k64, v64, static_cast<const T*>(a.o), a.lse, delta, static_cast<T*>(a.gq), a.po, a.pgq, sh, g,
-        a.drop);
+    kernel<<<persistent_grid(g.total, 1), bq::kThreads, smem, a.stream>>>(
+        q128, do128, o128, k64, v64, a.lse, delta, static_cast<T*>(a.gq), a.pgq, sh, g, a.drop);
     PMB_CHECK_LAUNCH(name);
   }
   const int kblk = (sh.nk + BM - 1) / BM;
@@ -1477,9 +1535,8 @@ int backward_launch(const Shape& sh, const Backward& a, Geometry g, const char* 
   auto kernel = xattn_bwd_dkdv<T, DC, DROP>;
   constexpr int smem = bk::L<DC>::SMEM;
   PMB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), name);
-  kernel<<<persistent_grid(items, 1), bw::kThreads, smem, a.stream>>>(
-      k128, v128, q64, do64, a.lse, delta, static_cast<T*>(a.gk), static_cast<T*>(a.gv), a.pgk, a.pgv, sh, g, kblk,
-      a.drop);
+  kernel<<<persistent_grid(items, 1), bk::kThreads, smem, a.stream>>>(
+      k128, v128, q64, do64, a.lse, delta, static_cast<T*>(a.gk), static_cast<T*>(a.gv), a.pgk, a.pgv, sh, g, a.drop);
   PMB_CHECK_LAUNCH(name);
   return PMB_OK;
 }
@@ -1538,6 +1595,7 @@ int tc_forward(const Shape& sh, const Forward& a, const char* name) {
 int tc_backward(const Shape& sh, const Backward& a, const char* name) {
   Geometry g = geometry(sh);
   g.splits = 1;
+  g.by_splits = divisor(1);
   if (int st = count_items(sh, g, name)) return st;
   const Plane planes[8] = {a.pq, a.pk, a.pv, a.po, a.pgo, a.pgq, a.pgk, a.pgv};
   const void* ptrs[8] = {a.q, a.k, a.v, a.o, a.go, a.gq, a.gk, a.gv};
