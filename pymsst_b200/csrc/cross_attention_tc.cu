@@ -1007,16 +1007,20 @@ __global__ void __launch_bounds__(bq::kThreads, 1)
           }
           umma::tc_fence_after();
           T* dst = dq + it.b * pdq.s_b + pos * pdq.s_n + head * pdq.s_h;
-#pragma unroll 1
-          for (int k = 0; k < 2 * DC; ++k) {
-            if (idle || k * 32 >= sh.dim) break;
-            uint32_t a[32];
-            tmem_ld32_nowait(tmem + lane_off + Y::kTmemDQ + k * 32, a);
-            wait_ld();
-            tie32(a);
-            if (valid) store_row<T>(dst, k * 32, sh.dim, a, sh.scale);
+#pragma unroll
+          for (int dc = 0; dc < DC; ++dc) {  // 64 columns read at once, the last before the stores
+            uint32_t a0[32], a1[32];
+            if (!idle) {
+              tmem_ld32_nowait(tmem + lane_off + Y::kTmemDQ + dc * 64, a0);
+              tmem_ld32_nowait(tmem + lane_off + Y::kTmemDQ + dc * 64 + 32, a1);
+              tmem_wait2(a0, a1);
+            }
+            if (dc == DC - 1) warp_arrive(dq_empty, false);
+            if (valid) {
+              store_row<T>(dst, dc * 64, sh.dim, a0, sh.scale);
+              store_row<T>(dst, dc * 64 + 32, sh.dim, a1, sh.scale);
+            }
           }
-          warp_arrive(dq_empty, false);
         }
       }
     }
