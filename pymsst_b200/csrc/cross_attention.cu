@@ -10,10 +10,16 @@
 // O = 0, lse = -inf and no gradient; keys at or behind `len` are never read,
 // and their gradients are zeros.
 //
-// The C entries, and the row form: one warp per query row (forward, dQ) or
-// key row (dK / dV), all arithmetic fp32; every output row is written by one
-// warp, so results do not depend on the order of execution.  It serves fp32
-// and head dims the tensor-core form (cross_attention_tc.cu) does not take.
+// The C entries, and the row form, all arithmetic fp32: it serves fp32 and
+// head dims the tensor-core form (cross_attention_tc.cu) does not take.  A
+// warp owns eight rows (queries in the forward and for dQ, keys for dK / dV);
+// tiles of 32 rows of the other side come through shared memory for the four
+// warps of a CTA.  For the dot products a lane takes one row of the tile and
+// multiplies it with the eight owned rows, which all lanes read alike; for the
+// sums a lane takes every 32nd head element.  Bound by shared-memory reads
+// (9 of 16 bytes for 32 fused multiply-adds).  Every output row is summed by
+// one warp in the order of the tiles, so results do not depend on the order of
+// execution.
 #include "cross_attention.cuh"
 
 namespace pmb {
@@ -24,182 +30,278 @@ using xattn::Shape;
 
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
+constexpr int kOwn = 8;                 // rows of a warp
+constexpr int kTile = 32;               // streamed rows
+constexpr int kRows = kWarps * kOwn;    // owned rows of a CTA
 constexpr int kMaxDim = 256;
-constexpr int kAcc = kMaxDim / 32;
 
-// sum_c a[c] * row[c] with a in shared memory
+__host__ __device__ inline int pitch_of(int dim) { return (dim + 3) / 4 * 4 + 4; }  // floats; rows start 16-byte aligned
+__host__ __device__ inline int own_pitch_of(int dim) { return (dim + 3) / 4 * 4; }
+
+// Shared memory: two streamed tiles, two owned row sets, the warps' weights [2][32][8].
+inline int shared_bytes(int dim) {
+  return (2 * kTile * pitch_of(dim) + 2 * kRows * own_pitch_of(dim) + kWarps * 2 * kTile * kOwn) * 4;
+}
+
+struct Shared {
+  float *ta, *tb, *oa, *ob, *w;
+  __device__ __forceinline__ Shared(float* base, int dim) {
+    ta = base;
+    tb = ta + kTile * pitch_of(dim);
+    oa = tb + kTile * pitch_of(dim);
+    ob = oa + kRows * own_pitch_of(dim);
+    w = ob + kRows * own_pitch_of(dim);
+  }
+};
+
+// `count` rows (the rest of `rows`, and the row's padding, zeros) of a plane, times mul, into shared memory.
 template <typename T>
-__device__ __forceinline__ float dot(const float* a, const T* __restrict__ row, int dim) {
-  float s = 0.f;
-  for (int c = 0; c < dim; ++c) s = fmaf(a[c], Elem<T>::to_f(row[c]), s);
-  return s;
+__device__ __forceinline__ void stage(float* dst, int pitch, const T* __restrict__ src, int64_t s_n, int count,
+                                      int rows, int dim, float mul) {
+  const int width = own_pitch_of(dim);
+  for (int i = threadIdx.x; i < rows * width; i += kThreads) {
+    const int r = i / width, c = i - r * width;
+    dst[r * pitch + c] = r < count && c < dim ? Elem<T>::to_f(src[r * s_n + c]) * mul : 0.f;
+  }
+}
+
+// s[i] = sum_c own[i][c] tile[lane][c]
+__device__ __forceinline__ void dots(float (&s)[kOwn], const float* own, int own_pitch, const float* tile, int pitch,
+                                     int dim) {
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) s[i] = 0.f;
+  const float* mine = tile + (threadIdx.x & 31) * pitch;
+  for (int c = 0; c < dim; c += 4) {
+    const float4 x = *reinterpret_cast<const float4*>(mine + c);
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const float4 y = *reinterpret_cast<const float4*>(own + i * own_pitch + c);
+      s[i] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s[i]))));
+    }
+  }
+}
+
+// acc[i][a] += sum_t w[t][i] tile[t][lane + 32 a]
+template <int NA>
+__device__ __forceinline__ void sums(float (&acc)[kOwn][NA], const float* w, const float* tile, int pitch, int dim,
+                                     int count) {
+  const int lane = threadIdx.x & 31;
+  for (int t = 0; t < count; ++t) {
+    const float4 p0 = *reinterpret_cast<const float4*>(w + t * kOwn);
+    const float4 p1 = *reinterpret_cast<const float4*>(w + t * kOwn + 4);
+    const float p[kOwn] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
+#pragma unroll
+    for (int a = 0; a < NA; ++a) {
+      const float x = lane + 32 * a < dim ? tile[t * pitch + lane + 32 * a] : 0.f;
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) acc[i][a] = fmaf(p[i], x, acc[i][a]);
+    }
+  }
+}
+
+// the lane's eight weights, one row of [32][8]
+__device__ __forceinline__ void put_weights(float* w, const float (&p)[kOwn]) {
+  float* mine = w + (threadIdx.x & 31) * kOwn;
+  *reinterpret_cast<float4*>(mine) = make_float4(p[0], p[1], p[2], p[3]);
+  *reinterpret_cast<float4*>(mine + 4) = make_float4(p[4], p[5], p[6], p[7]);
 }
 
 // 16-bit number of (key, query, batch head) against the drop limit
-__device__ __forceinline__ bool kept(const Philox& rng, uint32_t limit, int key, int query, int bh) {
+__device__ __forceinline__ bool kept_key(const Philox& rng, uint32_t limit, int key, int query, int bh) {
   return (keep_bits(rng((uint32_t)key >> 3, (uint32_t)query, (uint32_t)bh), limit) >> (key & 7)) & 1u;
 }
 
-template <typename T, bool DROP>
+// Grid: (tiles of kRows queries) x batch x heads.
+template <typename T, bool DROP, int NA>
 __global__ void __launch_bounds__(kThreads)
     attn_rows_fwd(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ o,
-                  float* __restrict__ lse, Plane pq, Plane pk, Plane pv, Plane po, Shape sh, DropArgs drop) {
-  __shared__ float qs[kWarps][kMaxDim];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * kWarps + warp;
-  if (row >= (int64_t)sh.batch * sh.heads * sh.nq) return;
-  const int i = (int)(row % sh.nq), bh = (int)(row / sh.nq), h = bh % sh.heads, b = bh / sh.heads;
+                  float* __restrict__ lse, Plane pq, Plane pk, Plane pv, Plane po, Shape sh, int blocks,
+                  DropArgs drop) {
+  extern __shared__ float4 smem4[];
+  const Shared m_(reinterpret_cast<float*>(smem4), sh.dim);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pitch = pitch_of(sh.dim), own = own_pitch_of(sh.dim);
+  const int bh = blockIdx.x / blocks, i0 = (blockIdx.x - bh * blocks) * kRows, h = bh % sh.heads, b = bh / sh.heads;
   const int kh = h / (sh.heads / sh.kv_heads), len = sh.keys(b);
   const Philox rng(DROP ? drop : DropArgs{});
-  const T* qr = q + b * pq.s_b + i * pq.s_n + h * pq.s_h;
-  for (int c = lane; c < sh.dim; c += 32) qs[warp][c] = Elem<T>::to_f(qr[c]) * sh.scale;
-  __syncwarp();
+  stage(m_.oa, own, q + b * pq.s_b + i0 * pq.s_n + h * pq.s_h, pq.s_n, sh.nq - i0, kRows, sh.dim, sh.scale);
   k += b * pk.s_b + kh * pk.s_h;
   v += b * pv.s_b + kh * pv.s_h;
-  float m = -INFINITY, l = 0.f, acc[kAcc] = {};
-  for (int j0 = 0; j0 < len; j0 += 32) {
-    const int j = j0 + lane;
-    const float s = j < len ? dot(qs[warp], k + j * pk.s_n, sh.dim) : -INFINITY;
-    float mx = s;
+  float m[kOwn], l[kOwn], acc[kOwn][NA] = {};
 #pragma unroll
-    for (int w = 16; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
-    const float mn = fmaxf(m, mx), corr = expf(m - mn);
-    float p = j < len ? expf(s - mn) : 0.f;
-    l = l * corr + warp_sum(p);
-    m = mn;
-    if (DROP && j < len) p = kept(rng, drop.limit, j, i, bh) ? p * drop.scale : 0.f;
-#pragma unroll
-    for (int a = 0; a < kAcc; ++a) acc[a] *= corr;
-    const int n = len - j0 < 32 ? len - j0 : 32;
-    for (int t = 0; t < n; ++t) {
-      const float pt = __shfl_sync(0xffffffffu, p, t);
-      const T* vr = v + (j0 + t) * pv.s_n;
-#pragma unroll
-      for (int a = 0; a < kAcc; ++a)
-        if (lane + 32 * a < sh.dim) acc[a] = fmaf(pt, Elem<T>::to_f(vr[lane + 32 * a]), acc[a]);
-    }
+  for (int i = 0; i < kOwn; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
   }
-  T* out = o + b * po.s_b + i * po.s_n + h * po.s_h;
-  const float inv = len > 0 ? 1.f / l : 0.f;
+  float* w = m_.w + warp * 2 * kTile * kOwn;
+  for (int j0 = 0; j0 < len; j0 += kTile) {
+    const int count = len - j0 < kTile ? len - j0 : kTile, j = j0 + lane;
+    __syncthreads();
+    stage(m_.ta, pitch, k + j0 * pk.s_n, pk.s_n, count, kTile, sh.dim, 1.f);
+    stage(m_.tb, pitch, v + j0 * pv.s_n, pv.s_n, count, kTile, sh.dim, 1.f);
+    __syncthreads();
+    float p[kOwn];
+    dots(p, m_.oa + warp * kOwn * own, own, m_.ta, pitch, sh.dim);
 #pragma unroll
-  for (int a = 0; a < kAcc; ++a)
-    if (lane + 32 * a < sh.dim) out[lane + 32 * a] = Elem<T>::from_f(acc[a] * inv);
-  if (lane == 0) lse[row] = len > 0 ? m + logf(l) : -INFINITY;
+    for (int i = 0; i < kOwn; ++i) {
+      float mx = lane < count ? p[i] : -INFINITY;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      const float mn = fmaxf(m[i], mx), corr = expf(m[i] - mn);
+      p[i] = lane < count ? expf(p[i] - mn) : 0.f;
+      l[i] = l[i] * corr + warp_sum(p[i]);
+      m[i] = mn;
+#pragma unroll
+      for (int a = 0; a < NA; ++a) acc[i][a] *= corr;
+      if (DROP && lane < count)
+        p[i] = kept_key(rng, drop.limit, j, i0 + warp * kOwn + i, bh) ? p[i] * drop.scale : 0.f;
+    }
+    put_weights(w, p);
+    __syncwarp();
+    sums<NA>(acc, w, m_.tb, pitch, sh.dim, count);
+    __syncwarp();
+  }
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    const int r = i0 + warp * kOwn + i;
+    if (r >= sh.nq) break;
+    T* out = o + b * po.s_b + r * po.s_n + h * po.s_h;
+    const float inv = len > 0 ? 1.f / l[i] : 0.f;
+#pragma unroll
+    for (int a = 0; a < NA; ++a)
+      if (lane + 32 * a < sh.dim) out[lane + 32 * a] = Elem<T>::from_f(acc[i][a] * inv);
+    if (lane == 0) lse[(int64_t)bh * sh.nq + r] = len > 0 ? m[i] + logf(l[i]) : -INFINITY;
+  }
 }
 
-template <typename T, bool DROP>
+template <typename T, bool DROP, int NA>
 __global__ void __launch_bounds__(kThreads)
     attn_rows_dq(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ o,
                  const T* __restrict__ go, const float* __restrict__ lse, T* __restrict__ gq,
                  float* __restrict__ delta, Plane pq, Plane pk, Plane pv, Plane po, Plane pgo, Plane pgq, Shape sh,
-                 DropArgs drop) {
-  __shared__ float qs[kWarps][kMaxDim], gs[kWarps][kMaxDim];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * kWarps + warp;
-  if (row >= (int64_t)sh.batch * sh.heads * sh.nq) return;
-  const int i = (int)(row % sh.nq), bh = (int)(row / sh.nq), h = bh % sh.heads, b = bh / sh.heads;
+                 int blocks, DropArgs drop) {
+  extern __shared__ float4 smem4[];
+  const Shared m_(reinterpret_cast<float*>(smem4), sh.dim);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pitch = pitch_of(sh.dim), own = own_pitch_of(sh.dim);
+  const int bh = blockIdx.x / blocks, i0 = (blockIdx.x - bh * blocks) * kRows, h = bh % sh.heads, b = bh / sh.heads;
   const int kh = h / (sh.heads / sh.kv_heads), len = sh.keys(b);
   const Philox rng(DROP ? drop : DropArgs{});
-  const T* qr = q + b * pq.s_b + i * pq.s_n + h * pq.s_h;
-  const T* gr = go + b * pgo.s_b + i * pgo.s_n + h * pgo.s_h;
-  const T* orow = o + b * po.s_b + i * po.s_n + h * po.s_h;
-  float d = 0.f;
-  for (int c = lane; c < sh.dim; c += 32) {
-    qs[warp][c] = Elem<T>::to_f(qr[c]) * sh.scale;
-    gs[warp][c] = Elem<T>::to_f(gr[c]);
-    d = fmaf(gs[warp][c], Elem<T>::to_f(orow[c]), d);
+  stage(m_.oa, own, q + b * pq.s_b + i0 * pq.s_n + h * pq.s_h, pq.s_n, sh.nq - i0, kRows, sh.dim, sh.scale);
+  stage(m_.ob, own, go + b * pgo.s_b + i0 * pgo.s_n + h * pgo.s_h, pgo.s_n, sh.nq - i0, kRows, sh.dim, 1.f);
+  __syncthreads();
+  float d[kOwn], ls[kOwn];
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    const int r = i0 + warp * kOwn + i;
+    float x = 0.f;
+    if (r < sh.nq) {
+      const T* orow = o + b * po.s_b + r * po.s_n + h * po.s_h;
+      for (int c = lane; c < sh.dim; c += 32)
+        x = fmaf(m_.ob[(warp * kOwn + i) * own + c], Elem<T>::to_f(orow[c]), x);
+    }
+    d[i] = warp_sum(x);
+    ls[i] = r < sh.nq ? lse[(int64_t)bh * sh.nq + r] : 0.f;
+    if (r < sh.nq && lane == 0) delta[(int64_t)bh * sh.nq + r] = d[i];
   }
-  d = warp_sum(d);
-  if (lane == 0) delta[row] = d;
-  __syncwarp();
   k += b * pk.s_b + kh * pk.s_h;
   v += b * pv.s_b + kh * pv.s_h;
-  const float ls = lse[row];
-  float acc[kAcc] = {};
-  for (int j0 = 0; j0 < len; j0 += 32) {
-    const int j = j0 + lane;
-    float ds = 0.f;
-    if (j < len) {
-      float dp = dot(gs[warp], v + j * pv.s_n, sh.dim);
-      if (DROP) dp = kept(rng, drop.limit, j, i, bh) ? dp * drop.scale : 0.f;
-      ds = expf(dot(qs[warp], k + j * pk.s_n, sh.dim) - ls) * (dp - d);
-    }
-    const int n = len - j0 < 32 ? len - j0 : 32;
-    for (int t = 0; t < n; ++t) {
-      const float dt = __shfl_sync(0xffffffffu, ds, t);
-      const T* kr = k + (j0 + t) * pk.s_n;
+  float acc[kOwn][NA] = {};
+  float* w = m_.w + warp * 2 * kTile * kOwn;
+  for (int j0 = 0; j0 < len; j0 += kTile) {
+    const int count = len - j0 < kTile ? len - j0 : kTile, j = j0 + lane;
+    __syncthreads();
+    stage(m_.ta, pitch, k + j0 * pk.s_n, pk.s_n, count, kTile, sh.dim, 1.f);
+    stage(m_.tb, pitch, v + j0 * pv.s_n, pv.s_n, count, kTile, sh.dim, 1.f);
+    __syncthreads();
+    float p[kOwn], dp[kOwn];
+    dots(p, m_.oa + warp * kOwn * own, own, m_.ta, pitch, sh.dim);
+    dots(dp, m_.ob + warp * kOwn * own, own, m_.tb, pitch, sh.dim);
 #pragma unroll
-      for (int a = 0; a < kAcc; ++a)
-        if (lane + 32 * a < sh.dim) acc[a] = fmaf(dt, Elem<T>::to_f(kr[lane + 32 * a]), acc[a]);
+    for (int i = 0; i < kOwn; ++i) {
+      if (DROP && lane < count)
+        dp[i] = kept_key(rng, drop.limit, j, i0 + warp * kOwn + i, bh) ? dp[i] * drop.scale : 0.f;
+      p[i] = lane < count ? expf(p[i] - ls[i]) * (dp[i] - d[i]) : 0.f;
     }
+    put_weights(w, p);
+    __syncwarp();
+    sums<NA>(acc, w, m_.ta, pitch, sh.dim, count);
+    __syncwarp();
   }
-  T* out = gq + b * pgq.s_b + i * pgq.s_n + h * pgq.s_h;
 #pragma unroll
-  for (int a = 0; a < kAcc; ++a)
-    if (lane + 32 * a < sh.dim) out[lane + 32 * a] = Elem<T>::from_f(acc[a] * sh.scale);
+  for (int i = 0; i < kOwn; ++i) {
+    const int r = i0 + warp * kOwn + i;
+    if (r >= sh.nq) break;
+    T* out = gq + b * pgq.s_b + r * pgq.s_n + h * pgq.s_h;
+#pragma unroll
+    for (int a = 0; a < NA; ++a)
+      if (lane + 32 * a < sh.dim) out[lane + 32 * a] = Elem<T>::from_f(acc[i][a] * sh.scale);
+  }
 }
 
-template <typename T, bool DROP>
+// Grid: (tiles of kRows keys) x batch x key / value heads.
+template <typename T, bool DROP, int NA>
 __global__ void __launch_bounds__(kThreads)
     attn_rows_dkdv(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ go,
                    const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ gk,
                    T* __restrict__ gv, Plane pq, Plane pk, Plane pv, Plane pgo, Plane pgk, Plane pgv, Shape sh,
-                   DropArgs drop) {
-  __shared__ float ks[kWarps][kMaxDim], vs[kWarps][kMaxDim];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * kWarps + warp;
-  if (row >= (int64_t)sh.batch * sh.kv_heads * sh.nk) return;
-  const int j = (int)(row % sh.nk), bk = (int)(row / sh.nk), kh = bk % sh.kv_heads, b = bk / sh.kv_heads;
-  const int group = sh.heads / sh.kv_heads;
+                   int blocks, DropArgs drop) {
+  extern __shared__ float4 smem4[];
+  const Shared m_(reinterpret_cast<float*>(smem4), sh.dim);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pitch = pitch_of(sh.dim), own = own_pitch_of(sh.dim);
+  const int bk = blockIdx.x / blocks, j0 = (blockIdx.x - bk * blocks) * kRows, kh = bk % sh.kv_heads, b = bk / sh.kv_heads;
+  const int group = sh.heads / sh.kv_heads, len = sh.keys(b), live = len - j0 < 0 ? 0 : len - j0;
   const Philox rng(DROP ? drop : DropArgs{});
-  float ak[kAcc] = {}, av[kAcc] = {};
-  if (j < sh.keys(b)) {
-    const T* kr = k + b * pk.s_b + j * pk.s_n + kh * pk.s_h;
-    const T* vr = v + b * pv.s_b + j * pv.s_n + kh * pv.s_h;
-    for (int c = lane; c < sh.dim; c += 32) {
-      ks[warp][c] = Elem<T>::to_f(kr[c]) * sh.scale;
-      vs[warp][c] = Elem<T>::to_f(vr[c]);
-    }
-    __syncwarp();
+  float ak[kOwn][NA] = {}, av[kOwn][NA] = {};
+  if (live > 0) {
+    stage(m_.oa, own, k + b * pk.s_b + j0 * pk.s_n + kh * pk.s_h, pk.s_n, live, kRows, sh.dim, sh.scale);
+    stage(m_.ob, own, v + b * pv.s_b + j0 * pv.s_n + kh * pv.s_h, pv.s_n, live, kRows, sh.dim, 1.f);
+    float* w = m_.w + warp * 2 * kTile * kOwn;
     for (int h = kh * group; h < (kh + 1) * group; ++h) {
-      const T* qh = q + b * pq.s_b + h * pq.s_h;
-      const T* gh = go + b * pgo.s_b + h * pgo.s_h;
       const int bh = b * sh.heads + h;
-      const float* lh = lse + (int64_t)bh * sh.nq;
-      const float* dh = delta + (int64_t)bh * sh.nq;
-      for (int i0 = 0; i0 < sh.nq; i0 += 32) {
-        const int i = i0 + lane;
-        float p = 0.f, ds = 0.f;
-        if (i < sh.nq) {
-          p = expf(dot(ks[warp], qh + i * pq.s_n, sh.dim) - lh[i]);
-          float dp = dot(vs[warp], gh + i * pgo.s_n, sh.dim);
-          float mult = 1.f;
-          if (DROP) mult = kept(rng, drop.limit, j, i, bh) ? drop.scale : 0.f;
-          ds = p * ((mult > 0.f ? dp * mult : 0.f) - dh[i]);
-          p *= mult;
-        }
-        const int n = sh.nq - i0 < 32 ? sh.nq - i0 : 32;
-        for (int t = 0; t < n; ++t) {
-          const float pt = __shfl_sync(0xffffffffu, p, t), dt = __shfl_sync(0xffffffffu, ds, t);
-          const T* qr = qh + (i0 + t) * pq.s_n;
-          const T* gr = gh + (i0 + t) * pgo.s_n;
+      for (int i0 = 0; i0 < sh.nq; i0 += kTile) {
+        const int count = sh.nq - i0 < kTile ? sh.nq - i0 : kTile, i = i0 + lane;
+        __syncthreads();
+        stage(m_.ta, pitch, q + b * pq.s_b + i0 * pq.s_n + h * pq.s_h, pq.s_n, count, kTile, sh.dim, 1.f);
+        stage(m_.tb, pitch, go + b * pgo.s_b + i0 * pgo.s_n + h * pgo.s_h, pgo.s_n, count, kTile, sh.dim, 1.f);
+        __syncthreads();
+        const float ls = lane < count ? lse[(int64_t)bh * sh.nq + i] : 0.f;
+        const float d = lane < count ? delta[(int64_t)bh * sh.nq + i] : 0.f;
+        float p[kOwn], ds[kOwn];
+        dots(p, m_.oa + warp * kOwn * own, own, m_.ta, pitch, sh.dim);
+        dots(ds, m_.ob + warp * kOwn * own, own, m_.tb, pitch, sh.dim);
+        // the eight keys of a warp are one group of the random bits: j0 and kOwn are multiples of eight
+        uint32_t keep = 0xffu;
+        if (DROP && lane < count)
+          keep = keep_bits(rng((uint32_t)(j0 + warp * kOwn) >> 3, (uint32_t)i, (uint32_t)bh), drop.limit);
+        const float mult = DROP ? drop.scale : 1.f;
 #pragma unroll
-          for (int a = 0; a < kAcc; ++a) {
-            if (lane + 32 * a >= sh.dim) break;
-            ak[a] = fmaf(dt, Elem<T>::to_f(qr[lane + 32 * a]), ak[a]);
-            av[a] = fmaf(pt, Elem<T>::to_f(gr[lane + 32 * a]), av[a]);
-          }
+        for (int r = 0; r < kOwn; ++r) {
+          const bool on = (keep >> r) & 1u;
+          const float e = lane < count ? expf(p[r] - ls) : 0.f;
+          ds[r] = lane < count ? e * ((on ? ds[r] * mult : 0.f) - d) : 0.f;
+          p[r] = on ? e * mult : 0.f;
         }
+        put_weights(w, p);
+        put_weights(w + kTile * kOwn, ds);
+        __syncwarp();
+        sums<NA>(av, w, m_.tb, pitch, sh.dim, count);
+        sums<NA>(ak, w + kTile * kOwn, m_.ta, pitch, sh.dim, count);
+        __syncwarp();
       }
     }
   }
-  T* ok = gk + b * pgk.s_b + j * pgk.s_n + kh * pgk.s_h;
-  T* ov = gv + b * pgv.s_b + j * pgv.s_n + kh * pgv.s_h;
 #pragma unroll
-  for (int a = 0; a < kAcc; ++a) {
-    if (lane + 32 * a >= sh.dim) break;
-    ok[lane + 32 * a] = Elem<T>::from_f(ak[a] * sh.scale);
-    ov[lane + 32 * a] = Elem<T>::from_f(av[a]);
+  for (int r = 0; r < kOwn; ++r) {
+    const int j = j0 + warp * kOwn + r;
+    if (j >= sh.nk) break;
+    const bool on = j < len;
+    T* ok = gk + b * pgk.s_b + j * pgk.s_n + kh * pgk.s_h;
+    T* ov = gv + b * pgv.s_b + j * pgv.s_n + kh * pgv.s_h;
+#pragma unroll
+    for (int a = 0; a < NA; ++a) {
+      if (lane + 32 * a >= sh.dim) break;
+      ok[lane + 32 * a] = Elem<T>::from_f(on ? ak[r][a] * sh.scale : 0.f);
+      ov[lane + 32 * a] = Elem<T>::from_f(on ? av[r][a] : 0.f);
+    }
   }
 }
 
@@ -219,10 +321,22 @@ int make_shape(Shape& sh, int64_t batch, int64_t heads, int64_t kv_heads, int64_
   return PMB_OK;
 }
 
-int row_grid(int64_t rows, unsigned& grid, const char* name) {
-  const int64_t g = (rows + kWarps - 1) / kWarps;
-  PMB_REQUIRE(g < ((int64_t)1 << 31), "%s: too many rows", name);
-  grid = (unsigned)g;
+// CTAs of `sets` (batch, head) pairs of `rows` rows each, `blocks` per pair.
+int row_grid(int64_t sets, int64_t rows, unsigned& grid, int& blocks, const char* name) {
+  const int64_t n = (rows + kRows - 1) / kRows;
+  PMB_REQUIRE(n * sets < ((int64_t)1 << 31), "%s: too many rows", name);
+  blocks = (int)n;
+  grid = (unsigned)(n * sets);
+  return PMB_OK;
+}
+
+// Launch one of the row kernels with the shared memory the head dim needs.
+template <typename... P, typename... A>
+int launch_rows(void (*kernel)(P...), unsigned grid, int dim, cudaStream_t s, const char* name, A... args) {
+  const int bytes = shared_bytes(dim);
+  PMB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), name);
+  kernel<<<grid, kThreads, bytes, s>>>(args...);
+  PMB_CHECK_LAUNCH(name);
   return PMB_OK;
 }
 
@@ -277,13 +391,15 @@ extern "C" int pmb_cross_attention_forward(const void* q, const void* k, const v
                                             workspace_bytes, s},
                              name);
   unsigned grid;
-  if (int st = row_grid(rows, grid, name)) return st;
+  int blocks;
+  if (int st = row_grid(batch * heads, nq, grid, blocks, name)) return st;
   return PMB_DISPATCH(dtype, T, name, [&] {
-    auto kernel = threshold > 0 ? attn_rows_fwd<T, true> : attn_rows_fwd<T, false>;
-    kernel<<<grid, kThreads, 0, s>>>(static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
-                                     static_cast<T*>(o), lse, pq, pk, pv, po, sh, drop);
-    PMB_CHECK_LAUNCH(name);
-    return PMB_OK;
+    auto run = [&](auto kernel) {
+      return launch_rows(kernel, grid, sh.dim, s, name, static_cast<const T*>(q), static_cast<const T*>(k),
+                         static_cast<const T*>(v), static_cast<T*>(o), lse, pq, pk, pv, po, sh, blocks, drop);
+    };
+    if (dim <= 64) return threshold > 0 ? run(attn_rows_fwd<T, true, 2>) : run(attn_rows_fwd<T, false, 2>);
+    return threshold > 0 ? run(attn_rows_fwd<T, true, 8>) : run(attn_rows_fwd<T, false, 8>);
   });
 }
 
@@ -328,23 +444,27 @@ extern "C" int pmb_cross_attention_backward(const void* q, const void* k, const 
                               name);
   float* delta = static_cast<float*>(workspace);
   unsigned qgrid, kgrid;
-  if (int st = row_grid(rows, qgrid, name)) return st;
-  if (int st = row_grid(keys, kgrid, name)) return st;
+  int qblocks, kblocks;
+  if (int st = row_grid(batch * heads, nq, qgrid, qblocks, name)) return st;
+  if (int st = row_grid(batch * kv_heads, nk, kgrid, kblocks, name)) return st;
   return PMB_DISPATCH(dtype, T, name, [&] {
+    auto run_q = [&](auto kernel) {
+      return launch_rows(kernel, qgrid, sh.dim, s, name, static_cast<const T*>(q), static_cast<const T*>(k),
+                         static_cast<const T*>(v), static_cast<const T*>(o), static_cast<const T*>(grad_out), lse,
+                         static_cast<T*>(grad_q), delta, pq, pk, pv, po, pgo, pgq, sh, qblocks, drop);
+    };
+    auto run_k = [&](auto kernel) {
+      return launch_rows(kernel, kgrid, sh.dim, s, name, static_cast<const T*>(q), static_cast<const T*>(k),
+                         static_cast<const T*>(v), static_cast<const T*>(grad_out), lse, (const float*)delta,
+                         static_cast<T*>(grad_k), static_cast<T*>(grad_v), pq, pk, pv, pgo, pgk, pgv, sh, kblocks, drop);
+    };
     if (rows > 0) {
-      auto kernel = threshold > 0 ? attn_rows_dq<T, true> : attn_rows_dq<T, false>;
-      kernel<<<qgrid, kThreads, 0, s>>>(static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
-                                        static_cast<const T*>(o), static_cast<const T*>(grad_out), lse,
-                                        static_cast<T*>(grad_q), delta, pq, pk, pv, po, pgo, pgq, sh, drop);
-      PMB_CHECK_LAUNCH(name);
+      const int st = dim <= 64 ? (threshold > 0 ? run_q(attn_rows_dq<T, true, 2>) : run_q(attn_rows_dq<T, false, 2>))
+                               : (threshold > 0 ? run_q(attn_rows_dq<T, true, 8>) : run_q(attn_rows_dq<T, false, 8>));
+      if (st) return st;
     }
-    if (keys > 0) {
-      auto kernel = threshold > 0 ? attn_rows_dkdv<T, true> : attn_rows_dkdv<T, false>;
-      kernel<<<kgrid, kThreads, 0, s>>>(static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
-                                        static_cast<const T*>(grad_out), lse, delta, static_cast<T*>(grad_k),
-                                        static_cast<T*>(grad_v), pq, pk, pv, pgo, pgk, pgv, sh, drop);
-      PMB_CHECK_LAUNCH(name);
-    }
-    return PMB_OK;
+    if (keys == 0) return PMB_OK;
+    return dim <= 64 ? (threshold > 0 ? run_k(attn_rows_dkdv<T, true, 2>) : run_k(attn_rows_dkdv<T, false, 2>))
+                     : (threshold > 0 ? run_k(attn_rows_dkdv<T, true, 8>) : run_k(attn_rows_dkdv<T, false, 8>));
   });
 }
