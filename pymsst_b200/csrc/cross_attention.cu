@@ -17,7 +17,10 @@
 // warps of a CTA.  For the dot products a lane takes one row of the tile and
 // multiplies it with the eight owned rows, which all lanes read alike; for the
 // sums a lane takes every 32nd head element.  Bound by shared-memory reads
-// (9 of 16 bytes for 32 fused multiply-adds).  Every output row is summed by
+// (9 of 16 bytes for 32 fused multiply-adds).  Measured for 62 x 8 heads x 258
+// x 258, dim 64, fp32 with dropout: forward 0.58, dQ 0.87, dK / dV 0.92 ms,
+// where a warp to one row without tiles took 10.7, 16.2 and 17.0 ms.
+// Every output row is summed by
 // one warp in the order of the tiles, so results do not depend on the order of
 // execution.
 #include "cross_attention.cuh"
@@ -54,14 +57,23 @@ struct Shared {
   }
 };
 
-// `count` rows (the rest of `rows`, and the row's padding, zeros) of a plane, times mul, into shared memory.
+// The first `count` of 32 rows of a plane (zeros for the rest and for the rows' padding), times mul, into shared
+// memory.  A warp takes eight rows whose loads are issued together: one row after the other, the forward of 62 x 8
+// heads x 258 x 258, dim 64, with dropout took 1.21 ms, like this 0.58 ms.
 template <typename T>
 __device__ __forceinline__ void stage(float* dst, int pitch, const T* __restrict__ src, int64_t s_n, int count,
-                                      int rows, int dim, float mul) {
-  const int width = own_pitch_of(dim);
-  for (int i = threadIdx.x; i < rows * width; i += kThreads) {
-    const int r = i / width, c = i - r * width;
-    dst[r * pitch + c] = r < count && c < dim ? Elem<T>::to_f(src[r * s_n + c]) * mul : 0.f;
+                                      int dim, float mul) {
+  static_assert(kTile == kRows && kTile % kWarps == 0);
+  const int width = own_pitch_of(dim), warp = threadIdx.x >> 5;
+  for (int c = threadIdx.x & 31; c < width; c += 32) {
+    float x[kTile / kWarps];
+#pragma unroll
+    for (int i = 0; i < kTile / kWarps; ++i) {
+      const int r = warp + i * kWarps;
+      x[i] = r < count && c < dim ? Elem<T>::to_f(src[r * s_n + c]) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kTile / kWarps; ++i) dst[(warp + i * kWarps) * pitch + c] = x[i] * mul;
   }
 }
 
@@ -106,9 +118,17 @@ __device__ __forceinline__ void put_weights(float* w, const float (&p)[kOwn]) {
   *reinterpret_cast<float4*>(mine + 4) = make_float4(p[4], p[5], p[6], p[7]);
 }
 
-// 16-bit number of (key, query, batch head) against the drop limit
-__device__ __forceinline__ bool kept_key(const Philox& rng, uint32_t limit, int key, int query, int bh) {
-  return (keep_bits(rng((uint32_t)key >> 3, (uint32_t)query, (uint32_t)bh), limit) >> (key & 7)) & 1u;
+// Keep bits of a tile of 32 keys (j0 a multiple of eight) and the warp's eight queries from i0 on: one Philox call
+// covers eight keys of one query, so lane l draws keys j0 + 8 (l / 8).. of query i0 + l % 8 and `kept_key` hands them out.
+__device__ __forceinline__ uint32_t draw(const Philox& rng, uint32_t limit, int j0, int i0, int bh) {
+  const int lane = threadIdx.x & 31;
+  return keep_bits(rng((uint32_t)(j0 >> 3) + (lane >> 3), (uint32_t)(i0 + (lane & 7)), (uint32_t)bh), limit);
+}
+
+// the bit of the lane's key and query i0 + i; the whole warp calls it
+__device__ __forceinline__ bool kept_key(uint32_t bits, int i) {
+  const int lane = threadIdx.x & 31;
+  return (__shfl_sync(0xffffffffu, bits, (lane & 24) | i) >> (lane & 7)) & 1u;
 }
 
 // Grid: (tiles of kRows queries) x batch x heads.
@@ -123,7 +143,7 @@ __global__ void __launch_bounds__(kThreads)
   const int bh = blockIdx.x / blocks, i0 = (blockIdx.x - bh * blocks) * kRows, h = bh % sh.heads, b = bh / sh.heads;
   const int kh = h / (sh.heads / sh.kv_heads), len = sh.keys(b);
   const Philox rng(DROP ? drop : DropArgs{});
-  stage(m_.oa, own, q + b * pq.s_b + i0 * pq.s_n + h * pq.s_h, pq.s_n, sh.nq - i0, kRows, sh.dim, sh.scale);
+  stage(m_.oa, own, q + b * pq.s_b + i0 * pq.s_n + h * pq.s_h, pq.s_n, sh.nq - i0, sh.dim, sh.scale);
   k += b * pk.s_b + kh * pk.s_h;
   v += b * pv.s_b + kh * pv.s_h;
   float m[kOwn], l[kOwn], acc[kOwn][NA] = {};
@@ -134,13 +154,14 @@ __global__ void __launch_bounds__(kThreads)
   }
   float* w = m_.w + warp * 2 * kTile * kOwn;
   for (int j0 = 0; j0 < len; j0 += kTile) {
-    const int count = len - j0 < kTile ? len - j0 : kTile, j = j0 + lane;
+    const int count = len - j0 < kTile ? len - j0 : kTile;
     __syncthreads();
-    stage(m_.ta, pitch, k + j0 * pk.s_n, pk.s_n, count, kTile, sh.dim, 1.f);
-    stage(m_.tb, pitch, v + j0 * pv.s_n, pv.s_n, count, kTile, sh.dim, 1.f);
+    stage(m_.ta, pitch, k + j0 * pk.s_n, pk.s_n, count, sh.dim, 1.f);
+    stage(m_.tb, pitch, v + j0 * pv.s_n, pv.s_n, count, sh.dim, 1.f);
     __syncthreads();
     float p[kOwn];
     dots(p, m_.oa + warp * kOwn * own, own, m_.ta, pitch, sh.dim);
+    const uint32_t bits = DROP ? draw(rng, drop.limit, j0, i0 + warp * kOwn, bh) : 0u;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       float mx = lane < count ? p[i] : -INFINITY;
@@ -152,8 +173,7 @@ __global__ void __launch_bounds__(kThreads)
       m[i] = mn;
 #pragma unroll
       for (int a = 0; a < NA; ++a) acc[i][a] *= corr;
-      if (DROP && lane < count)
-        p[i] = kept_key(rng, drop.limit, j, i0 + warp * kOwn + i, bh) ? p[i] * drop.scale : 0.f;
+      if (DROP) p[i] = kept_key(bits, i) ? p[i] * drop.scale : 0.f;
     }
     put_weights(w, p);
     __syncwarp();
@@ -185,8 +205,8 @@ __global__ void __launch_bounds__(kThreads)
   const int bh = blockIdx.x / blocks, i0 = (blockIdx.x - bh * blocks) * kRows, h = bh % sh.heads, b = bh / sh.heads;
   const int kh = h / (sh.heads / sh.kv_heads), len = sh.keys(b);
   const Philox rng(DROP ? drop : DropArgs{});
-  stage(m_.oa, own, q + b * pq.s_b + i0 * pq.s_n + h * pq.s_h, pq.s_n, sh.nq - i0, kRows, sh.dim, sh.scale);
-  stage(m_.ob, own, go + b * pgo.s_b + i0 * pgo.s_n + h * pgo.s_h, pgo.s_n, sh.nq - i0, kRows, sh.dim, 1.f);
+  stage(m_.oa, own, q + b * pq.s_b + i0 * pq.s_n + h * pq.s_h, pq.s_n, sh.nq - i0, sh.dim, sh.scale);
+  stage(m_.ob, own, go + b * pgo.s_b + i0 * pgo.s_n + h * pgo.s_h, pgo.s_n, sh.nq - i0, sh.dim, 1.f);
   __syncthreads();
   float d[kOwn], ls[kOwn];
 #pragma unroll
@@ -207,18 +227,18 @@ __global__ void __launch_bounds__(kThreads)
   float acc[kOwn][NA] = {};
   float* w = m_.w + warp * 2 * kTile * kOwn;
   for (int j0 = 0; j0 < len; j0 += kTile) {
-    const int count = len - j0 < kTile ? len - j0 : kTile, j = j0 + lane;
+    const int count = len - j0 < kTile ? len - j0 : kTile;
     __syncthreads();
-    stage(m_.ta, pitch, k + j0 * pk.s_n, pk.s_n, count, kTile, sh.dim, 1.f);
-    stage(m_.tb, pitch, v + j0 * pv.s_n, pv.s_n, count, kTile, sh.dim, 1.f);
+    stage(m_.ta, pitch, k + j0 * pk.s_n, pk.s_n, count, sh.dim, 1.f);
+    stage(m_.tb, pitch, v + j0 * pv.s_n, pv.s_n, count, sh.dim, 1.f);
     __syncthreads();
     float p[kOwn], dp[kOwn];
     dots(p, m_.oa + warp * kOwn * own, own, m_.ta, pitch, sh.dim);
     dots(dp, m_.ob + warp * kOwn * own, own, m_.tb, pitch, sh.dim);
+    const uint32_t bits = DROP ? draw(rng, drop.limit, j0, i0 + warp * kOwn, bh) : 0u;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      if (DROP && lane < count)
-        dp[i] = kept_key(rng, drop.limit, j, i0 + warp * kOwn + i, bh) ? dp[i] * drop.scale : 0.f;
+      if (DROP) dp[i] = kept_key(bits, i) ? dp[i] * drop.scale : 0.f;
       p[i] = lane < count ? expf(p[i] - ls[i]) * (dp[i] - d[i]) : 0.f;
     }
     put_weights(w, p);
@@ -252,16 +272,16 @@ __global__ void __launch_bounds__(kThreads)
   const Philox rng(DROP ? drop : DropArgs{});
   float ak[kOwn][NA] = {}, av[kOwn][NA] = {};
   if (live > 0) {
-    stage(m_.oa, own, k + b * pk.s_b + j0 * pk.s_n + kh * pk.s_h, pk.s_n, live, kRows, sh.dim, sh.scale);
-    stage(m_.ob, own, v + b * pv.s_b + j0 * pv.s_n + kh * pv.s_h, pv.s_n, live, kRows, sh.dim, 1.f);
+    stage(m_.oa, own, k + b * pk.s_b + j0 * pk.s_n + kh * pk.s_h, pk.s_n, live, sh.dim, sh.scale);
+    stage(m_.ob, own, v + b * pv.s_b + j0 * pv.s_n + kh * pv.s_h, pv.s_n, live, sh.dim, 1.f);
     float* w = m_.w + warp * 2 * kTile * kOwn;
     for (int h = kh * group; h < (kh + 1) * group; ++h) {
       const int bh = b * sh.heads + h;
       for (int i0 = 0; i0 < sh.nq; i0 += kTile) {
         const int count = sh.nq - i0 < kTile ? sh.nq - i0 : kTile, i = i0 + lane;
         __syncthreads();
-        stage(m_.ta, pitch, q + b * pq.s_b + i0 * pq.s_n + h * pq.s_h, pq.s_n, count, kTile, sh.dim, 1.f);
-        stage(m_.tb, pitch, go + b * pgo.s_b + i0 * pgo.s_n + h * pgo.s_h, pgo.s_n, count, kTile, sh.dim, 1.f);
+        stage(m_.ta, pitch, q + b * pq.s_b + i0 * pq.s_n + h * pq.s_h, pq.s_n, count, sh.dim, 1.f);
+        stage(m_.tb, pitch, go + b * pgo.s_b + i0 * pgo.s_n + h * pgo.s_h, pgo.s_n, count, sh.dim, 1.f);
         __syncthreads();
         const float ls = lane < count ? lse[(int64_t)bh * sh.nq + i] : 0.f;
         const float d = lane < count ? delta[(int64_t)bh * sh.nq + i] : 0.f;
