@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kThreads)
       float mx = lane < count ? p[i] : -INFINITY;
 #pragma unroll
       for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-      const float mn = fmaxf(m[i], mx), corr = expf(m[i] - mn);
+      const float mn = fmaxf(fmaxf(m[i], mx), xattn::kLowest), corr = expf(m[i] - mn);
       p[i] = lane < count ? expf(p[i] - mn) : 0.f;
       l[i] = l[i] * corr + warp_sum(p[i]);
       m[i] = mn;

@@ -9,6 +9,10 @@
 namespace pmb {
 namespace xattn {
 
+// Lower limit of a row's running maximum (the lowest fp32 value): scores of -infinity, from a dot product that
+// overflows, then weigh exp(-infinity) = 0 where -infinity - (-infinity) would be NaN.
+constexpr float kLowest = -3.402823466e38f;
+
 struct Plane {
   int64_t s_b, s_n, s_h;  // element strides, the head elements contiguous
 };

@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
           }
           mx *= sl2;
           if (c == c0) {
-            m = mx;
+            m = fmaxf(mx, xattn::kLowest);  // finite: a chunk of scores of -infinity weighs nothing
           } else {
             const bool grows = mx > m + kRescale;
             if (__any_sync(0xffffffffu, grows)) {

@@ -221,6 +221,28 @@ def test_large_scores_do_not_overflow(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nq", [1, 70])
+def test_leading_scores_of_minus_infinity_weigh_nothing(cuda_device, dtype, nq):
+    """Keys of the type's lowest value whose scores overflow to -infinity, whole tiles of them before ordinary ones:
+    their weights are zero, so values and gradients are those of the ordinary keys alone (zero terms leave every sum
+    as it is, and 0 times the finite key is 0)."""
+    low, n, d = 200, 260, 64
+    q, k, v, go = _inputs(2, 2, 2, nq, n, d, dtype)
+    q = q.abs() + 0.5  # every score of a low key is at most -0.5 * 3.38e38 * 64, below the lowest fp32
+    k[:, :, :low] = torch.finfo(dtype).min
+    leaves = [t.to(cuda_device).requires_grad_() for t in (q, k, v)]
+    o = cross_attention(*leaves)
+    dq, dk, dv = torch.autograd.grad(o, leaves, go.to(cuda_device))
+    assert not dk[:, :, :low].any() and not dv[:, :, :low].any()
+    rest = [t.double() for t in (q, k[:, :, low:], v[:, :, low:], go)]
+    exact = (ref.attention(*rest[:3], None, None, None), *ref.attention_grads(*rest, None, None, None))
+    bounds = ref.attention_bounds(*rest, None, None, None, dtype)
+    for got, e, bound, what in zip((o, dq, dk[:, :, low:], dv[:, :, low:]), exact, bounds, ("o", "dq", "dk", "dv")):
+        _within(got, e, bound, what)
+
+
+@pytest.mark.gpu
 def test_layouts(cuda_device):
     """[b, h, n, d] planes, packed projections, transposed heads, odd offsets and broadcasts give what copies give."""
     b, h, n, d = 2, 4, 75, 64
