@@ -71,6 +71,7 @@ class DropoutGenerator:
         key = torch.empty_like(self.state)
         with on_device(device):
             nat.call("pmb_dropout_next_key", self.state.data_ptr(), key.data_ptr(), nat.stream_handle(device))
+        torch.autograd.graph.increment_version(self.state)  # a backward that saved the state itself now raises
         return key
 
     def manual_seed(self, seed: int, step: int = 0) -> None:

@@ -211,6 +211,16 @@ def test_second_derivatives_are_refused(cuda_device):
 
 
 @pytest.mark.gpu
+def test_generator_state_used_as_key_is_an_error_after_its_next_key(cuda_device):
+    gen = DropoutGenerator(5, cuda_device)
+    x = torch.randn(64, device=cuda_device, requires_grad=True)
+    y = dropout(x, 0.5, gen.state)
+    gen.next_key()
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+
+
+@pytest.mark.gpu
 def test_generator_steps_and_restores(cuda_device):
     gen = DropoutGenerator(2**64 - 2, cuda_device)
     k0, k1 = gen.next_key(), gen.next_key()
