@@ -452,8 +452,8 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
         if (!idle) {
           // Without dropout a chunk's scores stay in registers and its code is straight; with it (45 more
           // instructions per eight scores) a loop over 32 scores that reads them twice is ahead, as the code
-          // stays small: 258 keys 182 against 224 us with dropout, 127 against 123 us without, 4096 keys 135
-          // against 116 us without.
+          // stays small.  Measured rolled against straight when this was chosen: 258 keys 182 against 224 us with
+          // dropout, 127 against 123 us without, 4096 keys 135 against 116 us without.
           uint32_t s[DROP ? 1 : 3][32];
           float mx = -INFINITY;
           if constexpr (DROP) {
@@ -640,7 +640,9 @@ __global__ void __launch_bounds__(256)
 // chunk).  With three pairs the scores a group takes next are ready when it
 // finishes a chunk.  (Time axis, 258 positions, dropout, dK / dV + dQ: one
 // pair per CTA and two CTAs per SM 321 + 219 us, three groups with a pair each
-// 355 + 290, this 310 + 247 with one issuing warp.)
+// 355 + 290, two groups over three pairs 310 + 247 with one issuing warp, 288
+// + 228 with two; now, with D from a warp of its own and item decoding without
+// divisions, 269 + 191, and 196 + 144 without dropout.)
 //
 // Barriers that groups wait on out of step have turns: item t uses barrier
 // t % NB.  A chunk's scores are complete only after the products of the chunk
