@@ -220,16 +220,46 @@ __device__ __forceinline__ float max32(const uint32_t (&s)[32], float mx) {
   return max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);
 }
 
-// 2^(s sl2 - m) of 32 scores: added to the pair of sums, and rounded to pairs of T.
-template <typename T>
+// 2^a and 2^b for a, b <= 127 on the FMA pipe, relative error 2^-22.5: n = round(x) falls out of the addition of 1.5
+// 2^23, and 2^(x - n) on [-1/2, 1/2] is a degree-five polynomial (least maximum relative error with the constant term
+// fixed at 1, fitted by reweighted least squares).  Powers below 2^-127 become 2^-127, whose exponent bits are those
+// of zero, so masked scores give exactly 0; NaN passes through the maximum and the product.
+__device__ __forceinline__ void exp2_pair(float& a, float& b) {
+  constexpr float kRound = 12582912.f;
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-127.f));
+  const uint64_t x = pk2(a, b), t = add2(x, pk2(kRound, kRound));
+  const uint64_t f = fma2(add2(t, pk2(-kRound, -kRound)), pk2(-1.f, -1.f), x);
+  uint64_t p = pk2(0.001326472731307149f, 0.001326472731307149f);
+  p = fma2(p, f, pk2(0.009671512991189957f, 0.009671512991189957f));
+  p = fma2(p, f, pk2(0.05550733581185341f, 0.05550733581185341f));
+  p = fma2(p, f, pk2(0.24022242426872253f, 0.24022242426872253f));
+  p = fma2(p, f, pk2(0.6931470036506653f, 0.6931470036506653f));
+  p = fma2(p, f, pk2(1.f, 1.f));
+  float u, v;
+  unpk2(t, u, v);
+  u = __uint_as_float((__float_as_uint(u) << 23) + 0x3f800000u);
+  v = __uint_as_float((__float_as_uint(v) << 23) + 0x3f800000u);
+  unpk2(mul2(p, pk2(u, v)), a, b);
+}
+
+// 2^(s sl2 - m) of 32 scores: added to the pair of sums, and rounded to pairs of T.  With MIX every fourth pair comes
+// from the FMA pipe, the rest from the special-function pipe, which alone is busy for half the time: 4096 x 4096
+// without dropout 119.5 us with none of 16 pairs, 116.8 with two, 113.9 with four, 126.5 with eight; one query over
+// 8192 keys 81.4, 78.7, 78.0, 80.5.  With dropout instruction issue is the bound and all stay there.
+template <typename T, bool MIX>
 __device__ __forceinline__ void exp32(const uint32_t (&s)[32], uint64_t sl22, uint64_t m22, uint64_t& sum,
                                       uint32_t (&p2)[16]) {
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
     float a, b;
     unpk2(fma2(pk2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sl22, m22), a, b);
-    a = ex2(a);
-    b = ex2(b);
+    if (MIX && e % 4 == 1) {
+      exp2_pair(a, b);
+    } else {
+      a = ex2(a);
+      b = ex2(b);
+    }
     sum = add2(sum, pk2(a, b));
     p2[e] = pack2<T>(a, b);
   }
@@ -521,7 +551,7 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
               wait_ld();
               tie32(s[0]);
               if (first + 32 > keys) mask_tail(s[0], keys - first);
-              exp32<T>(s[0], sl22, m22, sum, p2);
+              exp32<T, false>(s[0], sl22, m22, sum, p2);
 #pragma unroll
               for (int e = 0; e < 16; ++e) p2[e] &= mask[e];
               umma::tmem_st16(src + first / 2, p2);  // over scores this warp has read
@@ -530,7 +560,7 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
 #pragma unroll
             for (int i = 0; i < 3; ++i) {
               if (i * 32 < keys) {
-                exp32<T>(s[i], sl22, m22, sum, p2);
+                exp32<T, true>(s[i], sl22, m22, sum, p2);
                 umma::tmem_st16(src + i * 16, p2);
               }
             }

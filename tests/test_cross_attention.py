@@ -243,6 +243,20 @@ def test_leading_scores_of_minus_infinity_weigh_nothing(cuda_device, dtype, nq):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,p", [(torch.float16, 0.0), (torch.bfloat16, 0.0), (torch.bfloat16, 0.1),
+                                     (torch.float32, 0.0)])
+def test_nan_in_a_live_key_reaches_every_row(cuda_device, dtype, p):
+    """One key of each batch item is NaN, at every place of a tile's 32 columns: no row may come out finite."""
+    places, n = 33, 130
+    q, k, v, _ = _inputs(places, 2, 1, 3, n, 64, dtype)
+    for i in range(places):
+        k[i, :, i + (96 if i % 2 else 0)] = float("nan")
+    key = _key(cuda_device) if p > 0 else None
+    o = cross_attention(*(t.to(cuda_device) for t in (q, k, v)), dropout_p=p, key=key, site=SITE)
+    assert bool(torch.isnan(o).any(dim=-1).all())
+
+
+@pytest.mark.gpu
 def test_layouts(cuda_device):
     """[b, h, n, d] planes, packed projections, transposed heads, odd offsets and broadcasts give what copies give."""
     b, h, n, d = 2, 4, 75, 64
