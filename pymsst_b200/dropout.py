@@ -27,6 +27,10 @@ from . import _native as nat
 _NO_GUARD = contextlib.nullcontext()
 _MAX_SITE = 2**32
 
+# Generator states whose addresses captured graphs hold: every replay reads and writes them, so they must not go back
+# to the allocator when the generator does.
+_captured_states: list[torch.Tensor] = []
+
 
 def on_device(device: torch.device):
     """Context in which launches go to ``device`` (nothing to do when it is the current one)."""
@@ -58,7 +62,8 @@ def check_key(key, threshold: int, site: int, device: torch.device, name: str) -
 class DropoutGenerator:
     """Source of dropout keys: ``state`` holds (seed, step) on the device, :meth:`next_key` returns a copy of it and
     moves the step on, in one kernel.  Captured into a CUDA graph, every replay draws new masks; the steps go on
-    where the last replay or eager call left them."""
+    where the last replay or eager call left them.  The graph keeps to the generator it was captured with, whose
+    state then stays allocated for good: a model that is given another one has to be captured again (Trainer does)."""
 
     def __init__(self, seed: int = 0, device: torch.device | str | None = None):
         if device is None:
@@ -70,6 +75,8 @@ class DropoutGenerator:
         device = nat.require_cuda(self.state, name="DropoutGenerator")
         key = torch.empty_like(self.state)
         with on_device(device):
+            if torch.cuda.is_current_stream_capturing() and not any(t is self.state for t in _captured_states):
+                _captured_states.append(self.state)
             nat.call("pmb_dropout_next_key", self.state.data_ptr(), key.data_ptr(), nat.stream_handle(device))
         torch.autograd.graph.increment_version(self.state)  # a backward that saved the state itself now raises
         return key

@@ -98,7 +98,10 @@ class Trainer:
     library plan and cached table exists before the capture, initialises the
     Adam state with an update of zero, and then captures; every call,
     including the first, applies exactly one update.  Input shapes must stay
-    fixed; the returned loss tensor is overwritten by the next step."""
+    fixed; the returned loss tensor is overwritten by the next step.  A step
+    after the model was given another dropout generator, or none, captures
+    again (with its untimed passes, so every rank has to change at the same
+    step); parameters and Adam state carry on."""
 
     def __init__(self, model: torch.nn.Module, *, lr: float = 1e-4, amp_dtype: torch.dtype | None = None,
                  grad_clip: float = 0.0, distributed: bool = False, device: torch.device | None = None,
@@ -154,6 +157,7 @@ class Trainer:
         self.optimizer = torch.optim.Adam(opt_params, lr=lr, fused=fused_adam and on_cuda,
                                           capturable=self.cuda_graph)
         self._graph = None
+        self._graph_generator = None  # the model's dropout generator that the captured step draws from
         self._static = None
         self.launches_per_step = None  # this package's kernels in one captured step
 
@@ -169,6 +173,7 @@ class Trainer:
         self._hook_handles = []
         self._works = []
         self._graph = None
+        self._graph_generator = None
         self._static = None
 
     # ------------------------------------------------------------- flat layout
@@ -375,7 +380,14 @@ class Trainer:
     def _capture(self, mixture, target):
         from . import _native as nat
 
-        static_mix, static_tgt = mixture.clone(), target.clone()
+        if self._static is not None:  # captured before: the buffers stay
+            torch.cuda.synchronize(self.device)
+            self._graph = None  # its memory pool goes before the new one grows
+            static_mix, static_tgt, _ = self._static
+            static_mix.copy_(mixture)
+            static_tgt.copy_(target)
+        else:
+            static_mix, static_tgt = mixture.clone(), target.clone()
         generator = getattr(self.model, "dropout_generator", None)
         steps = None if generator is None else generator.state.clone()
         side = torch.cuda.Stream(self.device)
@@ -386,18 +398,19 @@ class Trainer:
                 self._zero_grads()
                 self._forward_backward(static_mix, static_tgt)
                 self._finish_grads()
-            # Adam state (moments, device step counters) created by an update of zero
             if self.flat_grad is not None:
                 self.flat_grad.zero_()
-            else:
-                for p in self.params:
-                    p.grad = torch.zeros_like(p)
-            self.optimizer.step()
-            for group in self.optimizer.param_groups:
-                for p in group["params"]:
-                    st = self.optimizer.state[p]
-                    if "step" in st:
-                        st["step"].zero_()
+            if not self.optimizer.state:
+                # Adam state (moments, device step counters) created by an update of zero
+                if self.flat_grad is None:
+                    for p in self.params:
+                        p.grad = torch.zeros_like(p)
+                self.optimizer.step()
+                for group in self.optimizer.param_groups:
+                    for p in group["params"]:
+                        st = self.optimizer.state[p]
+                        if "step" in st:
+                            st["step"].zero_()
         torch.cuda.current_stream(self.device).wait_stream(side)
         self._zero_grads()
         self.check_kernels()
@@ -437,7 +450,10 @@ class Trainer:
             p.grad = None
 
     def _graph_step(self, mixture, target):
-        if self._graph is None:
+        generator = getattr(self.model, "dropout_generator", None)
+        if self._graph is None or generator is not self._graph_generator:
+            # the graph holds the generator's address: another one, or none, needs another graph
+            self._graph_generator = generator
             self._capture(mixture, target)
         static_mix, static_tgt, loss = self._static
         if mixture.data_ptr() != static_mix.data_ptr():

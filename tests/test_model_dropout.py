@@ -1,13 +1,18 @@
 """Models whose dropout comes from a generator, and the new operators in a row as a block uses them."""
 from __future__ import annotations
 
+import contextlib
+import gc
 import math
+import weakref
 
 import pytest
 import torch
 
 from oracle import context_ref as ref
+from pymsst_b200 import _native as nat
 from pymsst_b200 import config as cfg
+from pymsst_b200 import dropout as dropout_module
 from pymsst_b200 import synthetic
 from pymsst_b200.cross_attention import cross_attention, rotary_axes
 from pymsst_b200.dropout import DropoutGenerator, dropout, gelu_dropout
@@ -189,3 +194,102 @@ def test_captured_training_step_draws_new_masks_each_replay(cuda_device, recompu
     for a, b, c in zip(eager, captured, other):
         assert abs(a - b) <= 1e-4 * abs(a)
         assert abs(a - c) > 1e-4 * abs(a)
+
+
+class _Stub(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.lin = torch.nn.Linear(4, 4)
+        self.dropout_generator = None
+
+    def forward(self, mix, target):
+        return (self.lin(mix) - target).abs().mean()
+
+
+def test_exchanged_generator_captures_the_step_again(monkeypatch):
+    """Host logic of the captured step on the CPU, the capture and its replay replaced by counters."""
+    trainer = Trainer(_Stub(), device=torch.device("cpu"))
+    trainer.cuda_graph = True
+    replays = []
+
+    class Graph:
+        def replay(self):
+            replays.append(self)
+
+    def capture(mixture, target):
+        trainer._graph, trainer._static = Graph(), (mixture.clone(), target.clone(), torch.zeros(()))
+
+    monkeypatch.setattr(trainer, "_capture", capture)
+    mix = torch.zeros(2, 4)
+    seen = []
+    first, second = object(), object()
+    for generator in (None, None, first, first, second, None):
+        trainer.model.dropout_generator = generator
+        trainer.step(mix, mix)
+        seen.append(replays[-1])
+    assert seen[0] is seen[1] and seen[2] is seen[3]
+    assert len({id(g) for g in seen}) == 4
+
+
+def test_captured_state_outlives_its_generator(monkeypatch):
+    """A key drawn while a stream captures leaves the state's address in the graph; drawn otherwise it does not."""
+    monkeypatch.setattr(nat, "require_cuda", lambda *t, name: t[0].device)
+    monkeypatch.setattr(nat, "stream_handle", lambda device: 0)
+    monkeypatch.setattr(nat, "call", lambda *args: None)
+    monkeypatch.setattr(dropout_module, "on_device", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(dropout_module, "_captured_states", [])
+    for capturing in (False, True):
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+        gen = DropoutGenerator(1, "cpu")
+        gen.next_key()
+        gen.next_key()
+        state = weakref.ref(gen.state)
+        del gen
+        gc.collect()
+        assert (state() is not None) == capturing
+    assert len(dropout_module._captured_states) == 1
+
+
+@pytest.mark.gpu
+def test_replays_write_no_released_memory(cuda_device):
+    """The generator of a captured forward is dropped and blocks of its state's size are handed out again: replays leave
+    them alone and go on drawing new masks."""
+    gen = DropoutGenerator(6, cuda_device)
+    x = torch.ones(4096, device=cuda_device)
+    dropout(x, 0.5, gen.next_key())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = dropout(x, 0.5, gen.next_key())
+    del gen
+    gc.collect()
+    others = [torch.zeros(2, dtype=torch.int64, device=cuda_device) for _ in range(256)]
+    masks = []
+    for _ in range(3):
+        graph.replay()
+        masks.append(y.clone())
+    assert not any(bool(t.any()) for t in others)
+    for replay, mask in enumerate(masks):
+        assert torch.equal(mask.cpu().double(), ref.dropout_mult(x.numel(), 0.5, 6, 1 + replay, 0))
+
+
+@pytest.mark.gpu
+def test_captured_trainer_follows_an_exchanged_generator(cuda_device):
+    """Two steps with one generator, two with another, against the same steps uncaptured: equal losses to what fp32 sums
+    in another order leave (1e-4 relative over four Adam steps), equal steps of both generators; then none."""
+    mix, tgt = (t.to(cuda_device) for t in synthetic.make_batch(1, 256, seed=1))
+    losses = []
+    for graph in (False, True):
+        model = _model(TINY_LOSS, cuda_device)
+        trainer = Trainer(model, lr=1e-3, cuda_graph=graph, device=cuda_device)
+        run = []
+        for seed in (4, 8):
+            model.set_dropout_generator(DropoutGenerator(seed, cuda_device))
+            run += [float(trainer.step(mix, tgt)) for _ in range(2)]
+            assert model.dropout_generator.state_dict() == {"seed": seed, "step": 2}
+        losses.append(run)
+        model.set_dropout_generator(None)
+        last = [float(trainer.step(mix, tgt)) for _ in range(3)]
+        assert len(set(last)) == 3 and all(math.isfinite(v) for v in last)
+        trainer.close()
+    for a, b in zip(*losses):
+        assert abs(a - b) <= 1e-4 * abs(a)
