@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as nat
-from .dropout import check_key, drop_threshold, on_device
+from .dropout import check_key, drop_threshold, needs_function, on_device
 
 MAX_HEAD_DIM = 256
 
@@ -148,7 +148,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
         key_lengths = key_lengths.contiguous()
     scale = float(d) ** -0.5 if scale is None else float(scale)
     q, k, v = _plane(q), _plane(k), _plane(v)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if needs_function(q, k, v):
         return CrossAttentionFn.apply(q, k, v, key_lengths, scale, threshold, key, site)
     return _attention_forward(q, k, v, key_lengths, scale, threshold, key, site)[0]
 
@@ -233,6 +233,6 @@ def rotary_axes(t: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, s
         raise ValueError(f"{name}: positions and freqs get no gradient; detach them")
     nat.require_cuda(t, positions, freqs, name=name)
     positions, freqs = positions.contiguous(), freqs.contiguous()
-    if torch.is_grad_enabled() and t.requires_grad:
+    if needs_function(t, positions, freqs):
         return RotaryAxesFn.apply(t, positions, freqs, sections)
     return _rotary(t, positions, freqs, sections, 0)

@@ -20,6 +20,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as nat
@@ -35,6 +36,14 @@ _captured_states: list[torch.Tensor] = []
 def on_device(device: torch.device):
     """Context in which launches go to ``device`` (nothing to do when it is the current one)."""
     return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def needs_function(*tensors: torch.Tensor | None) -> bool:
+    """Whether a call has to go through its autograd Function: an input needs a gradient, or carries a forward-mode
+    tangent, which the Function refuses (the kernel alone would leave it out)."""
+    grad = torch.is_grad_enabled()
+    return any(t is not None and ((grad and t.requires_grad) or forward_ad.unpack_dual(t).tangent is not None)
+               for t in tensors)
 
 
 def drop_threshold(p: float) -> int:
@@ -142,7 +151,7 @@ def dropout(x: torch.Tensor, p: float, key: torch.Tensor | None = None, site: in
                          f"{residual.dtype}")
     nat.require_cuda(x, residual, name="dropout")
     nat.dtype_code(x.dtype)
-    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+    if needs_function(x, residual):
         return DropoutFn.apply(x, residual, threshold, key, site)
     return _dropout(x, residual, threshold, key, site)
 
@@ -186,6 +195,6 @@ def gelu_dropout(x: torch.Tensor, p: float, key: torch.Tensor | None = None, sit
     check_key(key, threshold, site, x.device, "gelu_dropout")
     nat.require_cuda(x, name="gelu_dropout")
     nat.dtype_code(x.dtype)
-    if torch.is_grad_enabled() and x.requires_grad:
+    if needs_function(x):
         return GeluDropoutFn.apply(x, threshold, key, site)
     return _gelu_dropout(x.contiguous(), threshold, key, site)

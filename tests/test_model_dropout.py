@@ -196,6 +196,54 @@ def test_captured_training_step_draws_new_masks_each_replay(cuda_device, recompu
         assert abs(a - c) > 1e-4 * abs(a)
 
 
+def _operator_calls(device):
+    """One call of each operator without a gradient to any input: the call, and the inputs that are numbers."""
+    def rand(*shape):
+        return torch.randn(*shape, device=device)
+
+    key = torch.tensor([1, 2], device=device)
+    q, k, v = rand(1, 2, 3, 8), rand(1, 1, 5, 8), rand(1, 1, 5, 8)
+    return {
+        "dropout": (lambda x, r: dropout(x, 0.5, key, residual=r), (rand(16), rand(16))),
+        "dropout_without_residual": (lambda x: dropout(x, 0.5, key), (rand(16),)),
+        "gelu_dropout": (lambda x: gelu_dropout(x, 0.5, key), (rand(16),)),
+        "cross_attention": (cross_attention, (q, k, v)),
+        "rotary_axes": (lambda t, pos, f: rotary_axes(t, pos, f, [2, 2]), (q, rand(3, 2), rand(4))),
+    }
+
+
+def _refuses_tangents(device):
+    forward_ad = torch.autograd.forward_ad
+    for name, (call, inputs) in _operator_calls(device).items():
+        call(*inputs)
+        with forward_ad.dual_level():
+            call(*inputs)  # no tangent among the inputs
+            for i in range(len(inputs)):
+                duals = [forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(inputs)]
+                for grad in (True, False):
+                    with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="jvp"):
+                        call(*duals)
+                        pytest.fail(f"{name}: input {i}'s tangent is gone without an error")
+
+
+def test_forward_mode_tangents_are_refused(monkeypatch):
+    """Nothing may drop a tangent; the launches are replaced by copies, as no GPU is needed to see which way a call
+    takes."""
+    from pymsst_b200 import cross_attention as attention_module
+
+    monkeypatch.setattr(nat, "require_cuda", lambda *t, name: t[0].device)
+    monkeypatch.setattr(dropout_module, "_dropout", lambda x, *rest: x.clone())
+    monkeypatch.setattr(dropout_module, "_gelu_dropout", lambda x, *rest: x.clone())
+    monkeypatch.setattr(attention_module, "_attention_forward", lambda q, *rest: (q.clone(), q.new_zeros(1)))
+    monkeypatch.setattr(attention_module, "_rotary", lambda t, *rest: t.clone())
+    _refuses_tangents("cpu")
+
+
+@pytest.mark.gpu
+def test_forward_mode_tangents_are_refused_on_the_device(cuda_device):
+    _refuses_tangents(cuda_device)
+
+
 class _Stub(torch.nn.Module):
     def __init__(self):
         super().__init__()
