@@ -679,8 +679,8 @@ PMB_API int pmb_gelu_dropout_backward(const void* grad_out, const void* x, void*
  * (forward: q, k, v, o = 12 values; backward: q, k, v, o, grad_out, grad_q,
  * grad_k, grad_v = 24 values).  key_lengths: device int32 [batch], clamped to
  * [0, nk], or NULL (every key).  Keys at or behind the length never reach a
- * result, whatever they hold, and get zero gradients.  A row without keys has
- * O = 0 and no gradient.  lse: fp32, pmb_cross_attention_lse_size(batch,
+ * result, whatever they hold, and get zero gradients.  A row without keys, or
+ * whose scores are all -infinity, has O = 0 and no gradient.  lse: fp32, pmb_cross_attention_lse_size(batch,
  * heads, nq) values, 16-byte aligned: row statistics that the forward writes
  * for the backward of the same call (their order and base are its own).
  * 16-bit types with head dims that are multiples of 8 up to 128 and scale >

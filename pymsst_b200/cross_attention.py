@@ -118,8 +118,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
     defaults to d ** -0.5.  fp32, bf16 and fp16.  Returns [b, heads, nq, d], a view of a [b, nq, heads, d] plane.
 
     ``key_lengths`` (int32 or int64 [b], values clamped to [0, nk]): each batch item's keys are its first ones; what
-    lies behind them is never used and gets a zero gradient.  Rows without keys give zeros.  ``dropout_p`` needs a
-    ``key`` of :class:`~pymsst_b200.dropout.DropoutGenerator`; ``site`` as in :func:`~pymsst_b200.dropout.dropout`.
+    lies behind them is never used and gets a zero gradient.  Rows without keys, or with scores of -infinity alone, give
+    zeros and no gradient; NaN in a row's live scores makes the row NaN.  ``dropout_p`` needs a ``key`` of :class:`~pymsst_b200.dropout.DropoutGenerator`; ``site`` as in :func:`~pymsst_b200.dropout.dropout`.
     Forward and backward are deterministic."""
     name = "cross_attention"
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:

@@ -6,9 +6,10 @@
 //   D = rowsum(dO * O) (= rowsum(P dP)),  dP = keep c (dO V^T),
 //   dS = P (dP - D),  dV = Pd^T dO,  dQ = scale dS K,  dK = scale dS^T Q
 //
-// dK and dV sum over the query heads of a group.  A row without keys has
-// O = 0, lse = -inf and no gradient; keys at or behind `len` are never read,
-// and their gradients are zeros.
+// dK and dV sum over the query heads of a group.  A row without keys, or with
+// scores of -infinity alone, has O = 0, P = 0 (its lse is stored so that the
+// backward's exponentials are zeros: +inf in the row form) and no gradient;
+// keys at or behind `len` are never read, and their gradients are zeros.
 //
 // The C entries, and the row form, all arithmetic fp32: it serves fp32 and
 // head dims the tensor-core form (cross_attention_tc.cu) does not take.  A
@@ -185,11 +186,11 @@ __global__ void __launch_bounds__(kThreads)
     const int r = i0 + warp * kOwn + i;
     if (r >= sh.nq) break;
     T* out = o + b * po.s_b + r * po.s_n + h * po.s_h;
-    const float inv = len > 0 ? 1.f / l[i] : 0.f;
+    const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];  // no keys, or scores of -infinity alone
 #pragma unroll
     for (int a = 0; a < NA; ++a)
       if (lane + 32 * a < sh.dim) out[lane + 32 * a] = Elem<T>::from_f(acc[i][a] * inv);
-    if (lane == 0) lse[(int64_t)bh * sh.nq + r] = len > 0 ? m[i] + logf(l[i]) : -INFINITY;
+    if (lane == 0) lse[(int64_t)bh * sh.nq + r] = l[i] == 0.f ? INFINITY : m[i] + logf(l[i]);
   }
 }
 

@@ -21,8 +21,8 @@
 //
 // Row statistics are base-2 logarithms (lse2 = max + log2(sum), of scores
 // times scale * log2 e), kept negated, as the backward adds them; -inf for a
-// row without keys, whose probabilities then come out as 0.  D is kept negated
-// too.
+// row without keys, or with scores of -infinity alone, whose probabilities then
+// come out as 0.  D is kept negated too.
 #include "attention_tiles.cuh"
 #include "cross_attention.cuh"
 #include "f32x2.cuh"
@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
         break;
       }
       umma::tc_fence_after();
-      const float inv = (DROP ? drop.scale : 1.f) / l;
+      const float inv = l == 0.f ? 0.f : (DROP ? drop.scale : 1.f) / l;  // every score -infinity: as without keys
 #pragma unroll 1
       for (int k = 0; k < 2 * DC; ++k) {
         if (idle || k * 32 >= sh.dim) break;
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(fw::kThreads, DC == 1 ? 2 : 1)
       if (valid) {
         const float stat2 = m + log2f(l);
         if (g.splits > 1) part_lse[prow()] = stat2;
-        else lse[stat()] = -stat2;
+        else lse[stat()] = l == 0.f ? -INFINITY : -stat2;
       }
     }
   }
@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(256)
   bool any = false;
   for (int s = 0; s < g.splits; ++s) {
     const float l2 = ls[(int64_t)s * g.rows];
-    if (l2 == -INFINITY) continue;  // no keys there
+    if (l2 == -INFINITY) continue;  // no keys there, or none that weighs anything
     any = true;
     const float ws = exp2f(l2 - mx);
     w += ws;

@@ -242,6 +242,67 @@ def test_leading_scores_of_minus_infinity_weigh_nothing(cuda_device, dtype, nq):
         _within(got, e, bound, what)
 
 
+def _splits(b, hq, hk, nq, nk, d, dtype):
+    return nat.library().pmb_cross_attention_forward_workspace_size(b, hq, hk, nq, nk, d, nat.dtype_code(dtype)) > 0
+
+
+# one key range per row tile, several that a second kernel joins, packed heads, a wide head, the row form
+INFINITE = [(2, 8, 2, 70, 130, 64, torch.bfloat16, False), (1, 2, 2, 3, 3000, 64, torch.bfloat16, True),
+            (2, 4, 1, 5, 2500, 128, torch.bfloat16, True), (2, 2, 1, 40, 70, 64, torch.float32, False),
+            (1, 2, 2, 5, 33, 136, torch.bfloat16, False)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("p", [0.0, 0.2])
+@pytest.mark.parametrize("b,hq,hk,nq,nk,d,dtype,split", INFINITE)
+def test_rows_of_scores_of_minus_infinity_are_zeros(cuda_device, b, hq, hk, nq, nk, d, dtype, split, p):
+    """Even queries meet keys of the type's lowest value in scores that overflow to -infinity (at most -0.5 * 3.38e38 *
+    d): zeros, and no gradient.  Odd queries are zero vectors, whose scores are zeros: with every value 1 they are means
+    of ones, and with dropout sums of the kept ones' scale over the row's count."""
+    assert _splits(b, hq, hk, nq, nk, d, dtype) == split
+    q, k, _, go = _inputs(b, hq, hk, nq, nk, d, dtype)
+    q = q.abs() + 0.5
+    q[:, :, 1::2] = 0
+    k = torch.full_like(k, torch.finfo(dtype).min)
+    leaves = [t.to(cuda_device).requires_grad_() for t in (q, k, torch.ones_like(k))]
+    key = _key(cuda_device) if p > 0 else None
+    o = cross_attention(*leaves, dropout_p=p, key=key, site=SITE)
+    only_even = go.clone()
+    only_even[:, :, 1::2] = 0
+    for grad in torch.autograd.grad(o, leaves, only_even.to(cuda_device), retain_graph=True):
+        assert not bool(grad.any())
+    _, _, dv = torch.autograd.grad(o, leaves, go.to(cuda_device))
+    o = o.detach().double().cpu()
+    assert not bool(o[:, :, 0::2].any())
+    mult = _mult(q, k, p)
+    weight = torch.ones(b, hq, nq, nk, dtype=torch.float64) if mult is None else mult
+    # sums of nk terms in fp32, a tile's at a time: 2^-24 nk of the sum bounds any order; one rounding to dtype
+    u = torch.finfo(dtype).eps / 2 + nk * 2.0**-24
+    exact = weight.mean(-1)[:, :, 1::2, None].expand_as(o[:, :, 1::2])
+    assert bool(((o[:, :, 1::2] - exact).abs() <= 2 * u * exact).all())  # 1/nk and its sum are rounded as well
+    odd = (weight / nk)[:, :, 1::2].transpose(-1, -2) @ go.double()[:, :, 1::2]
+    size = (weight / nk)[:, :, 1::2].transpose(-1, -2) @ go.double()[:, :, 1::2].abs()
+    odd, size = (t.reshape(b, hk, hq // hk, nk, d).sum(2) for t in (odd, size))
+    bound = 2 * (u + nq * (hq // hk) * 2.0**-24) * size + torch.finfo(dtype).tiny
+    assert bool(((dv.double().cpu() - odd).abs() <= bound).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("p", [0.0, 0.2])
+@pytest.mark.parametrize("b,hq,hk,nq,nk,d,dtype,split", INFINITE)
+def test_nan_beside_scores_of_minus_infinity_stays_nan(cuda_device, b, hq, hk, nq, nk, d, dtype, split, p):
+    """One live key of NaN among keys whose scores are -infinity: rows and gradients of the queries are NaN, whichever
+    form and range it falls to."""
+    q, k, v, go = _inputs(b, hq, hk, nq, nk, d, dtype)
+    q, k = q.abs() + 0.5, torch.full_like(k, torch.finfo(dtype).min)
+    k[:, :, nk * 2 // 3] = torch.nan
+    leaves = [t.to(cuda_device).requires_grad_() for t in (q, k, v)]
+    key = _key(cuda_device) if p > 0 else None
+    o = cross_attention(*leaves, dropout_p=p, key=key, site=SITE)
+    dq, _, _ = torch.autograd.grad(o, leaves, go.to(cuda_device))
+    assert bool(torch.isnan(o).any(dim=-1).all()) and bool(torch.isnan(dq).any(dim=-1).all())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,p", [(torch.float16, 0.0), (torch.bfloat16, 0.0), (torch.bfloat16, 0.1),
                                      (torch.float32, 0.0)])
