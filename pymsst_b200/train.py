@@ -13,6 +13,7 @@ records the loss of every step.
 """
 from __future__ import annotations
 
+import contextlib
 import os
 from dataclasses import dataclass, field
 
@@ -337,6 +338,16 @@ class Trainer:
         self.scaler.step(self.optimizer)
         self.scaler.update()
 
+    @contextlib.contextmanager
+    def _dropout_steps_kept(self):
+        """Passes inside are no training steps: the model's dropout generator is put back to where it was, so the
+        training steps' masks do not depend on them."""
+        generator = getattr(self.model, "dropout_generator", None)
+        state = None if generator is None else generator.state.clone()
+        yield
+        if state is not None:
+            generator.state.copy_(state)
+
     def _warm_relayout(self, mixture, target):
         """One untimed forward/backward that records the order in which gradients become final, then the
         flat layout in that order (overlap_allreduce only)."""
@@ -344,7 +355,8 @@ class Trainer:
             return
         self._zero_grads()
         self._ready_order = []
-        self._forward_backward(mixture, target)
+        with self._dropout_steps_kept():
+            self._forward_backward(mixture, target)
         self._maybe_relayout()
         self._zero_grads()
 
@@ -388,16 +400,15 @@ class Trainer:
             static_tgt.copy_(target)
         else:
             static_mix, static_tgt = mixture.clone(), target.clone()
-        generator = getattr(self.model, "dropout_generator", None)
-        steps = None if generator is None else generator.state.clone()
         side = torch.cuda.Stream(self.device)
         side.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(side):
             self._warm_relayout(static_mix, static_tgt)
-            for _ in range(3):
-                self._zero_grads()
-                self._forward_backward(static_mix, static_tgt)
-                self._finish_grads()
+            with self._dropout_steps_kept():  # the captured run draws the masks that an uncaptured one does
+                for _ in range(3):
+                    self._zero_grads()
+                    self._forward_backward(static_mix, static_tgt)
+                    self._finish_grads()
             if self.flat_grad is not None:
                 self.flat_grad.zero_()
             if not self.optimizer.state:
@@ -414,8 +425,6 @@ class Trainer:
         torch.cuda.current_stream(self.device).wait_stream(side)
         self._zero_grads()
         self.check_kernels()
-        if steps is not None:  # the untimed passes drew keys: the captured run draws those an uncaptured one does
-            generator.state.copy_(steps)
         graph = torch.cuda.CUDAGraph()
         before = nat.library().pmb_launch_count()
         with torch.cuda.graph(graph):
@@ -437,7 +446,7 @@ class Trainer:
         graph = torch.cuda.CUDAGraph()
         self._profiling = True
         try:
-            with torch.cuda.graph(graph):
+            with torch.cuda.graph(graph), self._dropout_steps_kept():  # in the graph, so at every replay
                 self._forward_backward(static_mix, static_tgt)
         finally:
             self._profiling = False

@@ -341,3 +341,47 @@ def test_captured_trainer_follows_an_exchanged_generator(cuda_device):
         trainer.close()
     for a, b in zip(*losses):
         assert abs(a - b) <= 1e-4 * abs(a)
+
+
+def test_relayout_pass_takes_no_step_of_the_generator(monkeypatch):
+    """The pass that orders the flat buffers (overlapped all-reduce, one rank here) draws a key; the training steps start
+    where the generator was."""
+    import torch.distributed as dist
+
+    class Counter:
+        def __init__(self):
+            self.state = torch.tensor([3, 0])
+            self.drawn = []
+
+        def next_key(self):
+            self.drawn.append(int(self.state[1]))
+            self.state[1] += 1
+
+    class Model(_Stub):
+        def forward(self, mix, target):
+            self.dropout_generator.next_key()
+            return super().forward(mix, target)
+
+    monkeypatch.setattr(dist, "broadcast", lambda tensor, src: None)
+    trainer = Trainer(Model(), device=torch.device("cpu"), flat_params=True)
+    generator = trainer.model.dropout_generator = Counter()
+    trainer._relayout_done = False
+    for _ in range(2):
+        trainer.step(torch.randn(2, 4), torch.randn(2, 4))
+    assert generator.drawn == [0, 0, 1] and generator.state.tolist() == [3, 2]
+
+
+@pytest.mark.gpu
+def test_profiled_replays_take_no_step_of_the_generator(cuda_device):
+    mix, tgt = (t.to(cuda_device) for t in synthetic.make_batch(1, 256, seed=1))
+    model = _model(TINY_LOSS, cuda_device)
+    model.set_dropout_generator(DropoutGenerator(4, cuda_device))
+    trainer = Trainer(model, lr=1e-3, cuda_graph=True, device=cuda_device)
+    trainer.step(mix, tgt)
+    profile = trainer.profile_graph()
+    for _ in range(3):
+        profile.replay()
+    assert model.dropout_generator.state_dict() == {"seed": 4, "step": 1}
+    trainer.step(mix, tgt)
+    assert model.dropout_generator.state_dict() == {"seed": 4, "step": 2}
+    trainer.close()
