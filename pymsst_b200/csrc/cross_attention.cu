@@ -329,13 +329,19 @@ __global__ void __launch_bounds__(kThreads)
 // ------------------------------------------------------------------ host
 Plane plane_at(const int64_t* s, int i) { return Plane{s[3 * i], s[3 * i + 1], s[3 * i + 2]}; }
 
+// Sizes that the kernels' 32-bit indices hold; products of them are formed only behind this.
+bool indexable(int64_t batch, int64_t heads, int64_t nq, int64_t nk) {
+  constexpr int64_t kMax = 1 << 30;
+  return batch < kMax && heads < kMax && nq < kMax && nk < kMax && batch * heads < kMax;
+}
+
 int make_shape(Shape& sh, int64_t batch, int64_t heads, int64_t kv_heads, int64_t nq, int64_t nk, int64_t dim,
                const int32_t* lengths, float scale, int threshold, const int64_t* key, const char* name) {
   PMB_REQUIRE(batch >= 0 && nq >= 0 && nk >= 0 && heads > 0 && kv_heads > 0, "%s: bad shape", name);
   PMB_REQUIRE(heads % kv_heads == 0, "%s: %lld heads are not a multiple of %lld key / value heads", name,
               (long long)heads, (long long)kv_heads);
   PMB_REQUIRE(dim > 0 && dim <= kMaxDim, "%s: head dim %lld outside [1, %d]", name, (long long)dim, kMaxDim);
-  PMB_REQUIRE(nq < (1 << 30) && nk < (1 << 30) && batch * heads < (1 << 30), "%s: too large", name);
+  PMB_REQUIRE(indexable(batch, heads, nq, nk), "%s: too large", name);
   PMB_REQUIRE(threshold >= 0 && threshold <= 65536, "%s: drop threshold %d outside [0, 65536]", name, threshold);
   PMB_REQUIRE(key || threshold == 0, "%s: NULL key", name);
   sh = Shape{(int)batch, (int)heads, (int)kv_heads, (int)nq, (int)nk, (int)dim, lengths, scale};
@@ -369,14 +375,17 @@ int64_t delta_bytes(int64_t rows) { return (rows * 4 + 255) / 256 * 256; }
 using namespace pmb;
 
 extern "C" int64_t pmb_cross_attention_lse_size(int64_t batch, int64_t heads, int64_t nq) {
-  return batch > 0 && heads > 0 && nq > 0 ? xattn::tc_lse_floats(batch * heads, nq) : 0;
+  return batch > 0 && heads > 0 && nq > 0 && indexable(batch, heads, nq, 0) ? xattn::tc_lse_floats(batch * heads, nq)
+                                                                            : 0;
 }
 
 namespace pmb {
 namespace {
 // Shape of a workspace query; false where the sizes make no call.
 bool query_shape(Shape& sh, int64_t batch, int64_t heads, int64_t kv_heads, int64_t nq, int64_t nk, int64_t dim) {
-  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || nq <= 0 || nk < 0 || dim <= 0) return false;
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || nq <= 0 || nk < 0 || dim <= 0 || dim > kMaxDim ||
+      !indexable(batch, heads, nq, nk))
+    return false;
   sh = Shape{(int)batch, (int)heads, (int)kv_heads, (int)nq, (int)nk, (int)dim, nullptr, 1.f};
   return true;
 }

@@ -2,7 +2,8 @@
 // 128 in multiples of 8); the formulas are at the top of cross_attention.cu.
 //
 // Rows.  Query heads that share a key / value head are packed: with gp the
-// largest power of two (up to 64) that divides the group, gp heads form a
+// largest power of two (up to 64) that divides the group (and keeps a unit
+// below 2^30 rows), gp heads form a
 // unit and row R = position * gp + head of the unit, so a few queries of many
 // heads fill a tile and each key / value head is read once for all of them.
 // A 5-D TMA map (dim, gp, positions, units, batch) loads packed tiles as they
@@ -1424,7 +1425,7 @@ int64_t round_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 // for a tile's start and end, and, with more than one range, the partial rows'
 // way out and back (about 5 GB a millisecond against 0.7 us per chunk) and the
 // second launch.
-int split_count(int64_t items, int nch, int64_t elements) {
+int split_count(int64_t items, int nch, double elements) {
   if (items == 0) return 1;
   const int64_t slots = (int64_t)num_sms() * 2;
   int best = 1;
@@ -1432,7 +1433,7 @@ int split_count(int64_t items, int nch, int64_t elements) {
   for (int s = 1; s <= kMaxSplits && (s == 1 || 2 * s <= nch); ++s) {
     const int64_t waves = (items * s + slots - 1) / slots;
     double t = (double)waves * ((nch + s - 1) / s + 2);
-    if (s > 1) t += (double)elements * s * 8 / 5e6 / 0.7 + 6.;
+    if (s > 1) t += elements * s * 8 / 5e6 / 0.7 + 6.;
     if (s == 1 || t < least) {
       least = t;
       best = s;
@@ -1453,7 +1454,8 @@ Geometry geometry(const Shape& sh) {
   Geometry g;
   const int group = sh.heads / sh.kv_heads;
   g.gp_shift = 0;
-  while (g.gp_shift < 6 && group % (2 << g.gp_shift) == 0) ++g.gp_shift;
+  while (g.gp_shift < 6 && group % (2 << g.gp_shift) == 0 && (int64_t)sh.nq << (g.gp_shift + 1) < (1 << 30))
+    ++g.gp_shift;
   g.units = sh.heads >> g.gp_shift;
   g.kv_units = group >> g.gp_shift;
   g.rows = sh.nq << g.gp_shift;
@@ -1461,7 +1463,7 @@ Geometry geometry(const Shape& sh) {
   g.nblk = (g.rows + BM - 1) / BM;
   const int nch = (sh.nk + fw::kMaxW - 1) / fw::kMaxW;
   g.width = (int)round_up((sh.nk + nch - 1) / nch, 16);
-  g.splits = split_count((int64_t)sh.batch * g.units * g.nblk, nch, (int64_t)sh.batch * g.units * g.rows * sh.dim);
+  g.splits = split_count((int64_t)sh.batch * g.units * g.nblk, nch, (double)sh.batch * g.units * g.rows * sh.dim);
   while ((int64_t)nch * g.splits >= ((int64_t)1 << 30)) --g.splits;
   g.total = 0;
   g.by_nblk = divisor(g.nblk);
@@ -1594,7 +1596,7 @@ int64_t forward_bytes(const Shape& sh, const Geometry& g) {
 
 int count_items(const Shape& sh, Geometry& g, const char* name) {
   const int64_t items = (int64_t)sh.batch * g.units * g.nblk * g.splits;
-  PMB_REQUIRE(items < ((int64_t)1 << 31) && ((int64_t)sh.nq << g.gp_shift) < (1 << 30), "%s: too many rows", name);
+  PMB_REQUIRE(items < ((int64_t)1 << 31), "%s: too many rows", name);
   g.total = (int)items;
   return PMB_OK;
 }

@@ -212,8 +212,9 @@ extern "C" int pmb_rotary_axes(const void* x, const void* positions, const float
   for (int a = axes; a < kMaxAxes; ++a) ax.end[a] = (int)end;
   PMB_REQUIRE(end <= dim / 2, "%s: sections hold %lld pairs, the head has %lld", name, (long long)end,
               (long long)(dim / 2));
-  if (batch * tokens * heads == 0) return PMB_OK;
-  PMB_REQUIRE(tokens < (1 << 30) && heads * (dim / 2) < (1 << 20), "%s: too large", name);
+  if (batch == 0 || tokens == 0 || heads == 0) return PMB_OK;
+  PMB_REQUIRE(batch < (1 << 30) && tokens < (1 << 30) && heads < (1 << 20) && heads * (dim / 2) < (1 << 20),
+              "%s: too large", name);
   PMB_REQUIRE(x && positions && freqs && y && strides, "%s: NULL argument", name);
   const View vx{strides[0], strides[1], strides[2]}, vy{strides[3], strides[4], strides[5]};
   // pairs are read and written whole: a pair is aligned to its size

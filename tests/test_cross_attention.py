@@ -136,6 +136,32 @@ def test_c_entries_refuse_bad_arguments_without_a_gpu():
     assert bwd == -5
 
 
+def test_c_entries_refuse_sizes_beyond_their_indices_without_a_gpu():
+    """Sizes whose 32-bit forms or products would wrap: 0 from the queries, an error from the entries; packed heads of
+    many queries stay inside (2^26 queries of 64 heads that share one)."""
+    lib = nat.library()
+    strides = nat.i64_array([8] * 24)
+    packed = (1, 64, 1, 2**26, 1, 8, 2)
+    assert lib.pmb_cross_attention_forward_workspace_size(*packed) == 0  # one key range
+    assert lib.pmb_cross_attention_backward_workspace_size(*packed) >= 64 * 2**26 * 4
+    for sizes in ((1, 2**32, 2**32, 1, 1), (2**32, 1, 1, 1, 1), (2**40, 2**40, 1, 1, 5), (2**15, 2**15, 1, 1, 5),
+                  (1, 1, 1, 2**30, 5), (1, 1, 1, 5, 2**32), (1, 2**31, 2**31, 2**31, 5)):
+        b, h, hk, nq, nk = sizes
+        assert lib.pmb_cross_attention_forward_workspace_size(*sizes, 8, 2) == 0
+        assert lib.pmb_cross_attention_backward_workspace_size(*sizes, 8, 2) == 0
+        assert nk == 2**32 or lib.pmb_cross_attention_lse_size(b, h, nq) == 0
+        assert lib.pmb_cross_attention_forward(16, 16, 16, 16, 16, None, *sizes, 8, strides, 1.0, 0, None, 0, 2, None,
+                                               0, None) == -1
+        assert b"too large" in lib.pmb_last_error()
+        assert lib.pmb_cross_attention_backward(16, 16, 16, 16, 16, 16, 16, 16, 16, None, *sizes, 8, strides, 1.0, 0,
+                                                None, 0, 2, None, 0, None) == -1
+        assert b"too large" in lib.pmb_last_error()
+    one = nat.i64_array([4])
+    for batch, tokens, heads in ((2**32, 2**32, 1), (1, 2**32, 2**32), (2**30, 1, 1), (1, 1, 2**62)):
+        assert lib.pmb_rotary_axes(16, 16, 16, 16, batch, tokens, heads, 8, strides, 0, 0, 1, one, 0, 2, None) == -1
+        assert b"too large" in lib.pmb_last_error()
+
+
 # ------------------------------------------------------------------ kernels
 SHAPES = [
     # b, hq, hk, nq, nk, d
