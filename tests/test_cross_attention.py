@@ -35,6 +35,11 @@ def _within(got, exact, bound, what):
     assert bool((err <= bound).all()), f"{what}: off by {worst:.3f} of the bound"
 
 
+def _splits(b, hq, hk, nq, nk, d, dtype):
+    """Whether the forward of this shape joins several key ranges."""
+    return nat.library().pmb_cross_attention_forward_workspace_size(b, hq, hk, nq, nk, d, nat.dtype_code(dtype)) > 0
+
+
 def _check(device, q, k, v, go, lengths=None, p=0.0, scale=None, lengths_dtype=torch.int32):
     dtype = q.dtype
     leaves = [t.to(device).requires_grad_() for t in (q, k, v)]
@@ -180,6 +185,34 @@ SHAPES = [
 ]
 
 
+# few row tiles over long contexts: several key ranges, joined by a second kernel
+SPLIT = [
+    # b, hq, hk, nq, nk, d, lengths
+    (3, 8, 2, 5, 3000, 64, None),
+    (3, 8, 2, 5, 3000, 64, [0, 100, 3000]),
+    (2, 4, 1, 40, 2500, 128, None),
+    (2, 4, 1, 40, 2500, 128, [1, 2499]),
+    (4, 4, 2, 6, 2500, 96, [0, 1, 100, 2500]),
+    (1, 6, 1, 130, 1111, 40, [577]),
+    (5, 2, 2, 1, 4001, 8, [4001, 0, 2, 97, 4000]),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,p", [(torch.bfloat16, 0.0), (torch.float16, 0.0), (torch.bfloat16, 0.25),
+                                     (torch.float16, 0.25)])
+@pytest.mark.parametrize("b,hq,hk,nq,nk,d,lengths", SPLIT)
+def test_joined_key_ranges_match_the_definition(cuda_device, b, hq, hk, nq, nk, d, lengths, dtype, p):
+    """Several rows, batch items, packed heads and head dims through the partial sums and their join, with ranges (and
+    whole rows) without keys; NaN and infinities behind the lengths."""
+    assert _splits(b, hq, hk, nq, nk, d, dtype)
+    q, k, v, go = _inputs(b, hq, hk, nq, nk, d, dtype)
+    for i, n in enumerate(lengths or []):
+        k[i, :, n:] = torch.nan if i % 2 else torch.inf
+        v[i, :, n:] = -torch.inf if i % 2 else torch.nan
+    _check(cuda_device, q, k, v, go, lengths, p)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("p", [0.0, 0.25])
@@ -266,10 +299,6 @@ def test_leading_scores_of_minus_infinity_weigh_nothing(cuda_device, dtype, nq):
     bounds = ref.attention_bounds(*rest, None, None, None, dtype)
     for got, e, bound, what in zip((o, dq, dk[:, :, low:], dv[:, :, low:]), exact, bounds, ("o", "dq", "dk", "dv")):
         _within(got, e, bound, what)
-
-
-def _splits(b, hq, hk, nq, nk, d, dtype):
-    return nat.library().pmb_cross_attention_forward_workspace_size(b, hq, hk, nq, nk, d, nat.dtype_code(dtype)) > 0
 
 
 # one key range per row tile, several that a second kernel joins, packed heads, a wide head, the row form

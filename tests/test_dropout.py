@@ -7,6 +7,7 @@ import torch
 
 from oracle import context_ref as ref
 from pymsst_b200 import _native as nat
+from pymsst_b200.cross_attention import cross_attention
 from pymsst_b200.dropout import DropoutGenerator, drop_threshold, dropout, gelu_dropout
 
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -27,6 +28,22 @@ def test_bits_are_uniform_and_tell_sites_and_steps_apart():
     for seed, step, site in ((6, 9, 2), (5, 10, 2), (5, 9, 3), (5 + (1 << 40), 9, 2)):
         other = ref.philox16(g, 0, 0xFFFFFFFF, seed, step, site).reshape(-1)
         assert (base == other).sum() < 40
+
+
+# Philox4x32 with seven rounds, the known answers that its authors published with it: counter words, key words, result
+# words.
+KNOWN = [
+    ((0, 0, 0, 0), (0, 0), (0x5F6FB709, 0x0D893F64, 0x4F121F81, 0x4F730A48)),
+    ((0xFFFFFFFF,) * 4, (0xFFFFFFFF,) * 2, (0x5207DDC2, 0x45165E59, 0x4D8EE751, 0x8C52F662)),
+    ((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0),
+     (0x4DFCCABA, 0x190A87F0, 0xC47362BA, 0xB6B5242A)),
+]
+
+
+@pytest.mark.parametrize("counter,key,words", KNOWN)
+def test_bits_are_the_published_generators(counter, key, words):
+    got = ref.philox16(*counter[:3], key[0] | (key[1] << 32), counter[3], 0).tolist()
+    assert got == [half for w in words for half in (w & 0xFFFF, w >> 16)]
 
 
 def test_multiplier_keeps_the_mean():
@@ -144,6 +161,23 @@ def test_gelu_dropout(cuda_device, dtype, rows, cols, p):
         slack_g = mult * gy.double().abs() * (2.0**-14 * (cdf + (x64 * pdf).abs()) + (x64 < -5.5) * 2.0**-25)
     _close(y.detach(), exact, _bound(dtype, exact, exact.abs()) + slack)
     _close(gx, exact_g, _bound(dtype, exact_g, exact_g.abs()) + slack_g)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_kernel_bits_are_the_published_generators(cuda_device, dtype):
+    """Eight keys of the first query, head and batch item, seed, step and site 0: the zero counter under the zero key.
+    Each of its eight numbers u keeps its key at a threshold of u and drops it at u + 1.  Scores of zero and the
+    identity as values show the kept ones."""
+    words = KNOWN[0][2]
+    numbers = [half for w in words for half in (w & 0xFFFF, w >> 16)]
+    q, k = torch.zeros(1, 1, 1, 8, device=cuda_device, dtype=dtype), torch.zeros(1, 1, 8, 8, device=cuda_device, dtype=dtype)
+    v = torch.eye(8, device=cuda_device, dtype=dtype).reshape(1, 1, 8, 8)
+    key = _key(0, 0, cuda_device)
+    for u in numbers:
+        for threshold in (u, u + 1):
+            o = cross_attention(q, k, v, dropout_p=threshold / 65536, key=key)
+            assert (o.flatten() != 0).tolist() == [n >= threshold for n in numbers]
 
 
 @pytest.mark.gpu
