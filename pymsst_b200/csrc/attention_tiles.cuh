@@ -108,19 +108,6 @@ __device__ __forceinline__ void tmem_wait16(uint32_t (&a)[16], uint32_t (&b)[16]
   tie16(b);
 }
 
-// 8 columns of this warp's TMEM lane quarter, without waiting (see tmem_wait8).
-__device__ __forceinline__ void tmem_ld8_nowait(uint32_t taddr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr));
-}
-
-__device__ __forceinline__ void tmem_wait8(uint32_t (&a)[8], uint32_t (&b)[8]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-  asm volatile("" : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]), "+r"(a[6]), "+r"(a[7]));
-  asm volatile("" : "+r"(b[0]), "+r"(b[1]), "+r"(b[2]), "+r"(b[3]), "+r"(b[4]), "+r"(b[5]), "+r"(b[6]), "+r"(b[7]));
-}
-
 // 16 fp32 values -> chunks c0, c0 + 1 of row r of a 16-bit SW128 tile
 template <typename T>
 __device__ __forceinline__ void put_row16(uint8_t* tile, int r, int c0, const float* v) {
