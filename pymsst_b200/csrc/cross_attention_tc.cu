@@ -169,7 +169,9 @@ __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.
 // previous product to release P, 360 fences.
 //
 // O stays in tensor memory; the running maximum moves only when a row's grows
-// by more than 8 (a factor 256 in P, harmless in fp32 sums and 16-bit P),
+// by more than 8 (a factor 256 in P, harmless in fp32 sums and 16-bit P; a
+// known step of published attention kernels, as is sharing the exponentials
+// between the two pipes),
 // which after the first chunks is rare, and then the row threads rescale O
 // themselves.  P is rounded to the input type (as in attention.cu); the row
 // sums add the unrounded values before dropout, whose scale is applied once
@@ -222,9 +224,10 @@ __device__ __forceinline__ float max32(const uint32_t (&s)[32], float mx) {
 }
 
 // 2^a and 2^b for a, b <= 127 on the FMA pipe, relative error 2^-22.5: n = round(x) falls out of the addition of 1.5
-// 2^23, and 2^(x - n) on [-1/2, 1/2] is a degree-five polynomial (least maximum relative error with the constant term
-// fixed at 1, fitted by reweighted least squares).  Powers below 2^-127 become 2^-127, whose exponent bits are those
-// of zero, so masked scores give exactly 0; NaN passes through the maximum and the product.
+// 2^23 (range reduction as in Cody and Waite, 1980), and 2^(x - n) on [-1/2, 1/2] is a degree-five polynomial with the
+// constant term 1 (pymsst_b200/exp2_fit.py fits it and emulates this arithmetic).  Powers below 2^-127 become 2^-127,
+// whose exponent bits are those of zero, so masked scores give exactly 0; NaN passes through the maximum and the
+// product.
 __device__ __forceinline__ void exp2_pair(float& a, float& b) {
   constexpr float kRound = 12582912.f;
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-127.f));
