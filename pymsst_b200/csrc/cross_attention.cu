@@ -186,11 +186,14 @@ __global__ void __launch_bounds__(kThreads)
     const int r = i0 + warp * kOwn + i;
     if (r >= sh.nq) break;
     T* out = o + b * po.s_b + r * po.s_n + h * po.s_h;
-    const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];  // no keys, or scores of -infinity alone
+    // no keys, or scores of -infinity alone: zeros.  (A sum without keys is 0 too; with the length in the test the
+    // compiler stays at 128 registers and four CTAs an SM, without it at 139 and three: 0.58 against 0.67 ms.)
+    const bool some = len > 0 && l[i] != 0.f;
+    const float inv = some ? 1.f / l[i] : 0.f;
 #pragma unroll
     for (int a = 0; a < NA; ++a)
       if (lane + 32 * a < sh.dim) out[lane + 32 * a] = Elem<T>::from_f(acc[i][a] * inv);
-    if (lane == 0) lse[(int64_t)bh * sh.nq + r] = l[i] == 0.f ? INFINITY : m[i] + logf(l[i]);
+    if (lane == 0) lse[(int64_t)bh * sh.nq + r] = some ? m[i] + logf(l[i]) : INFINITY;
   }
 }
 
