@@ -17,13 +17,13 @@
 // tiles of 32 rows of the other side come through shared memory for the four
 // warps of a CTA.  For the dot products a lane takes one row of the tile and
 // multiplies it with the eight owned rows, which all lanes read alike; for the
-// sums a lane takes every 32nd head element.  Bound by shared-memory reads
-// (9 of 16 bytes for 32 fused multiply-adds).  Measured for 62 x 8 heads x 258
-// x 258, dim 64, fp32 with dropout: forward 0.58, dQ 0.87, dK / dV 0.92 ms,
-// where a warp to one row without tiles took 10.7, 16.2 and 17.0 ms.
-// Every output row is summed by
-// one warp in the order of the tiles, so results do not depend on the order of
-// execution.
+// sums a lane takes every 32nd head element.  Nearest limit: shared-memory
+// reads (9 of 16 bytes for 32 fused multiply-adds; ncu: 59 to 67 % of the
+// wavefronts, 0.59 to 0.68 of the issue slots, at three to four CTAs an SM).  Measured
+// for 62 x 8 heads x 258 x 258, dim 64, fp32 with dropout: forward 0.58, dQ
+// 0.87, dK / dV 0.92 ms, where a warp to one row without tiles took 10.7, 16.2
+// and 17.0 ms.  Every output row is summed by one warp in the order of the
+// tiles, so results do not depend on the order of execution.
 #include "cross_attention.cuh"
 
 namespace pmb {

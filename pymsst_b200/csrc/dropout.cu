@@ -7,13 +7,15 @@
 // or NaN under the mask does not reach y.  Computed in fp32 and rounded once.
 //
 // One thread takes groups of eight consecutive elements: one Philox call, and
-// for 16-bit types one 16-byte vector per tensor.  Bound by HBM: nothing but
-// the tensors themselves moves (a stored mask would add a byte per element to
-// both passes).  One group per thread: many small CTAs keep more loads in
-// flight than a loop does (the residual form over 63,984 x 192 bf16 takes
-// 16.3 us so, 20.7 with two groups per thread, 22.4 in a loop that loads one
-// group ahead; floor 11.4).  The GELU forms are bound by instruction issue:
-// 62 and 75 us for 63,984 x 768 bf16, floors 30.5 and 45.7.
+// for 16-bit types one 16-byte vector per tensor.  Nothing but the tensors
+// themselves moves (a stored mask would add a byte per element to both
+// passes).  One group per thread: many small CTAs keep more loads in flight
+// than a loop does (the residual form over 63,984 x 192 bf16 takes 16.4 us so,
+// 20.7 with two groups per thread, 22.4 in a loop that loads one group ahead;
+// floor 11.4, its backward 13.0, floor 7.6: kernels so short are bound by their
+// ramp and the latency of the loads behind it).  The GELU forms are bound by
+// instruction issue (ncu: 0.74 of the slots, FMA pipe 55 %, HBM 29 to 42 %): 62
+// and 75 us for 63,984 x 768 bf16, floors 30.5 and 45.7.
 #include "common.cuh"
 #include "gelu.cuh"
 #include "philox.cuh"

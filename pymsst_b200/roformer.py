@@ -220,7 +220,8 @@ class Attention(nn.Module):
 
     def set_cuda_attention_backend(self, backend: str) -> None:
         """Attention kernel choice, the hook the reference's training module calls on every module
-        (src/pymsst/training/module.py:416-425); one of ATTENTION_BACKENDS."""
+        (src/pymsst/training/module.py:416-425); one of ATTENTION_BACKENDS.  Live dropout from a dropout generator is
+        drawn inside the package's own kernels and does not look at it."""
         name = str(backend).strip().lower()
         if name not in ATTENTION_BACKENDS:
             raise ValueError(f"unknown cuda attention backend {backend!r}; expected one of {ATTENTION_BACKENDS}")
@@ -453,7 +454,9 @@ class _Roformer(nn.Module):
         """Take live dropout (attn_dropout / ff_dropout in training) from ``generator``, or, with None, from torch's
         as before.  Every dropout of the model gets a site of its own and each forward one key, so a recomputed
         transformer (use_torch_checkpoint) draws the same masks, in a captured step too, where every replay draws new
-        ones.  Data-parallel ranks need generators of different seeds.  CUDA only."""
+        ones.  A Trainer's captured step follows an exchange by capturing again; a graph captured by hand stays with
+        the generator it was captured with.  Attention with live dropout then runs on the package's kernels, whatever
+        set_cuda_attention_backend chose.  Data-parallel ranks need generators of different seeds.  CUDA only."""
         site = 0
         for module in self.modules():
             if isinstance(module, (Attention, FeedForward)):
