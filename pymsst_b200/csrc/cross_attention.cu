@@ -3,7 +3,7 @@
 // on the probabilities from counter-based bits (philox.cuh):
 //
 //   P = softmax_rows(scale Q K^T over keys < len),  Pd = keep c P,  O = Pd V
-//   D = rowsum(dO * O) (= rowsum(P dP)),  dP = keep c (dO V^T),
+//   D = rowsum(P dP) (= rowsum(dO * O), the form for more than one tile of keys),  dP = keep c (dO V^T),
 //   dS = P (dP - D),  dV = Pd^T dO,  dQ = scale dS K,  dK = scale dS^T Q
 //
 // dK and dV sum over the query heads of a group.  A row without keys, or with
@@ -24,6 +24,8 @@
 // 0.87, dK / dV 0.92 ms, where a warp to one row without tiles took 10.7, 16.2
 // and 17.0 ms.  Every output row is summed by one warp in the order of the
 // tiles, so results do not depend on the order of execution.
+#include <type_traits>
+
 #include "cross_attention.cuh"
 
 namespace pmb {
@@ -197,7 +199,8 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-template <typename T, bool DROP, int NA>
+// ONE: at most one tile of keys, D = rowsum(P dP) from it; O's rounding, which few keys do not average out, stays away.
+template <typename T, bool DROP, int NA, bool ONE>
 __global__ void __launch_bounds__(kThreads)
     attn_rows_dq(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ o,
                  const T* __restrict__ go, const float* __restrict__ lse, T* __restrict__ gq,
@@ -217,14 +220,14 @@ __global__ void __launch_bounds__(kThreads)
   for (int i = 0; i < kOwn; ++i) {
     const int r = i0 + warp * kOwn + i;
     float x = 0.f;
-    if (r < sh.nq) {
+    if (!ONE && r < sh.nq) {
       const T* orow = o + b * po.s_b + r * po.s_n + h * po.s_h;
       for (int c = lane; c < sh.dim; c += 32)
         x = fmaf(m_.ob[(warp * kOwn + i) * own + c], Elem<T>::to_f(orow[c]), x);
     }
-    d[i] = warp_sum(x);
+    d[i] = ONE ? 0.f : warp_sum(x);
     ls[i] = r < sh.nq ? lse[(int64_t)bh * sh.nq + r] : 0.f;
-    if (r < sh.nq && lane == 0) delta[(int64_t)bh * sh.nq + r] = d[i];
+    if (!ONE && r < sh.nq && lane == 0) delta[(int64_t)bh * sh.nq + r] = d[i];
   }
   k += b * pk.s_b + kh * pk.s_h;
   v += b * pv.s_b + kh * pv.s_h;
@@ -243,7 +246,13 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       if (DROP) dp[i] = kept_key(bits, i) ? dp[i] * drop.scale : 0.f;
-      p[i] = lane < count ? expf(p[i] - ls[i]) * (dp[i] - d[i]) : 0.f;
+      if constexpr (ONE) {
+        const float e = lane < count ? expf(p[i] - ls[i]) : 0.f;
+        d[i] = warp_sum(lane < count ? e * dp[i] : 0.f);
+        p[i] = lane < count ? e * (dp[i] - d[i]) : 0.f;
+      } else {
+        p[i] = lane < count ? expf(p[i] - ls[i]) * (dp[i] - d[i]) : 0.f;
+      }
     }
     put_weights(w, p);
     __syncwarp();
@@ -258,6 +267,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int a = 0; a < NA; ++a)
       if (lane + 32 * a < sh.dim) out[lane + 32 * a] = Elem<T>::from_f(acc[i][a] * sh.scale);
+    if (ONE && lane == 0) delta[(int64_t)bh * sh.nq + r] = d[i];
   }
 }
 
@@ -492,9 +502,12 @@ extern "C" int pmb_cross_attention_backward(const void* q, const void* k, const 
                          static_cast<T*>(grad_k), static_cast<T*>(grad_v), pq, pk, pv, pgo, pgk, pgv, sh, kblocks, drop);
     };
     if (rows > 0) {
-      const int st = dim <= 64 ? (threshold > 0 ? run_q(attn_rows_dq<T, true, 2>) : run_q(attn_rows_dq<T, false, 2>))
-                               : (threshold > 0 ? run_q(attn_rows_dq<T, true, 8>) : run_q(attn_rows_dq<T, false, 8>));
-      if (st) return st;
+      auto pick = [&](auto one) {
+        constexpr bool ONE = decltype(one)::value;
+        return dim <= 64 ? (threshold > 0 ? run_q(attn_rows_dq<T, true, 2, ONE>) : run_q(attn_rows_dq<T, false, 2, ONE>))
+                         : (threshold > 0 ? run_q(attn_rows_dq<T, true, 8, ONE>) : run_q(attn_rows_dq<T, false, 8, ONE>));
+      };
+      if (const int st = nk <= kTile ? pick(std::true_type{}) : pick(std::false_type{})) return st;
     }
     if (keys == 0) return PMB_OK;
     return dim <= 64 ? (threshold > 0 ? run_k(attn_rows_dkdv<T, true, 2>) : run_k(attn_rows_dkdv<T, false, 2>))

@@ -701,6 +701,15 @@ constexpr int G = 2;                   // groups of row warps
 // of the groups, from tiles (O's rows read from global memory took a group
 // 3000 cycles per item), and keeps it for the dK / dV kernel; the group with
 // an item's last chunk writes dQ.
+//
+// With ONE, at most one chunk of keys in all, the group forms D = rowsum(P dP)
+// itself before it uses the scores.  O is rounded, and what that leaves in D is
+// the same for all keys of a row: many keys average it out, few do not (errors
+// of dQ and dK against 64 bits, in units of fp32 arithmetic with one rounding:
+// 2.3 for two keys, 1.75 for four, 1.5 for 20, 1.45 for 100 and for all lengths
+// with D so formed, where dS rounded to 16 bits is what remains).  A kernel of
+// its own, as the longer form's registers would not hold it: decided within one
+// kernel it cost the time axis with dropout 191 -> 234 us.
 namespace bq {
 constexpr int kThreads = 128 + 128 * bw::G;  // one more control warp, for D
 template <int DC>
@@ -754,7 +763,7 @@ struct QueryCursor {
   __device__ __forceinline__ int keys() const { return min(bw::BC, len - c * bw::BC); }
 };
 
-template <typename T, int DC, bool DROP>
+template <typename T, int DC, bool DROP, bool ONE>
 __global__ void __launch_bounds__(bq::kThreads, 1)
     xattn_bwd_dq(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
                  const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmK,
@@ -917,7 +926,7 @@ __global__ void __launch_bounds__(bq::kThreads, 1)
       const uint8_t* go = smem + qd.s * Y::TILES + DC * TILE;
       float nd[4] = {0.f, 0.f, 0.f, 0.f};  // four rows at a time hide one another's latencies
 #pragma unroll 2
-      for (int c = 0; c < 8 * DC; ++c) {
+      for (int c = ONE ? 8 * DC : 0; c < 8 * DC; ++c) {
         uint4 o4[4], d4[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -935,7 +944,7 @@ __global__ void __launch_bounds__(bq::kThreads, 1)
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (lane + 32 * i < rows) delta[stat + 32 * i] = nd[i];
+        if (!ONE && lane + 32 * i < rows) delta[stat + 32 * i] = nd[i];
         nd_s[turn.s * 128 + lane + 32 * i] = nd[i];
         nl_s[turn.s * 128 + lane + 32 * i] = nlse[i];
       }
@@ -1002,17 +1011,46 @@ __global__ void __launch_bounds__(bq::kThreads, 1)
         const int keys = cu.keys();
         if (!idle) {
           const uint32_t bh = (uint32_t)(it.b * sh.heads + head);
+          uint64_t bits = ~0ull;  // of all keys, when they are one chunk
+          if constexpr (ONE) {
+            if (DROP) bits = 0;
+            float sum = 0.f;
+#pragma unroll 1
+            for (int first = 0; first < keys; first += 16) {
+              uint32_t su[16], du[16];
+              tmem_ld16_nowait(acc + first, su);
+              tmem_ld16_nowait(acc + 64 + first, du);
+              if (DROP) {
+                const uint32_t low = keep_bits(rng((uint32_t)first / 8, (uint32_t)pos, bh), drop.limit);
+                const uint32_t high = keep_bits(rng((uint32_t)first / 8 + 1, (uint32_t)pos, bh), drop.limit);
+                bits |= (uint64_t)(low | (high << 8)) << first;
+              }
+              const uint32_t live = (uint32_t)(bits >> first) & (0xffffffffu >> (32 - min(16, keys - first)));
+              tmem_wait16(su, du);
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) {
+                float p0, p1;
+                unpk2(fma2(pk2(__uint_as_float(su[i]), __uint_as_float(su[i + 1])), sl22, nlse2), p0, p1);
+                sum += (live >> i) & 1u ? ex2(p0) * __uint_as_float(du[i]) : 0.f;
+                sum += (live >> (i + 1)) & 1u ? ex2(p1) * __uint_as_float(du[i + 1]) : 0.f;
+              }
+            }
+            const float nd = -mult * sum;
+            nd2 = pk2(nd, nd);
+            if (valid) delta[(int64_t)(it.b * g.units + it.u) * g.ldr + R] = nd;
+          }
 #pragma unroll 1
           for (int first = 0; first < keys; first += 32) {
             uint32_t su[32], du[32];
             tmem_ld32_nowait(acc + first, su);
             tmem_ld32_nowait(acc + 64 + first, du);
             tmem_wait2(su, du);
+            const uint32_t now = (uint32_t)(bits >> first);
             uint32_t p2[16];
 #pragma unroll
             for (int q8 = 0; q8 < 4; ++q8) {
               uint4 r = make_uint4(0, 0, 0, 0);
-              if (DROP) r = rng((uint32_t)(cu.c * BC + first) / 8 + q8, (uint32_t)pos, bh);
+              if (DROP && !ONE) r = rng((uint32_t)(cu.c * BC + first) / 8 + q8, (uint32_t)pos, bh);
               const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
@@ -1021,8 +1059,8 @@ __global__ void __launch_bounds__(bq::kThreads, 1)
                 unpk2(fma2(pk2(__uint_as_float(su[2 * i]), __uint_as_float(su[2 * i + 1])), sl22, nlse2), p0, p1);
                 uint64_t x;
                 if (DROP) {
-                  d0 = kept(w[e], 0, drop.high) ? d0 : 0.f;
-                  d1 = kept(w[e], 1, drop.high) ? d1 : 0.f;
+                  d0 = (ONE ? (now >> (2 * i)) & 1u : kept(w[e], 0, drop.high)) ? d0 : 0.f;
+                  d1 = (ONE ? (now >> (2 * i + 1)) & 1u : kept(w[e], 1, drop.high)) ? d1 : 0.f;
                   x = fma2(pk2(d0, d1), mult2, nd2);
                 } else {
                   x = add2(pk2(d0, d1), nd2);
@@ -1566,7 +1604,7 @@ int backward_launch(const Shape& sh, const Backward& a, Geometry g, const char* 
   if (int st = key_map(v128, a.v, a.pv, sh, a.dtype, BM, name)) return st;
   float* delta = static_cast<float*>(a.workspace);
   {
-    auto kernel = xattn_bwd_dq<T, DC, DROP>;
+    auto kernel = sh.nk <= bw::BC ? xattn_bwd_dq<T, DC, DROP, true> : xattn_bwd_dq<T, DC, DROP, false>;
     constexpr int smem = bq::L<DC>::SMEM;
     PMB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), name);
     kernel<<<persistent_grid(g.total, 1), bq::kThreads, smem, a.stream>>>(

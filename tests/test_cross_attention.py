@@ -519,3 +519,65 @@ def test_captured_forward_and_backward_replay(cuda_device):
         torch.cuda.synchronize()
         replayed = [t.clone() for t in out]
         assert all(torch.equal(x, y) for x, y in zip(replayed, step()))
+
+
+def _bounds_with_exact_row_sums(q, k, v, go, lengths, mult, dtype):
+    """Bounds of dq and dk where D = rowsum(P dP) comes from the unrounded probabilities, term by term as in
+    attention_bounds, with e_dP = 2 (d + 16) 2^-24 |dO| |V|^T mult (d fp32 products and sums, truncated ones too):
+      D:  P (e_dP + (e_p + nk 2^-24) |dP|), summed;
+      dS: (u + e_p) |dS| + P (error of D + e_dP + 2^-22 (|dP| + |D|)) + tiny."""
+    u = torch.finfo(dtype).eps / 2
+    tiny = torch.finfo(dtype).smallest_normal * u
+    b, hq, nq, d = q.shape
+    hk, nk = k.shape[1], k.shape[2]
+    scale = d**-0.5
+    p, live = ref.probabilities(q, k, lengths, scale)
+    zero = torch.zeros((), dtype=q.dtype)
+    kr, vr = (torch.where(live.transpose(-1, -2), t.repeat_interleave(hq // hk, dim=1), zero) for t in (k, v))
+    mult = torch.ones((), dtype=q.dtype) if mult is None else mult
+    ep = 2 * ((d + 16) * 2.0**-24 * scale * (q.abs() @ kr.abs().transpose(-1, -2))).amax(-1, keepdim=True) + 2.0**-19
+    e_dp = 2 * (d + 16) * 2.0**-24 * (go.abs() @ vr.abs().transpose(-1, -2)) * mult
+    dp = (go @ vr.transpose(-1, -2)) * mult
+    row = (p * dp).sum(-1, keepdim=True)
+    ds = p * (dp - row)
+    e_d = (p * (e_dp + (ep + nk * 2.0**-24) * dp.abs())).sum(-1, keepdim=True)
+    e_ds = (u + ep) * ds.abs() + p * (e_d + e_dp + 2.0**-22 * (dp.abs() + row.abs())) + tiny * live
+    dq, dk, _ = ref.attention_grads(q, k, v, go, lengths, None, mult)
+    e_dk = (e_ds.transpose(-1, -2) @ q.abs()).reshape(b, hk, hq // hk, nk, d).sum(2)
+    return tuple(u * g.abs() + tiny + scale * e * (1 + 2.0**-10) for g, e in ((dq, e_ds @ kr.abs()), (dk, e_dk)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("p", [0.0, 0.3])
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.float16, 128), (torch.bfloat16, 33),
+                                     (torch.float16, 200), (torch.float32, 48)])
+@pytest.mark.parametrize("nk,lengths", [(1, None), (2, None), (5, None), (17, [17, 1, 0]), (32, [2, 32, 31])])
+def test_few_keys_keep_the_rounding_of_the_output_out_of_their_gradients(cuda_device, nk, lengths, dtype, d, p):
+    """dS = P (dP - D) cancels, most of all where few keys share a row's weight (one key: dS = 0); D from the rounded
+    output would leave 2^-9 |dO| |O| of bf16 there.  The tensor-core form's border of 64 keys is the next test's."""
+    b = 3
+    q, k, v, go = _inputs(b, 4, 2, 37, nk, d, dtype)
+    leaves = [t.to(cuda_device).requires_grad_() for t in (q, k, v)]
+    dev_len = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=cuda_device)
+    key = _key(cuda_device) if p > 0 else None
+    o = cross_attention(*leaves, key_lengths=dev_len, dropout_p=p, key=key, site=SITE)
+    dq, dk, _ = torch.autograd.grad(o, leaves, go.to(cuda_device))
+    wide = [t.double() for t in (q, k, v, go)]
+    mult = _mult(q, k, p)
+    eq, ek, _ = ref.attention_grads(*wide, lengths, None, mult)
+    bq, bk = _bounds_with_exact_row_sums(*wide, lengths, mult, dtype)
+    _within(dq, eq, bq, "dq")
+    _within(dk, ek, bk, "dk")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("p", [0.0, 0.3])
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.float16, 72), (torch.bfloat16, 136), (torch.float32, 64)])
+@pytest.mark.parametrize("nk", [31, 32, 33, 48, 63, 64, 65])
+def test_borders_of_the_forms_for_few_keys(cuda_device, nk, dtype, d, p):
+    """Every length behind the borders at a tile of the row form and a chunk of the tensor-core form, several query
+    tiles, packed heads, ragged batches."""
+    q, k, v, go = _inputs(5, 4, 2, 150, nk, d, dtype)
+    _check(cuda_device, q, k, v, go, [nk, 0, 1, nk - 1, nk // 2], p)
+    if dtype != torch.float32 and d <= 128 and nk <= 64:
+        test_few_keys_keep_the_rounding_of_the_output_out_of_their_gradients(cuda_device, nk, [nk, 3, nk - 1], dtype, d, p)
